@@ -1,0 +1,385 @@
+"""Performance cases of the 8-bit paged KV-cache operators and of windowed attention with sinks.
+
+Five operators, on the geometry of the library (16 query heads, 4 KV heads, head dim 128):
+
+  append         RMSNorm + RoPE of q and k, quantising append of k and v to 8-bit blocks (KvPath.append_q8)
+  decode         one token per sequence over the 8-bit cache (KvPath.decode_attn_q8)
+  prefill        the rows of a prompt wave over the 8-bit cache (KvPath.prefill_attn_q8)
+  decode_sinks   one token per sequence over an f16 cache, sliding window and sinks (KvPath.decode_attn_sinks, ..._paged_sinks)
+  prefill_sinks  the rows of a prompt wave, the same (KvPath.prefill_attn_sinks, ..._paged_sinks)
+
+A block of the 8-bit cache holds `bs` tokens x 4 KV heads x 128 codes, with one f32 scale per KV head for K and one for V.
+Where `own` is false `run` computes the plain form in torch; where it is true it calls the library."""
+import math
+
+import torch
+
+own = False
+
+NQ, NKV, GRP, HD = 16, 4, 4, 128
+EPS = 1e-5
+FMT_MAX = {"int8": 127.0, "e4m3": 448.0}
+CODE = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+
+
+# ---------------------------------------------------------------------------------------------- cases
+def listed():
+    return [
+        # one generated token for each of 128 sequences, wherever in its block it falls
+        dict(name="append_step_e4m3", op="append", fmt="e4m3", nseq=128, lo=100, hi=500, rlo=1, rhi=1, bs=16),
+        # a full prefill wave of 32 chunks of 128 rows
+        dict(name="append_wave_e4m3", op="append", fmt="e4m3", nseq=32, lo=0, hi=0, rlo=128, rhi=128, bs=16),
+        # chunks of odd lengths that begin inside a block, blocks of 64
+        dict(name="append_ragged_int8", op="append", fmt="int8", nseq=9, lo=5, hi=300, rlo=33, rhi=97, bs=64),
+        # a single conversation: the smallest call, all latency
+        dict(name="decode_one_int8", op="decode", fmt="int8", nseq=1, lo=512, hi=512, bs=16, window=0, sinks=0),
+        # the decode step of a full batch at 4,096 keys
+        dict(name="decode_full_int8", op="decode", fmt="int8", nseq=128, lo=4096, hi=4096, bs=16, window=0, sinks=0),
+        # long contexts of odd lengths under a sliding window with sinks, blocks of 64
+        dict(name="decode_window_e4m3", op="decode", fmt="e4m3", nseq=48, lo=700, hi=16001, bs=64, window=1024, sinks=4),
+        # a full prefill wave on prefixes of up to 8,192 keys
+        dict(name="prefill_wave_int8", op="prefill", fmt="int8", nseq=32, lo=0, hi=8192, rlo=128, rhi=128, bs=16, window=0, sinks=0),
+        # a few ragged chunks, window and sinks
+        dict(name="prefill_ragged_e4m3", op="prefill", fmt="e4m3", nseq=5, lo=17, hi=2500, rlo=40, rhi=128, bs=32, window=512, sinks=7),
+        # the decode step of a full batch, 4,096 keys visible of up to 20,000
+        dict(name="decode_sinks_full", op="decode_sinks", paged=False, nseq=128, lo=3000, hi=20000, window=4096, sinks=4),
+        # a small batch on the paged f16 layout with a short window
+        dict(name="decode_sinks_paged", op="decode_sinks", paged=True, nseq=8, lo=200, hi=3001, bs=16, window=256, sinks=5),
+        # a full wave deep in long prompts, each row sees 1,024 keys and the sinks
+        dict(name="prefill_sinks_wave", op="prefill_sinks", paged=False, nseq=32, lo=0, hi=8192, rlo=128, rhi=128, window=1024, sinks=4),
+        # ragged chunks on the paged f16 layout, a window shorter than a chunk
+        dict(name="prefill_sinks_paged", op="prefill_sinks", paged=True, nseq=6, lo=3, hi=1500, rlo=21, rhi=128, bs=64, window=100, sinks=70),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(["append", "decode", "decode", "prefill", "prefill", "decode_sinks", "prefill_sinks"])
+    fmt, bs = rng.choice(["int8", "e4m3"]), rng.choice([16, 32, 64, 128, 256])
+    window = 0 if rng.random() < 0.4 else _log_int(rng, 1, 5000)
+    sinks = 0 if rng.random() < 0.4 else _log_int(rng, 1, 200)
+    if op == "append":
+        nseq = _log_int(rng, 1, 128)
+        rhi = 1 if rng.random() < 0.4 else _log_int(rng, 1, min(128, 4096 // nseq))
+        lo = rng.randint(0, 100)
+        return dict(op=op, fmt=fmt, nseq=nseq, lo=lo, hi=lo + rng.randint(0, 300), rlo=max(1, rhi // 2), rhi=rhi, bs=bs)
+    if op in ("decode", "decode_sinks"):
+        nseq = _log_int(rng, 1, 128)
+        hi = _log_int(rng, 1, min(30000, 128 * 4096 // nseq))
+        c = dict(op=op, nseq=nseq, lo=max(1, int(hi * rng.random())), hi=hi)
+    else:
+        nseq = _log_int(rng, 1, 32)
+        rhi = _log_int(rng, 1, 128)
+        c = dict(op=op, nseq=nseq, lo=rng.randint(0, 500), hi=500 + _log_int(rng, 1, 7000), rlo=max(1, rhi // 2), rhi=rhi)
+    if op in ("decode", "prefill"):
+        return dict(c, fmt=fmt, bs=bs, window=window, sinks=sinks)
+    return dict(c, paged=rng.random() < 0.5, bs=bs, window=max(1, window), sinks=max(1, sinks))
+
+
+# ---------------------------------------------------------------------------------------------- lengths (from the case alone)
+def _spread(n, lo, hi):
+    """n whole numbers in [lo, hi], scattered and the same each time."""
+    return [lo + int((hi - lo) * ((i * 0.6180339887498949 + 0.371) % 1.0) + 0.5) for i in range(n)]
+
+
+def _shape(case):
+    """Per sequence: tokens in the cache before the call's rows, and the call's rows (decode: the one row is in the cache already)."""
+    n = case["nseq"]
+    if case["op"] in ("decode", "decode_sinks"):
+        return [x - 1 for x in _spread(n, case["lo"], case["hi"])], [1] * n
+    return _spread(n, case["lo"], case["hi"]), _spread(n, case["rlo"], case["rhi"])
+
+
+def _visible(length, window, sinks):
+    start = length - window if window and length > window else 0
+    return length - start + min(sinks, start)
+
+
+def work(case):
+    before, rows = _shape(case)
+    total = sum(rows)
+    if case["op"] == "append":
+        blocks = sum((b + r - 1) // case["bs"] - b // case["bs"] + 1 for b, r in zip(before, rows))
+        return {"bytes": total * (2 * NQ * HD * 2 + 2 * NKV * HD * 2 + 2 * NKV * HD) + blocks * 32, "flops": total * (NQ + NKV) * HD * 8}
+    w, k = case["window"], case["sinks"]
+    pairs = sum(_visible(b + i + 1, w, k) for b, r in zip(before, rows) for i in range(r))
+    read = 0  # keys that some row of the sequence sees
+    for b, r in zip(before, rows):
+        first = max(0, b + 1 - w) if w else 0
+        read += b + r - first + min(k, first)
+    per_key = 2 * NKV * HD + (32 / case["bs"]) if case["op"] in ("decode", "prefill") else 2 * NKV * HD * 2
+    return {"bytes": int(read * per_key) + total * (2 * NQ * HD * 2 + NQ * 2), "flops": pairs * 4 * NQ * HD}
+
+
+# ---------------------------------------------------------------------------------------------- inputs
+def _quantised(x, fmt):
+    """Codes and scales of whole blocks x [blocks][bs][4][128] f32."""
+    amax = x.abs().amax(dim=(1, 3))
+    s = _scale_of(amax, fmt)
+    y = x / torch.where(s > 0, s, torch.ones_like(s))[:, None, :, None]
+    return (torch.round(y).clamp_(-127, 127).to(torch.int8) if fmt == "int8" else y.clamp_(-448, 448).to(torch.float8_e4m3fn)), s
+
+
+def _scale_of(amax, fmt):
+    if fmt == "int8":
+        return amax / 127.0
+    m, e = torch.frexp(amax / 448.0)
+    return torch.where(amax > 0, torch.ldexp(torch.ones_like(amax), torch.where(m > 0.5, e, e - 1)), torch.zeros_like(amax))
+
+
+def prepare(case, seed):
+    dev = "cuda"
+    g = torch.Generator(device=dev).manual_seed(int(seed) * 7919 + 13)
+    randn = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+    before, rows = _shape(case)
+    n, total = case["nseq"], sum(rows)
+    lens = [b + r for b, r in zip(before, rows)]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    s = {"case": case, "n": n, "total": total, "rmax": max(rows), "lmax": max(lens)}
+    s["row_seq"] = i32([i for i in range(n) for _ in range(rows[i])])
+    s["pos"] = i32([before[i] + j for i in range(n) for j in range(rows[i])])
+    s["seq_lens"] = s["pos"] + 1
+    s["first_row"] = i32([sum(rows[:i]) for i in range(n)])  # where a sequence's rows begin
+    s["nrows"], s["before"] = i32(rows), i32(before)
+    bs = case.get("bs", 0)
+    paged = case["op"] in ("append", "decode", "prefill") or case.get("paged")
+    if paged:
+        need = [(x + bs - 1) // bs for x in lens]
+        nblocks = sum(need) + 2
+        perm = torch.randperm(nblocks, generator=g, device=dev).to(torch.int32)
+        ends = torch.cumsum(torch.tensor(need), 0).tolist()
+        tables = torch.zeros(n, max(need) + 1, dtype=torch.int32, device=dev)
+        for i in range(n):
+            tables[i, :need[i]] = perm[ends[i] - need[i]:ends[i]]
+        s["tables"] = tables
+    s["q"] = (randn(total, NQ, HD) * 1.3).half()
+    s["gate"] = randn(total, NQ).half()
+    s["ctx"] = torch.zeros(total, NQ, HD, dtype=torch.float16, device=dev)
+    op = case["op"]
+    if op == "append":
+        s["k"], s["v"] = randn(total, NKV, HD).half(), (randn(total, NKV, HD) * (randn(total, 1, 1) * 0.5).exp()).half()
+        s["wq"], s["wk"] = (1 + 0.1 * randn(HD)).half(), (1 + 0.1 * randn(HD)).half()
+        maxp = s["lmax"] + 1
+        inv = torch.zeros(HD // 2, device=dev)
+        inv[:32] = 1e6 ** (-torch.arange(32, device=dev, dtype=torch.float32) * 2 / HD)
+        ang = torch.arange(maxp, device=dev, dtype=torch.float32)[:, None] * torch.cat([inv, inv])[None]
+        s["cos"], s["sin"] = ang.cos().half(), ang.sin().half()
+        s["q_out"] = torch.zeros_like(s["q"])
+        s["kp"], s["ks"] = _quantised(randn(nblocks, bs, NKV, HD), case["fmt"])
+        s["vp"], s["vs"] = _quantised(randn(nblocks, bs, NKV, HD) * (randn(nblocks, 1, 1, 1) * 0.5).exp(), case["fmt"])
+        if case["fmt"] == "int8":
+            s["kval"], s["vval"] = (torch.zeros(nblocks, bs, NKV, HD, dtype=torch.float16, device=dev) for _ in range(2))
+    elif op in ("decode", "prefill"):
+        s["kp"], s["ks"] = _quantised(randn(nblocks, bs, NKV, HD), case["fmt"])
+        s["vp"], s["vs"] = _quantised(randn(nblocks, bs, NKV, HD) * (randn(nblocks, 1, 1, 1) * 0.5).exp(), case["fmt"])
+    elif paged:
+        s["kp"], s["vp"] = randn(nblocks, bs, NKV, HD).half(), randn(nblocks, bs, NKV, HD).half()
+    else:
+        s["cap"] = cap = sum(lens)
+        s["kp"], s["vp"] = randn(cap, NKV, HD).half(), randn(cap, NKV, HD).half()
+        off = torch.cumsum(torch.tensor([0] + lens[:-1]), 0).to(dev)
+        s["off"] = off
+        s["k_ptrs"] = s["kp"].data_ptr() + off[s["row_seq"].long()] * (NKV * HD * 2)
+        s["v_ptrs"] = s["vp"].data_ptr() + off[s["row_seq"].long()] * (NKV * HD * 2)
+    if own:
+        import oxide_infer_b200 as oxi
+        s["kv"] = oxi.KvPath(0, max_batch=n, max_seq_len=s["lmax"] + 1, max_prefill_rows=total if op != "decode" else 0)
+        if op in ("append", "decode", "prefill"):
+            s["layout"] = oxi.PagedQ8Layout.of(s["kp"], s["vp"], s["ks"], s["vs"], s["tables"])
+        elif paged:
+            s["layout"] = oxi.PagedLayout.of(s["kp"], s["vp"], s["tables"], bs)
+    return s
+
+
+# ---------------------------------------------------------------------------------------------- one pass
+def run(state):
+    s, c = state, state["case"]
+    op = c["op"]
+    if op == "append":
+        if own:
+            s["kv"].append_q8(s["q_out"], s["q"], s["k"], s["v"], s["wq"], s["wk"], s["cos"], s["sin"], s["pos"], s["layout"],
+                              row_seq=s["row_seq"], eps=EPS)
+        else:
+            _plain_append(s)
+        out = {"q": s["q_out"], "k_scales": s["ks"], "v_scales": s["vs"]}
+        if c["fmt"] == "int8":  # the values that the codes stand for
+            out["k"] = torch.mul(s["kp"], s["ks"][:, None, :, None], out=s["kval"])
+            out["v"] = torch.mul(s["vp"], s["vs"][:, None, :, None], out=s["vval"])
+        else:
+            out["k"], out["v"] = s["kp"], s["vp"]
+        return out
+    if own:
+        kv, w, k = s["kv"], c["window"], c["sinks"]
+        if op == "decode":
+            kv.decode_attn_q8(s["ctx"], s["q"], s["gate"], s["layout"], s["seq_lens"], window=w, sinks=k)
+        elif op == "prefill":
+            kv.prefill_attn_q8(s["ctx"], s["q"], s["gate"], s["layout"], s["row_seq"], s["seq_lens"], window=w, sinks=k)
+        elif op == "decode_sinks" and c["paged"]:
+            kv.decode_attn_paged_sinks(s["ctx"], s["q"], s["gate"], s["layout"], s["seq_lens"], window=w, sinks=k)
+        elif op == "decode_sinks":
+            kv.decode_attn_sinks(s["ctx"], s["q"], s["gate"], s["k_ptrs"], s["v_ptrs"], s["seq_lens"], window=w, sinks=k)
+        elif c["paged"]:
+            kv.prefill_attn_paged_sinks(s["ctx"], s["q"], s["gate"], s["layout"], s["row_seq"], s["seq_lens"], window=w, sinks=k)
+        else:
+            kv.prefill_attn_sinks(s["ctx"], s["q"], s["gate"], s["k_ptrs"], s["v_ptrs"], s["seq_lens"], window=w, sinks=k)
+    else:
+        _plain_attention(s)
+    return s["ctx"]
+
+
+def _rotated(x, w, cos, sin):
+    """RMSNorm and rotation of x [rows][heads][128] in f32."""
+    x = x.float()
+    y = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + EPS) * w.float()
+    half = torch.cat([-y[..., HD // 2:], y[..., :HD // 2]], -1)
+    return y * cos[:, None, :] + half * sin[:, None, :]
+
+
+def _plain_append(s):
+    c = s["case"]
+    bs, fmt = c["bs"], c["fmt"]
+    pos = s["pos"].long()
+    cos, sin = s["cos"][pos].float(), s["sin"][pos].float()
+    s["q_out"].copy_(_rotated(s["q"], s["wq"], cos, sin))
+    block = s["tables"][s["row_seq"].long(), pos // bs].long()
+    slot = pos % bs
+    nb = s["kp"].shape[0]
+    first = torch.full((nb,), bs, device=slot.device).scatter_reduce_(0, block, slot, "amin")  # first slot written; bs: untouched
+    touched = first < bs
+    kept = touched[:, None] & (torch.arange(bs, device=slot.device)[None] < first[:, None])
+    for x, pool, scale in ((_rotated(s["k"], s["wk"], cos, sin), s["kp"], s["ks"]), (s["v"].float(), s["vp"], s["vs"])):
+        amax = torch.zeros(nb, NKV, device=x.device).scatter_reduce_(0, block[:, None].expand(-1, NKV), x.abs().amax(-1), "amax")
+        new = torch.maximum(_scale_of(amax, fmt), torch.where((first > 0)[:, None], scale, torch.zeros_like(scale)))
+        new = torch.where(touched[:, None], new, scale)
+        safe = torch.where(new > 0, new, torch.ones_like(new))
+        again = pool.float() * scale[:, None, :, None] / safe[:, None, :, None]
+        mine = x / safe[block][:, :, None]
+        again, mine = (torch.round(t).clamp(-127, 127).to(torch.int8) if fmt == "int8" else t.clamp(-448, 448).to(CODE[fmt]) for t in (again, mine))
+        bits = pool.view(torch.int8)
+        bits.copy_(torch.where(kept[:, :, None, None], again.view(torch.int8), bits))
+        bits[block, slot] = mine.view(torch.int8)
+        scale.copy_(new)
+
+
+def _plain_attention(s):
+    c = s["case"]
+    w, sinks, n, rmax = c["window"], c["sinks"], s["n"], s["rmax"]
+    dev = s["q"].device
+    # the tokens that a sequence's rows may see: all, or the sinks and a stretch that holds every row's window
+    if w and w + rmax + sinks < s["lmax"]:
+        start = (s["before"].long() + 1 - w).clamp_min(0)[:, None]
+        stretch = start + torch.arange(w + rmax, device=dev)[None]
+        t = torch.cat([torch.arange(sinks, device=dev)[None].expand(n, -1), stretch], 1)
+        once = torch.cat([torch.arange(sinks, device=dev)[None] < start, torch.ones_like(stretch, dtype=torch.bool)], 1)
+    else:
+        t = torch.arange(s["lmax"], device=dev)[None].expand(n, -1)
+        once = torch.ones_like(t, dtype=torch.bool)
+    length = (s["before"] + s["nrows"]).long()[:, None]
+    inside = t.clamp_max(length - 1)
+    if "tables" in s:
+        block = torch.gather(s["tables"].long(), 1, inside // c["bs"])
+        slot = inside % c["bs"]
+        k, v = s["kp"][block, slot].float(), s["vp"][block, slot].float()  # [n][L][4][128]
+        if "ks" in s:
+            k, v = k * s["ks"][block][..., None], v * s["vs"][block][..., None]
+    else:
+        at = s["off"][:, None] + inside
+        k, v = s["kp"][at].float(), s["vp"][at].float()
+    i = torch.arange(rmax, device=dev)[None]
+    row = s["first_row"].long()[:, None] + torch.minimum(i, s["nrows"].long()[:, None] - 1)  # [n][rmax]; past a sequence's rows: its last
+    p = s["pos"].long()[row][:, :, None]
+    seen = once[:, None] & (t[:, None] <= p)
+    if w:
+        seen = seen & ((t[:, None] > p - w) | (t[:, None] < sinks))
+    q = s["q"][row].float().view(n, rmax, NKV, GRP, HD).permute(0, 2, 3, 1, 4).reshape(n, NKV, GRP * rmax, HD)
+    x = torch.matmul(q, k.permute(0, 2, 3, 1)).view(n, NKV, GRP, rmax, -1) * (1.0 / math.sqrt(HD))
+    x = x.masked_fill_(~seen[:, None, None], -math.inf)
+    e = torch.exp(x - x.amax(-1, keepdim=True))
+    o = torch.matmul(e.view(n, NKV, GRP * rmax, -1), v.permute(0, 2, 1, 3)).view(n, NKV, GRP, rmax, HD) / e.sum(-1, keepdim=True)
+    o = o.permute(0, 3, 1, 2, 4).reshape(n, rmax, NQ, HD) * torch.sigmoid(s["gate"][row].float())[..., None]
+    s["ctx"][row] = o.half()  # a repeated last row writes the same values
+
+
+# ---------------------------------------------------------------------------------------------- 64 bits
+def exact(case, seed):
+    s = prepare(case, seed)
+    return _exact_append(s) if case["op"] == "append" else _exact_attention(s)
+
+
+def _codes64(y, fmt):
+    """The code values nearest to y, ties to even."""
+    if fmt == "int8":
+        return torch.round(y).clamp(-127, 127)
+    _, e = torch.frexp(y)
+    step = torch.ldexp(torch.ones_like(y), (e - 1).clamp_min(-6) - 3)
+    return (torch.round(y / step) * step).clamp(-448, 448)
+
+
+def _exact_append(s):
+    c = s["case"]
+    bs, fmt = c["bs"], c["fmt"]
+    rows, seq, pos = s["total"], s["row_seq"].tolist(), s["pos"].tolist()
+    cos, sin = s["cos"].double()[s["pos"].long()], s["sin"].double()[s["pos"].long()]
+
+    def norm_rope(x, w):
+        x = x.double()
+        y = x / torch.sqrt((x * x).sum(-1, keepdim=True) / HD + EPS) * w.double()
+        a, b = y[..., :64], y[..., 64:]
+        return torch.cat([a * cos[:, None, :64] - b * sin[:, None, :64], b * cos[:, None, 64:] + a * sin[:, None, 64:]], -1)
+
+    out = {"q": norm_rope(s["q"], s["wq"])}
+    tables = s["tables"].tolist()
+    for name, x in (("k", norm_rope(s["k"], s["wk"])), ("v", s["v"].double())):
+        codes, scale = s[name + "p"].double(), s[name + "s"].double()
+        r = 0
+        while r < rows:
+            e = r + 1
+            while e < rows and seq[e] == seq[r] and pos[e] // bs == pos[r] // bs:
+                e += 1
+            b, first = tables[seq[r]][pos[r] // bs], pos[r] % bs
+            amax = x[r:e].abs().amax(dim=(0, 2))
+            if fmt == "int8":
+                need = amax / 127.0
+            else:
+                need = torch.exp2(torch.ceil(torch.log2(amax / 448.0)))
+            new = torch.maximum(need, scale[b]) if first else need
+            codes[b, :first] = _codes64(codes[b, :first] * (scale[b] / new)[None, :, None], fmt)
+            codes[b, first:first + e - r] = _codes64(x[r:e] / new[None, :, None], fmt)
+            scale[b] = new
+            r = e
+        out[name + "_scales"] = scale
+        out[name] = codes * scale[:, None, :, None] if fmt == "int8" else codes
+    return out
+
+
+def _exact_attention(s):
+    c = s["case"]
+    w, sinks = c["window"], c["sinks"]
+    out = torch.zeros(s["total"], NQ, HD, dtype=torch.float64, device=s["q"].device)
+    first, nrows, before = s["first_row"].tolist(), s["nrows"].tolist(), s["before"].tolist()
+    for i in range(s["n"]):
+        length = before[i] + nrows[i]
+        lo = max(0, before[i] + 1 - w) if w else 0
+        t = torch.arange(length, device=out.device)
+        t = t[(t >= lo) | (t < sinks)]
+        if "tables" in s:
+            b = s["tables"][i].long()[t // c["bs"]]
+            k, v = s["kp"][b, t % c["bs"]].double(), s["vp"][b, t % c["bs"]].double()
+            if "ks" in s:
+                k, v = k * s["ks"].double()[b][..., None], v * s["vs"].double()[b][..., None]
+        else:
+            k, v = s["kp"][s["off"][i] + t].double(), s["vp"][s["off"][i] + t].double()
+        r = slice(first[i], first[i] + nrows[i])
+        p = s["pos"][r].long()[:, None]
+        hidden = t[None] > p
+        if w:
+            hidden = hidden | ((p - t[None] >= w) & (t[None] >= sinks))
+        q = s["q"][r].double()
+        for h in range(NQ):
+            x = (q[:, h] @ k[:, h // GRP].T) / HD ** 0.5
+            x[hidden] = -math.inf
+            out[r, h] = torch.softmax(x, -1) @ v[:, h // GRP] / (1 + torch.exp(-s["gate"][r, h].double()))[:, None]
+    return out
