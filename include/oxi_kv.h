@@ -56,8 +56,12 @@ enum {
     OXI_DEV_WAIT_TIMEOUT = 4u,   /* an in-kernel pipeline wait gave up (internal error)       */
     OXI_DEV_BAD_TOKEN = 8u,      /* a token id was beyond the embedding table; row zero-filled */
     OXI_DEV_BAD_BLOCK = 16u,     /* a block id in a paged layout's table was >= num_blocks      */
-    OXI_DEV_OUT_OF_BOUNDS = 32u  /* raised only by libraries built with -DOXI_BOUNDS: a table-driven
+    OXI_DEV_OUT_OF_BOUNDS = 32u, /* raised only by libraries built with -DOXI_BOUNDS: a table-driven
                                     index was out of range; the access was not performed         */
+    OXI_DEV_BLOCK_CONFLICT = 64u, /* oxi_append_q8: two separate runs of rows of one call fall into the same
+                                     block of the same sequence; their k / v are not written       */
+    OXI_DEV_NONFINITE = 128u     /* oxi_append_q8: a k or v value was infinite, NaN or beyond f16; it was
+                                    stored as +-65504 (NaN: 0)                                    */
 };
 
 typedef struct oxi_handle oxi_handle;
@@ -286,6 +290,86 @@ int32_t oxi_append_decode_paged(oxi_handle* h, void* stream, void* ctx_out, void
                                 const void* k_norm_w, const void* cos_table, const void* sin_table,
                                 const uint32_t* seq_lens, const oxi_paged_layout* layout, uint32_t batch,
                                 uint32_t window, float eps);
+
+/* ---- K/V caches held in 8 bits ------------------------------------------- */
+/* Half the bytes of the f16 caches: a decode step reads the cache once, so it takes half the time, and a
+ * GPU holds twice the sequences.  No counterpart in the reference.  Paged as above: token t of row b lives
+ * in block block_tables[b][t / block_size] at slot t % block_size, one token = 4 KV heads x 128 codes (512
+ * bytes); block i's codes start at pool + i * block_stride_bytes.  Each (block, KV head) has one f32 scale
+ * for K and one for V at scales + i * scale_stride + head; a code stands for code * scale.
+ *   OXI_Q8_INT8  codes -127..127, scale = amax / 127: steps of equal size, the finer format for keys and
+ *                values without outliers (worst error amax / 254)
+ *   OXI_Q8_E4M3  codes are e4m3 floats, scale = the power of two that puts amax into (224, 448]: relative
+ *                steps, small values keep their precision next to outliers; changing the scale of stored
+ *                codes is exact except below 2^-6 of a code unit */
+enum { OXI_Q8_INT8 = 0, OXI_Q8_E4M3 = 1 };
+typedef struct oxi_paged_q8_layout {
+    void* k_pool;                  /* device, 16-byte aligned */
+    void* v_pool;
+    float* k_scales;               /* device, 16-byte aligned */
+    float* v_scales;
+    const uint32_t* block_tables;  /* device [batch][max_blocks] */
+    uint64_t block_stride_bytes;   /* multiple of 16, >= block_size * 512 */
+    uint64_t scale_stride;         /* floats between the scales of consecutive blocks: multiple of 4, >= 4 */
+    uint32_t max_blocks;
+    uint32_t block_size;           /* tokens per block: 16, 32, 64, 128 or 256 */
+    uint32_t num_blocks;
+    uint32_t format;               /* OXI_Q8_INT8 or OXI_Q8_E4M3 */
+} oxi_paged_q8_layout;
+
+/* Per-head Q/K RMSNorm + RoPE and the quantising append of k and v, for decode rows and prefill waves.
+ *   q_out, q_in [rows][16][128] (may be the same buffer); k_in, v_in [rows][4][128]; tables as oxi_append;
+ *   row r is token pos_ids[r] of table row row_seq[r] (row_seq NULL: of table row r).
+ * Norm and rotation are in f32 with one rounding at the end (f16 for q, the code for k): unlike oxi_append,
+ * which reproduces the reference's intermediate f16 roundings.  Consecutive rows with equal row_seq and
+ * consecutive positions form a run; the part of a run inside one block is written together: the block's
+ * scale becomes the larger of what its new tokens need and, if the run starts behind slot 0, the scale it
+ * has, in which case the codes of the slots before the run are requantised to a scale that grew (each such
+ * change rounds them once more).  A token at slot 0 starts its block afresh.  Slots behind the run keep
+ * their codes.  Two separate runs of one call must not fall into one block (OXI_DEV_BLOCK_CONFLICT, k / v of
+ * both skipped; with row_seq NULL every row is its own sequence), and table rows of one call must not share
+ * a block that is written.  A position >= max_seq_len or beyond max_blocks sets OXI_DEV_BAD_SEQ_LEN and the
+ * row is skipped, a block id >= num_blocks sets OXI_DEV_BAD_BLOCK and k / v are not written.  A row that is
+ * skipped ends a run.  16-byte alignment of all tensors.  rows <= max(max_batch, max_prefill_rows). */
+int32_t oxi_append_q8(oxi_handle* h, void* stream, void* q_out, const void* q_in, const void* k_in, const void* v_in,
+                      const void* q_norm_w, const void* k_norm_w, const void* cos_table, const void* sin_table,
+                      const uint32_t* pos_ids, const oxi_paged_q8_layout* layout, const uint32_t* row_seq, uint32_t rows,
+                      float eps);
+
+/* Gated GQA attention of one token per sequence over an 8-bit cache: row b attends the tokens t < seq_lens[b]
+ * with t >= seq_lens[b] - window (window 0: all) or t < sinks (the first tokens that stay visible behind the
+ * window; 0: none).  q, gate (nullable), ctx_out as oxi_decode_attn.  Scores and sums are f32, the codes enter
+ * the products exactly, the gated result is rounded once.  Codes and scales of visible tokens must be finite;
+ * what invisible slots hold does not matter.  Rows with a length of 0, above max_seq_len or beyond max_blocks
+ * set OXI_DEV_BAD_SEQ_LEN and keep their ctx_out; a block id >= num_blocks sets OXI_DEV_BAD_BLOCK and block 0
+ * is read instead.  A row's result does not depend on the rest of the batch. */
+int32_t oxi_decode_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
+                           const oxi_paged_q8_layout* layout, const uint32_t* seq_lens, uint32_t batch, uint32_t window,
+                           uint32_t sinks);
+
+/* The same for the rows of a prefill wave: row r attends the tokens of table row row_seq[r] that are visible
+ * from position seq_lens[r] - 1.  All rows' k / v were appended before (oxi_append_q8). */
+int32_t oxi_prefill_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
+                            const oxi_paged_q8_layout* layout, const uint32_t* row_seq, const uint32_t* seq_lens,
+                            uint32_t rows, uint32_t window, uint32_t sinks);
+
+/* ---- sliding window with sinks over the f16 caches ----------------------- */
+/* The attention entry points above with the first `sinks` tokens of a sequence staying visible behind its
+ * window: row b attends t < seq_lens[b] with t >= seq_lens[b] - window or t < sinks.  Keys keep the rotation of
+ * their own positions.  Arguments otherwise as the entry point without `_sinks`, whose bytes they return when
+ * window or sinks is 0; else the gated result is rounded once instead of before and after the gate. */
+int32_t oxi_decode_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
+                              const uint64_t* k_ptrs, const uint64_t* v_ptrs, const uint32_t* seq_lens, uint32_t batch,
+                              uint32_t window, uint32_t sinks);
+int32_t oxi_decode_attn_paged_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
+                                    const oxi_paged_layout* layout, const uint32_t* seq_lens, uint32_t batch,
+                                    uint32_t window, uint32_t sinks);
+int32_t oxi_prefill_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
+                               const uint64_t* k_ptrs, const uint64_t* v_ptrs, const uint32_t* seq_lens, uint32_t rows,
+                               uint32_t window, uint32_t sinks);
+int32_t oxi_prefill_attn_paged_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
+                                     const oxi_paged_layout* layout, const uint32_t* row_seq, const uint32_t* seq_lens,
+                                     uint32_t rows, uint32_t window, uint32_t sinks);
 
 /* ---- the sampling side of a decode step: the file's two other table kernels */
 /* out[b][:] = table[token_ids[b]][:] (f16 rows of `hidden` elements).

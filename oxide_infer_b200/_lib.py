@@ -35,6 +35,13 @@ SIGNATURES = {
     "oxi_prefill_split_configure": [_vp, _u32, _u32],
     "oxi_register_kv_slab": [_vp, _vp, C.c_uint64],
     "oxi_prefill_split_slot_bytes": [],
+    "oxi_append_q8": [_vp] * 13 + [_u32, _f32],
+    "oxi_decode_attn_q8": [_vp] * 7 + [_u32] * 3,
+    "oxi_prefill_attn_q8": [_vp] * 8 + [_u32] * 3,
+    "oxi_decode_attn_sinks": [_vp] * 8 + [_u32] * 3,
+    "oxi_decode_attn_paged_sinks": [_vp] * 7 + [_u32] * 3,
+    "oxi_prefill_attn_sinks": [_vp] * 8 + [_u32] * 3,
+    "oxi_prefill_attn_paged_sinks": [_vp] * 8 + [_u32] * 3,
     "oxi_embed_lookup": [_vp] * 5 + [_u32, _u32, _u32],
     "oxi_argmax": [_vp] * 4 + [_u32, _u32],
     "oxi_qk_rmsnorm": [_vp, _vp, _vp, _vp, _f32, _u32, _u32],

@@ -23,6 +23,8 @@ constexpr uint32_t DEV_WAIT_TIMEOUT = 4u;
 constexpr uint32_t DEV_BAD_TOKEN = 8u;
 constexpr uint32_t DEV_BAD_BLOCK = 16u;
 constexpr uint32_t DEV_OUT_OF_BOUNDS = 32u;  // only raised by builds with -DOXI_BOUNDS
+constexpr uint32_t DEV_BLOCK_CONFLICT = 64u;
+constexpr uint32_t DEV_NONFINITE = 128u;
 
 // Builds with -DOXI_BOUNDS check the indices of every table-driven access (cache rows, partial
 // slots, shared-memory stages, wave rows) and, instead of performing an access that is out of
@@ -52,6 +54,23 @@ struct PagedMap {
     uint32_t lbs;                  // log2(block size in tokens), 4 ... 8
     uint32_t num_blocks;           // blocks in the pool: larger ids are rejected
 };
+
+// Paged K/V layout held in 8 bits: as PagedMap with rows of 4 KV heads x 128 codes = 512 bytes, and one
+// f32 scale per (block, KV head) for K and for V.
+constexpr int Q8_ROW_BYTES = NKV * HD;
+struct Q8Map {
+    unsigned char* k_pool;
+    unsigned char* v_pool;
+    float* k_scales;               // block i: k_scales + i * scale_stride, 4 floats
+    float* v_scales;
+    const uint32_t* block_tables;  // [batch][max_blocks]
+    uint64_t block_stride;         // bytes
+    uint64_t scale_stride;         // floats
+    uint32_t max_blocks;
+    uint32_t lbs;                  // log2(block size in tokens), 4 ... 8
+    uint32_t num_blocks;
+};
+constexpr uint32_t Q8_INT8 = 0, Q8_E4M3 = 1;
 
 // ---- approximate instructions the reference uses (kept as PTX so results match bit for bit)
 __device__ __forceinline__ float ex2_approx_ftz(float x) {

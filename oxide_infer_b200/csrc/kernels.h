@@ -107,6 +107,18 @@ cudaError_t launch_append_decode_paged(cudaStream_t stream, const DecodeWorkspac
                                        const uint32_t* seq_lens, const PagedMap& pm, uint32_t batch, uint32_t window,
                                        float eps);
 
+// 8-bit paged caches, and f16 caches with a sliding window and sinks.
+cudaError_t launch_append_q8(cudaStream_t stream, void* q_out, const void* q_in, const void* k_in, const void* v_in,
+                             const void* q_norm_w, const void* k_norm_w, const void* cos_t, const void* sin_t,
+                             const uint32_t* pos_ids, const uint32_t* row_seq /* may be null */, const Q8Map& map,
+                             uint32_t format, uint32_t rows, uint32_t max_seq_len, float eps, uint32_t* status);
+cudaError_t launch_attn_q8(cudaStream_t stream, void* ctx_out, const void* q, const void* gate, const Q8Map& map, uint32_t format,
+                           const uint32_t* row_seq, const uint32_t* seq_lens, uint32_t rows, uint32_t window, uint32_t sinks,
+                           uint32_t max_seq_len, uint32_t* status);
+cudaError_t launch_attn_sinks(cudaStream_t stream, void* ctx_out, const void* q, const void* gate, const uint64_t* k_ptrs,
+                              const uint64_t* v_ptrs, const PagedMap* pm, const uint32_t* row_seq, const uint32_t* seq_lens,
+                              uint32_t rows, uint32_t window, uint32_t sinks, uint32_t max_seq_len, uint32_t* status);
+
 // Projection GEMM (tcgen05) with the append operator as its epilogue, and the same GEMM as a plain linear layer.
 cudaError_t proj_gemm_init();
 int proj_encode_map(TmaDesc* out, const void* base, uint64_t rows, uint32_t box_rows);  // tiled map over [rows][2048] f16; 0 = ok

@@ -494,6 +494,145 @@ int32_t oxi_prefill_attn(oxi_handle* h, void* stream, void* ctx_out, const void*
     return OXI_OK;
 }
 
+// ---- 8-bit paged caches
+static int32_t paged_q8_map(const oxi_paged_q8_layout* l, const char* who, Q8Map* m) {
+    if (!l || !l->k_pool || !l->v_pool || !l->k_scales || !l->v_scales || !l->block_tables) return fail(OXI_ERR_NULL, who);
+    uint32_t lbs = 0;
+    while ((1u << lbs) < l->block_size && lbs < 31) lbs++;
+    if (l->block_size < 16 || l->block_size > 256 || (1u << lbs) != l->block_size)
+        return fail(OXI_ERR_ARG, "paged q8 layout: block_size must be 16, 32, 64, 128 or 256 tokens");
+    if (l->max_blocks == 0 || l->num_blocks == 0) return fail(OXI_ERR_ARG, "paged q8 layout: max_blocks and num_blocks must be positive");
+    if ((l->block_stride_bytes & 15ull) != 0ull || l->block_stride_bytes < (uint64_t)l->block_size * Q8_ROW_BYTES)
+        return fail(OXI_ERR_ARG, "paged q8 layout: block_stride_bytes must be a multiple of 16 and hold block_size rows of 512 bytes");
+    if ((l->scale_stride & 3ull) != 0ull || l->scale_stride < (uint64_t)NKV)
+        return fail(OXI_ERR_ARG, "paged q8 layout: scale_stride must be a multiple of 4 floats and at least 4");
+    if (((uintptr_t)l->k_pool | (uintptr_t)l->v_pool | (uintptr_t)l->k_scales | (uintptr_t)l->v_scales) & 15u)
+        return fail(OXI_ERR_ARG, "paged q8 layout: pools and scales must be 16-byte aligned");
+    if (l->format != OXI_Q8_INT8 && l->format != OXI_Q8_E4M3) return fail(OXI_ERR_ARG, "paged q8 layout: unknown format");
+    m->k_pool = (unsigned char*)l->k_pool;
+    m->v_pool = (unsigned char*)l->v_pool;
+    m->k_scales = l->k_scales;
+    m->v_scales = l->v_scales;
+    m->block_tables = l->block_tables;
+    m->block_stride = l->block_stride_bytes;
+    m->scale_stride = l->scale_stride;
+    m->max_blocks = l->max_blocks;
+    m->lbs = lbs;
+    m->num_blocks = l->num_blocks;
+    return OXI_OK;
+}
+#define REQ_ALIGNED(bits, name) \
+    if (((uintptr_t)(bits) & 15u) != 0u) return fail(OXI_ERR_ARG, name ": tensors must be 16-byte aligned")
+
+int32_t oxi_append_q8(oxi_handle* h, void* stream, void* q_out, const void* q_in, const void* k_in, const void* v_in,
+                      const void* q_norm_w, const void* k_norm_w, const void* cos_table, const void* sin_table,
+                      const uint32_t* pos_ids, const oxi_paged_q8_layout* layout, const uint32_t* row_seq, uint32_t rows,
+                      float eps) {
+    REQ_HANDLE("oxi_append_q8");
+    REQ_PTR(q_out && q_in && k_in && v_in && q_norm_w && k_norm_w && cos_table && sin_table && pos_ids, "oxi_append_q8");
+    REQ_BATCH(rows, (h->max_batch > h->max_prefill_rows ? h->max_batch : h->max_prefill_rows), "oxi_append_q8");
+    if (!(eps >= 0.0f)) return fail(OXI_ERR_ARG, "oxi_append_q8: eps must be >= 0");
+    REQ_ALIGNED((uintptr_t)q_out | (uintptr_t)q_in | (uintptr_t)k_in | (uintptr_t)v_in | (uintptr_t)q_norm_w | (uintptr_t)k_norm_w |
+                    (uintptr_t)cos_table | (uintptr_t)sin_table, "oxi_append_q8");
+    Q8Map m;
+    if (int32_t rc = paged_q8_map(layout, "oxi_append_q8: the layout or one of its pointers is null", &m)) return rc;
+    OXI_CUDA(launch_append_q8((cudaStream_t)stream, q_out, q_in, k_in, v_in, q_norm_w, k_norm_w, cos_table, sin_table, pos_ids,
+                              row_seq, m, layout->format, rows, h->max_seq_len, eps, h->dws.status),
+             "append_q8 launch");
+    return OXI_OK;
+}
+
+int32_t oxi_decode_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
+                           const oxi_paged_q8_layout* layout, const uint32_t* seq_lens, uint32_t batch, uint32_t window,
+                           uint32_t sinks) {
+    REQ_HANDLE("oxi_decode_attn_q8");
+    REQ_PTR(ctx_out && q && seq_lens, "oxi_decode_attn_q8");
+    REQ_BATCH(batch, h->max_batch, "oxi_decode_attn_q8");
+    REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_decode_attn_q8");
+    Q8Map m;
+    if (int32_t rc = paged_q8_map(layout, "oxi_decode_attn_q8: the layout or one of its pointers is null", &m)) return rc;
+    OXI_CUDA(launch_attn_q8((cudaStream_t)stream, ctx_out, q, gate, m, layout->format, nullptr, seq_lens, batch, window, sinks,
+                            h->max_seq_len, h->dws.status),
+             "decode_attn_q8 launch");
+    return OXI_OK;
+}
+
+int32_t oxi_prefill_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
+                            const oxi_paged_q8_layout* layout, const uint32_t* row_seq, const uint32_t* seq_lens,
+                            uint32_t rows, uint32_t window, uint32_t sinks) {
+    REQ_HANDLE("oxi_prefill_attn_q8");
+    REQ_PTR(ctx_out && q && row_seq && seq_lens, "oxi_prefill_attn_q8");
+    REQ_BATCH(rows, h->max_prefill_rows, "oxi_prefill_attn_q8");
+    REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_prefill_attn_q8");
+    Q8Map m;
+    if (int32_t rc = paged_q8_map(layout, "oxi_prefill_attn_q8: the layout or one of its pointers is null", &m)) return rc;
+    OXI_CUDA(launch_attn_q8((cudaStream_t)stream, ctx_out, q, gate, m, layout->format, row_seq, seq_lens, rows, window, sinks,
+                            h->max_seq_len, h->dws.status),
+             "prefill_attn_q8 launch");
+    return OXI_OK;
+}
+
+// ---- sliding window with sinks over the f16 caches
+int32_t oxi_decode_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
+                              const uint64_t* k_ptrs, const uint64_t* v_ptrs, const uint32_t* seq_lens, uint32_t batch,
+                              uint32_t window, uint32_t sinks) {
+    if (window == 0u || sinks == 0u) return oxi_decode_attn(h, stream, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, batch, window);
+    REQ_HANDLE("oxi_decode_attn_sinks");
+    REQ_PTR(ctx_out && q && k_ptrs && v_ptrs && seq_lens, "oxi_decode_attn_sinks");
+    REQ_BATCH(batch, h->max_batch, "oxi_decode_attn_sinks");
+    REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_decode_attn_sinks");
+    OXI_CUDA(launch_attn_sinks((cudaStream_t)stream, ctx_out, q, gate, k_ptrs, v_ptrs, nullptr, nullptr, seq_lens, batch, window,
+                               sinks, h->max_seq_len, h->dws.status),
+             "decode_attn_sinks launch");
+    return OXI_OK;
+}
+
+int32_t oxi_decode_attn_paged_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
+                                    const oxi_paged_layout* layout, const uint32_t* seq_lens, uint32_t batch,
+                                    uint32_t window, uint32_t sinks) {
+    if (window == 0u || sinks == 0u) return oxi_decode_attn_paged(h, stream, ctx_out, q, gate, layout, seq_lens, batch, window);
+    REQ_HANDLE("oxi_decode_attn_paged_sinks");
+    REQ_PTR(ctx_out && q && seq_lens, "oxi_decode_attn_paged_sinks");
+    REQ_BATCH(batch, h->max_batch, "oxi_decode_attn_paged_sinks");
+    REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_decode_attn_paged_sinks");
+    PagedMap pm;
+    if (int32_t rc = paged_map(layout, "oxi_decode_attn_paged_sinks", &pm)) return rc;
+    OXI_CUDA(launch_attn_sinks((cudaStream_t)stream, ctx_out, q, gate, nullptr, nullptr, &pm, nullptr, seq_lens, batch, window,
+                               sinks, h->max_seq_len, h->dws.status),
+             "decode_attn_paged_sinks launch");
+    return OXI_OK;
+}
+
+int32_t oxi_prefill_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
+                               const uint64_t* k_ptrs, const uint64_t* v_ptrs, const uint32_t* seq_lens, uint32_t rows,
+                               uint32_t window, uint32_t sinks) {
+    if (window == 0u || sinks == 0u) return oxi_prefill_attn(h, stream, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, rows, window);
+    REQ_HANDLE("oxi_prefill_attn_sinks");
+    REQ_PTR(ctx_out && q && k_ptrs && v_ptrs && seq_lens, "oxi_prefill_attn_sinks");
+    REQ_BATCH(rows, h->max_prefill_rows, "oxi_prefill_attn_sinks");
+    REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_prefill_attn_sinks");
+    OXI_CUDA(launch_attn_sinks((cudaStream_t)stream, ctx_out, q, gate, k_ptrs, v_ptrs, nullptr, nullptr, seq_lens, rows, window,
+                               sinks, h->max_seq_len, h->dws.status),
+             "prefill_attn_sinks launch");
+    return OXI_OK;
+}
+
+int32_t oxi_prefill_attn_paged_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
+                                     const oxi_paged_layout* layout, const uint32_t* row_seq, const uint32_t* seq_lens,
+                                     uint32_t rows, uint32_t window, uint32_t sinks) {
+    if (window == 0u || sinks == 0u) return oxi_prefill_attn_paged(h, stream, ctx_out, q, gate, layout, row_seq, seq_lens, rows, window);
+    REQ_HANDLE("oxi_prefill_attn_paged_sinks");
+    REQ_PTR(ctx_out && q && row_seq && seq_lens, "oxi_prefill_attn_paged_sinks");
+    REQ_BATCH(rows, h->max_prefill_rows, "oxi_prefill_attn_paged_sinks");
+    REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_prefill_attn_paged_sinks");
+    PagedMap pm;
+    if (int32_t rc = paged_map(layout, "oxi_prefill_attn_paged_sinks", &pm)) return rc;
+    OXI_CUDA(launch_attn_sinks((cudaStream_t)stream, ctx_out, q, gate, nullptr, nullptr, &pm, row_seq, seq_lens, rows, window,
+                               sinks, h->max_seq_len, h->dws.status),
+             "prefill_attn_paged_sinks launch");
+    return OXI_OK;
+}
+
 int32_t oxi_conv_decode(oxi_handle* h, void* stream, void* y_out, const uint64_t* conv_ptrs,
                         const void* bcx, const void* conv_w, uint32_t batch) {
     REQ_HANDLE("oxi_conv_decode");

@@ -37,6 +37,38 @@ class PagedLayout(C.Structure):
         return out
 
 
+class PagedQ8Layout(C.Structure):
+    """oxi_paged_q8_layout of include/oxi_kv.h: one layer's 8-bit K/V pools, their scales and the rows' block tables."""
+    INT8, E4M3 = 0, 1
+    _fields_ = [("k_pool", C.c_void_p), ("v_pool", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+                ("block_tables", C.c_void_p), ("block_stride_bytes", C.c_uint64), ("scale_stride", C.c_uint64),
+                ("max_blocks", C.c_uint32), ("block_size", C.c_uint32), ("num_blocks", C.c_uint32), ("format", C.c_uint32)]
+
+    @classmethod
+    def of(cls, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+           block_tables: torch.Tensor) -> "PagedQ8Layout":
+        """k_pool / v_pool [num_blocks][block_size][4][128] of torch.int8 or torch.float8_e4m3fn (the blocks may
+        lie further apart than their size), k_scales / v_scales [num_blocks][4] float32 (the same),
+        block_tables [batch][max_blocks] int32."""
+        formats = {torch.int8: cls.INT8, torch.float8_e4m3fn: cls.E4M3}
+        for p, sc in ((k_pool, k_scales), (v_pool, v_scales)):
+            if p.dtype not in formats or p.dtype != k_pool.dtype:
+                raise ValueError("k_pool and v_pool must both be int8 or both float8_e4m3fn")
+            if p.dim() != 4 or p.shape != k_pool.shape or p.shape[2:] != (4, 128) or p.stride()[1:] != (512, 128, 1):
+                raise ValueError("pools must be [num_blocks][block_size][4][128] with contiguous blocks")
+            if sc.dtype != torch.float32 or sc.shape != (p.shape[0], 4) or sc.stride(1) != 1:
+                raise ValueError("scales must be float32 [num_blocks][4]")
+        if k_pool.stride(0) != v_pool.stride(0) or k_scales.stride(0) != v_scales.stride(0):
+            raise ValueError("K and V must have the same strides")
+        if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous():
+            raise ValueError("block_tables must be contiguous int32 [batch][max_blocks]")
+        tensors = (k_pool, v_pool, k_scales, v_scales, block_tables)
+        out = cls(*[t.data_ptr() for t in tensors], k_pool.stride(0), k_scales.stride(0), block_tables.shape[1],
+                  k_pool.shape[1], k_pool.shape[0], formats[k_pool.dtype])
+        out._keep = tensors
+        return out
+
+
 class Linear:
     """Tensor maps over projection weights (oxi_qkvg_create / oxi_linear_create).  The weight tensors are
     kept alive by the object."""
@@ -201,6 +233,57 @@ class KvPath:
         n = q.shape[0] if rows is None else rows
         _check(self.lib.oxi_prefill_attn_paged(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), C.addressof(layout),
                                                _p(row_seq), _p(seq_lens), n, window), "oxi_prefill_attn_paged")
+
+    # ---- paged K/V layout held in 8 bits
+    def append_q8(self, q_out, q_in, k_in, v_in, q_norm_w, k_norm_w, cos, sin, pos_ids, layout: PagedQ8Layout,
+                  row_seq=None, eps: float = 1e-5, rows: int | None = None):
+        """RMSNorm + RoPE of q and k and the quantising append of k and v (oxi_append_q8): row r is token pos_ids[r]
+        of table row row_seq[r] (None: of row r).  q_out may be q_in."""
+        n = q_in.shape[0] if rows is None else rows
+        _check(self.lib.oxi_append_q8(self.h, _stream(), _p(q_out), _p(q_in), _p(k_in), _p(v_in), _p(q_norm_w),
+                                      _p(k_norm_w), _p(cos), _p(sin), _p(pos_ids), C.addressof(layout), _p(row_seq), n,
+                                      eps), "oxi_append_q8")
+
+    def decode_attn_q8(self, ctx_out, q, gate, layout: PagedQ8Layout, seq_lens, window: int = 0, sinks: int = 0,
+                       batch: int | None = None):
+        """Attention of one token per sequence over the 8-bit cache; window 0: every token is visible, otherwise the
+        last `window` and the first `sinks` tokens are (oxi_decode_attn_q8)."""
+        b = q.shape[0] if batch is None else batch
+        _check(self.lib.oxi_decode_attn_q8(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), C.addressof(layout),
+                                           _p(seq_lens), b, window, sinks), "oxi_decode_attn_q8")
+
+    def prefill_attn_q8(self, ctx_out, q, gate, layout: PagedQ8Layout, row_seq, seq_lens, window: int = 0,
+                        sinks: int = 0, rows: int | None = None):
+        """Attention of the rows of a prefill wave over the 8-bit cache (oxi_prefill_attn_q8)."""
+        n = q.shape[0] if rows is None else rows
+        _check(self.lib.oxi_prefill_attn_q8(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), C.addressof(layout),
+                                            _p(row_seq), _p(seq_lens), n, window, sinks), "oxi_prefill_attn_q8")
+
+    # ---- sliding window with sinks (the first tokens stay visible) over the f16 caches
+    def decode_attn_sinks(self, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, window: int, sinks: int,
+                          batch: int | None = None):
+        b = q.shape[0] if batch is None else batch
+        _check(self.lib.oxi_decode_attn_sinks(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), _p(k_ptrs), _p(v_ptrs),
+                                              _p(seq_lens), b, window, sinks), "oxi_decode_attn_sinks")
+
+    def decode_attn_paged_sinks(self, ctx_out, q, gate, layout: PagedLayout, seq_lens, window: int, sinks: int,
+                                batch: int | None = None):
+        b = q.shape[0] if batch is None else batch
+        _check(self.lib.oxi_decode_attn_paged_sinks(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), C.addressof(layout),
+                                                    _p(seq_lens), b, window, sinks), "oxi_decode_attn_paged_sinks")
+
+    def prefill_attn_sinks(self, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, window: int, sinks: int,
+                           rows: int | None = None):
+        n = q.shape[0] if rows is None else rows
+        _check(self.lib.oxi_prefill_attn_sinks(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), _p(k_ptrs), _p(v_ptrs),
+                                               _p(seq_lens), n, window, sinks), "oxi_prefill_attn_sinks")
+
+    def prefill_attn_paged_sinks(self, ctx_out, q, gate, layout: PagedLayout, row_seq, seq_lens, window: int, sinks: int,
+                                 rows: int | None = None):
+        n = q.shape[0] if rows is None else rows
+        _check(self.lib.oxi_prefill_attn_paged_sinks(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), C.addressof(layout),
+                                                     _p(row_seq), _p(seq_lens), n, window, sinks),
+               "oxi_prefill_attn_paged_sinks")
 
     def prefill_attn(self, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, window: int = 0,
                      rows: int | None = None):
