@@ -364,6 +364,18 @@ int32_t oxi_decode_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const 
 int32_t oxi_decode_attn_paged_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
                                     const oxi_paged_layout* layout, const uint32_t* seq_lens, uint32_t batch,
                                     uint32_t window, uint32_t sinks);
+/* the fused step: cache rows as oxi_append's, ctx_out the bytes of oxi_append + oxi_decode_attn_sinks (paged: the
+ * paged pair's) */
+int32_t oxi_append_decode_sinks(oxi_handle* h, void* stream, void* ctx_out, void* q_io, const void* k_in,
+                                const void* v_in, const void* gate, const void* q_norm_w, const void* k_norm_w,
+                                const void* cos_table, const void* sin_table, const uint32_t* pos_ids,
+                                const uint32_t* seq_lens, const uint64_t* k_ptrs, const uint64_t* v_ptrs,
+                                uint32_t batch, uint32_t window, uint32_t sinks, float eps);
+int32_t oxi_append_decode_paged_sinks(oxi_handle* h, void* stream, void* ctx_out, void* q_io, const void* k_in,
+                                      const void* v_in, const void* gate, const void* q_norm_w, const void* k_norm_w,
+                                      const void* cos_table, const void* sin_table, const uint32_t* seq_lens,
+                                      const oxi_paged_layout* layout, uint32_t batch, uint32_t window, uint32_t sinks,
+                                      float eps);
 int32_t oxi_prefill_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
                                const uint64_t* k_ptrs, const uint64_t* v_ptrs, const uint32_t* seq_lens, uint32_t rows,
                                uint32_t window, uint32_t sinks);

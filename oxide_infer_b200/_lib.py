@@ -40,6 +40,8 @@ SIGNATURES = {
     "oxi_prefill_attn_q8": [_vp] * 8 + [_u32] * 3,
     "oxi_decode_attn_sinks": [_vp] * 8 + [_u32] * 3,
     "oxi_decode_attn_paged_sinks": [_vp] * 7 + [_u32] * 3,
+    "oxi_append_decode_sinks": [_vp] * 15 + [_u32] * 3 + [_f32],
+    "oxi_append_decode_paged_sinks": [_vp] * 13 + [_u32] * 3 + [_f32],
     "oxi_prefill_attn_sinks": [_vp] * 8 + [_u32] * 3,
     "oxi_prefill_attn_paged_sinks": [_vp] * 8 + [_u32] * 3,
     "oxi_embed_lookup": [_vp] * 5 + [_u32, _u32, _u32],

@@ -252,6 +252,36 @@ __device__ __forceinline__ uint32_t window_start(uint32_t slen, uint32_t window)
     return (window != 0u && slen > window) ? slen - window : 0u;
 }
 
+// What a row sees under a sliding window whose first `sinks` tokens stay visible: tokens t < min(sinks, start)
+// and start <= t < slen, as a list of aligned groups of G tokens - gs groups from token 0, then the groups from
+// token gw * G on; the groups at the edges hold invisible tokens too (visible_bits).
+struct RowView {
+    uint32_t gs, gw, ng;  // groups of the sinks, first group of the window, groups in all
+    uint32_t sinks, start, slen;
+    template <uint32_t G>
+    __device__ __forceinline__ uint32_t token(uint32_t v) const { return (v < gs ? v : v - gs + gw) * G; }
+    // bit i: token t0 + i is visible (i < G <= 8)
+    template <uint32_t G>
+    __device__ __forceinline__ uint32_t visible_bits(uint32_t t0) const {
+        const uint32_t all = (1u << G) - 1u;
+        const uint32_t in_sinks = (1u << min(G, sinks - min(sinks, t0))) - 1u;
+        const uint32_t in_window = (all << min(G, start - min(start, t0))) & all;
+        const uint32_t in_row = (1u << min(G, slen - min(slen, t0))) - 1u;
+        return (in_sinks | in_window) & in_row;
+    }
+};
+template <uint32_t G>
+__device__ __forceinline__ RowView row_view(uint32_t slen, uint32_t window, uint32_t sinks) {
+    RowView r;
+    r.slen = slen;
+    r.start = window_start(slen, window);
+    r.sinks = min(sinks, r.start);
+    r.gs = (r.sinks + G - 1u) / G;
+    r.gw = max(r.gs, r.start / G);
+    r.ng = r.gs + (slen + G - 1u) / G - r.gw;
+    return r;
+}
+
 // Host side: launch `kernel` so that it may overlap the tail of the previous kernel in `stream`.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,

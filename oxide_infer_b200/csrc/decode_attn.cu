@@ -85,7 +85,7 @@ constexpr int Q_BYTES = NQ * HD * 2;            // the row's q (all heads), carr
 // extra inputs of the fused variant: cos row, sin row (256 B each), raw k row, raw v row (1 KB each)
 constexpr int X_COS = 0, X_SIN = 256, X_K = 512, X_V = 512 + KV_ROW_BYTES;
 constexpr int X_BYTES = 512 + 2 * KV_ROW_BYTES;
-constexpr int DESC_BYTES = 32;
+constexpr int DESC_BYTES = 48;
 constexpr int Q_OFF = 2 * HALF_BYTES, X_OFF = Q_OFF + Q_BYTES, DESC_OFF = X_OFF + X_BYTES;
 constexpr int STAGE_BYTES = DESC_OFF + DESC_BYTES;
 constexpr int CHUNK = OXI_DEC_CHUNK;            // keys per work item
@@ -121,6 +121,7 @@ struct DecodeParams {
     uint32_t* merge_count; // [batch][4] arrival counters of those rows, zero between launches
     uint32_t batch;
     uint32_t window;
+    uint32_t sinks;        // kSinks variants only
     uint32_t max_chunks;
     uint32_t max_seq_len;
     // paged variant only: K/V rows live in fixed-size blocks of a pool, block_tables[b][i] is the
@@ -141,6 +142,10 @@ __device__ __forceinline__ uint32_t row_chunks(uint32_t slen, uint32_t window) {
     const uint32_t eff = slen - window_start(slen, window);
     return (eff + dec::CHUNK - 1) / dec::CHUNK;
 }
+// with sinks a row's keys are the groups of its view, in order: CHUNK / GK groups make a work item
+__device__ __forceinline__ uint32_t view_chunks(const RowView& rv) {
+    return (rv.ng + dec::CHUNK / dec::GK - 1) / (dec::CHUNK / dec::GK);
+}
 
 // largest b with prefix[b] <= item  (prefix[0] = 0, prefix[batch] = total)
 __device__ __forceinline__ uint32_t find_row(const uint32_t* prefix, uint32_t batch, uint32_t item) {
@@ -152,7 +157,11 @@ __device__ __forceinline__ uint32_t find_row(const uint32_t* prefix, uint32_t ba
     return lo;
 }
 
-template <bool kFused, bool kPaged>
+// kSinks: a sliding window whose first `sinks` tokens stay visible.  The row's keys are then the aligned groups
+// of four tokens of its RowView, numbered through ("virtual" positions, in which items and stages count); a group
+// is one copy inside one page, and the stage's descriptor has a bit per key because the groups at the edges of
+// sinks and window hold invisible tokens.  The gate is applied before the one rounding of the result.
+template <bool kFused, bool kPaged, bool kSinks>
 __global__ void __launch_bounds__(dec::THREADS, 1)
 decode_attn_kernel(const DecodeParams p) {
     using namespace dec;
@@ -190,7 +199,7 @@ decode_attn_kernel(const DecodeParams p) {
         } else if (!kPaged && ((p.k_ptrs[b] | p.v_ptrs[b]) & 15ull) != 0ull) {
             if (blockIdx.x == 0) atomicOr(p.status, DEV_MISALIGNED_PTR);
         } else {
-            n = row_chunks(slen, p.window);
+            n = kSinks ? view_chunks(row_view<GK>(slen, p.window, p.sinks)) : row_chunks(slen, p.window);
         }
         prefix[b + 1] = n;
         s_len[b] = slen;
@@ -232,7 +241,30 @@ decode_attn_kernel(const DecodeParams p) {
         // paged: lane l holds the block of the item's l-th page (an item spans at most CHUNK / 16 + 1 = 17
         // pages), fetched one item ahead like the row pointers
         uint32_t cpg = 0, cfp = 0;
-        auto fetch_pages = [&](uint32_t b, uint32_t c, uint32_t slen, uint32_t& first_page) -> uint32_t {
+        // kSinks: lanes 0 .. npa-1 hold the pages of the item's sink groups from page `first_page` on, the lanes
+        // behind them those of its window groups from page `first_page_w` on (CHUNK / 16 + 2 pages at most)
+        uint32_t cfw = 0, cna = 0;
+        auto fetch_pages = [&](uint32_t b, uint32_t c, uint32_t slen, uint32_t& first_page, uint32_t& first_page_w,
+                               uint32_t& npa) -> uint32_t {
+            if (kSinks) {
+                const RowView rv = row_view<GK>(slen, p.window, p.sinks);
+                const uint32_t v0 = c * (CHUNK / GK), v1 = min(v0 + (uint32_t)(CHUNK / GK), rv.ng);
+                first_page = (v0 * GK) >> p.paged.lbs;
+                npa = v0 < rv.gs ? (((min(v1, rv.gs) - 1u) * GK) >> p.paged.lbs) - first_page + 1u : 0u;
+                const uint32_t vw = max(v0, rv.gs);
+                first_page_w = rv.token<GK>(vw) >> p.paged.lbs;
+                const uint32_t npw = vw < v1 ? (rv.token<GK>(v1 - 1u) >> p.paged.lbs) - first_page_w + 1u : 0u;
+                uint32_t id = 0;
+                if ((uint32_t)lane < npa + npw) {
+                    id = __ldg(p.paged.block_tables + (size_t)b * p.paged.max_blocks +
+                               ((uint32_t)lane < npa ? first_page + lane : first_page_w + lane - npa));
+                    if (id >= p.paged.num_blocks) {
+                        atomicOr(p.status, DEV_BAD_BLOCK);
+                        id = 0;
+                    }
+                }
+                return id;
+            }
             const uint32_t t0 = window_start(slen, p.window) + c * CHUNK;
             const uint32_t t1 = min(t0 + (uint32_t)CHUNK, slen);
             first_page = t0 >> p.paged.lbs;
@@ -252,7 +284,7 @@ decode_attn_kernel(const DecodeParams p) {
             cc = cur - prefix[cb];
             cslen = s_len[cb];
             if (kPaged) {
-                cpg = fetch_pages(cb, cc, cslen, cfp);
+                cpg = fetch_pages(cb, cc, cslen, cfp, cfw, cna);
             } else {
                 ckp = p.k_ptrs[cb];
                 cvp = p.v_ptrs[cb];
@@ -264,7 +296,7 @@ decode_attn_kernel(const DecodeParams p) {
         while (cur < total_items && ok) {
             uint32_t nxt = __shfl_sync(0xffffffffu, claim, 0);
             nxt = (nxt >= total_items) ? total_items : min(nxt + gridDim.x, total_items);
-            uint32_t nb = 0, nc = 0, nslen = 0, npg = 0, nfp = 0;
+            uint32_t nb = 0, nc = 0, nslen = 0, npg = 0, nfp = 0, nfw = 0, nna = 0;
             uint64_t nkp = 0, nvp = 0;
             claim = 0xffffffffu;  // "no more items" unless a new claim is made
             if (nxt < total_items) {
@@ -273,7 +305,7 @@ decode_attn_kernel(const DecodeParams p) {
                 nc = nxt - prefix[nb];
                 nslen = s_len[nb];
                 if (kPaged) {
-                    npg = fetch_pages(nb, nc, nslen, nfp);
+                    npg = fetch_pages(nb, nc, nslen, nfp, nfw, nna);
                 } else {
                     nkp = p.k_ptrs[nb];
                     nvp = p.v_ptrs[nb];
@@ -285,13 +317,20 @@ decode_attn_kernel(const DecodeParams p) {
             const char* qp = reinterpret_cast<const char*>(p.q) + (size_t)cb * Q_BYTES;
             const char* kp = reinterpret_cast<const char*>(ckp);
             const char* vp = reinterpret_cast<const char*>(cvp);
-            const uint32_t t0 = window_start(cslen, p.window) + cc * CHUNK;
-            const uint32_t t1 = min(t0 + (uint32_t)CHUNK, cslen);
+            const RowView rv = kSinks ? row_view<GK>(cslen, p.window, p.sinks) : RowView{};
+            // kSinks: virtual positions; the last group of the view ends with the row's last key
+            const uint32_t vend = rv.ng * GK - ((0u - cslen) & (uint32_t)(GK - 1));
+            const uint32_t t0 = kSinks ? cc * CHUNK : window_start(cslen, p.window) + cc * CHUNK;
+            const uint32_t t1 = min(t0 + (uint32_t)CHUNK, kSinks ? vend : cslen);
+            // the lane that holds the page of token `tok` of virtual group v
+            auto page_lane = [&](uint32_t v, uint32_t tok) -> uint32_t {
+                return v < rv.gs ? (tok >> p.paged.lbs) - cfp : cna + (tok >> p.paged.lbs) - cfw;
+            };
             const uint32_t bs_mask = kPaged ? (1u << p.paged.lbs) - 1u : 0u;
             if (kPaged && kFused) {
                 // the consumers write the appended row at base + pos * row bytes: give them the base that
                 // makes this the row's place in its block (only meaningful in the row's last range)
-                const uint32_t pid = __shfl_sync(0xffffffffu, cpg, ((pos >> p.paged.lbs) - cfp) & 31u);
+                const uint32_t pid = __shfl_sync(0xffffffffu, cpg, (kSinks ? page_lane(rv.ng - 1u, pos) : (pos >> p.paged.lbs) - cfp) & 31u);
                 const uint64_t off = (uint64_t)pid * p.paged.block_stride + (uint64_t)(pos & bs_mask) * KV_ROW_BYTES -
                                      (uint64_t)pos * KV_ROW_BYTES;
                 ckp = (uint64_t)(uintptr_t)p.paged.k_pool + off;
@@ -314,7 +353,15 @@ decode_attn_kernel(const DecodeParams p) {
                 const bool owner = kFused && last && last_range;
                 const uint32_t ncopy = owner ? nvalid - 1u : nvalid;
                 unsigned char* sb = stages + (size_t)slot * STAGE_BYTES;
+                const uint32_t vgrp = t / GK + (lane & (NGROUP - 1));         // kSinks: this lane's group and its first token
+                const uint32_t gtok = kSinks ? rv.token<GK>(vgrp) : 0u;
+                uint32_t vis = 0;
+                if (kSinks) {
+                    if (lane < NGROUP && vgrp * GK < t1) vis = rv.visible_bits<GK>(gtok) << (lane * GK);
+                    vis = __reduce_or_sync(0xffffffffu, vis);
+                }
                 if (lane == 0) {
+                    if (kSinks) *reinterpret_cast<uint32_t*>(sb + DESC_OFF + 32) = vis;
                     *reinterpret_cast<uint4*>(sb + DESC_OFF) =
                         make_uint4(cb, cc | (nchunks << 16),
                                    nvalid | (first ? F_FIRST : 0u) | (last ? F_LAST : 0u) |
@@ -331,7 +378,9 @@ decode_attn_kernel(const DecodeParams p) {
                 // row; fused: lanes 17/18 the cos/sin rows, lanes 19/20 the raw k/v rows of the owner
                 // paged: a group of 4 tokens lies in one block or straddles two (blocks hold >= 16 tokens)
                 uint32_t pid0 = 0, pid1 = 0;
-                if (kPaged) {
+                if (kPaged && kSinks) {
+                    pid0 = __shfl_sync(0xffffffffu, cpg, page_lane(vgrp, gtok) & 31u);  // a group lies in one block
+                } else if (kPaged) {
                     const uint32_t pi = ((t + (lane & (NGROUP - 1)) * GK) >> p.paged.lbs) - cfp;
                     pid0 = __shfl_sync(0xffffffffu, cpg, pi & 31u);
                     pid1 = __shfl_sync(0xffffffffu, cpg, (pi + 1u) & 31u);
@@ -343,14 +392,15 @@ decode_attn_kernel(const DecodeParams p) {
                         const uint32_t nk = min((uint32_t)GK, ncopy - grp * GK);
                         const uint32_t dst = sbase + (is_v ? HALF_BYTES : 0) + grp * GPITCH;
                         // bounds build: the copied rows lie inside the row's keys and inside the stage
-                        if (!OXI_IN_BOUNDS(cb < p.batch && t + grp * GK + nk <= cslen &&
+                        const uint32_t tok = kSinks ? gtok : t + grp * GK;
+                        if (!OXI_IN_BOUNDS(cb < p.batch && tok + nk <= cslen &&
                                                grp * GPITCH + nk * KV_ROW_BYTES <= (uint32_t)HALF_BYTES, p.status)) {
                             // nothing is copied; the stage's expected byte count must still be met
                             asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full_bar[slot])),
                                          "r"(nk * KV_ROW_BYTES) : "memory");
                         } else if (kPaged) {
                             const unsigned char* pool = is_v ? p.paged.v_pool : p.paged.k_pool;
-                            const uint32_t off = (t + grp * GK) & bs_mask;
+                            const uint32_t off = tok & bs_mask;
                             const uint32_t n1 = min(nk, bs_mask + 1u - off);
                             bulk_g2s_hint(dst, pool + (size_t)pid0 * p.paged.block_stride + (size_t)off * KV_ROW_BYTES,
                                           n1 * KV_ROW_BYTES, &full_bar[slot], policy);
@@ -358,7 +408,7 @@ decode_attn_kernel(const DecodeParams p) {
                                 bulk_g2s_hint(dst + n1 * KV_ROW_BYTES, pool + (size_t)pid1 * p.paged.block_stride,
                                               (nk - n1) * KV_ROW_BYTES, &full_bar[slot], policy);
                         } else {
-                            const char* src = (is_v ? vp : kp) + (size_t)(t + grp * GK) * KV_ROW_BYTES;
+                            const char* src = (is_v ? vp : kp) + (size_t)tok * KV_ROW_BYTES;
                             bulk_g2s_hint(dst, src, nk * KV_ROW_BYTES, &full_bar[slot], policy);
                         }
                     }
@@ -372,7 +422,7 @@ decode_attn_kernel(const DecodeParams p) {
                     bulk_g2s(sbase + X_OFF + (lane == 19 ? X_K : X_V), src, KV_ROW_BYTES, &full_bar[slot]);
                 }
             }
-            cur = nxt; cb = nb; cc = nc; cslen = nslen; ckp = nkp; cvp = nvp; cpg = npg; cfp = nfp;
+            cur = nxt; cb = nb; cc = nc; cslen = nslen; ckp = nkp; cvp = nvp; cpg = npg; cfp = nfp; cfw = nfw; cna = nna;
         }
         if (ok) {
             // end-of-work descriptor so the consumers leave their loop
@@ -490,7 +540,16 @@ decode_attn_kernel(const DecodeParams p) {
             if (row_ok) *reinterpret_cast<uint2*>(vp64 + (size_t)desc.w * KV_ROW_BYTES + kvh * (HD * 2) + lane * 8) = vv;
             __syncwarp();
         }
-        if (nvalid < KS) {
+        const uint32_t vis = kSinks ? *reinterpret_cast<const uint32_t*>(sb + DESC_OFF + 32) : 0xffffffffu;
+        if (kSinks && vis != 0xffffffffu) {
+            // invisible keys of the view's edge groups, and rows behind its end
+            for (uint32_t i = lane; i < KS * 16u; i += 32) {
+                const uint32_t row = i >> 4;
+                if (!((vis >> row) & 1u))
+                    *reinterpret_cast<uint4*>(vst + (row >> 2) * GPITCH + (row & 3u) * KV_ROW_BYTES + (i & 15u) * 16u) = make_uint4(0, 0, 0, 0);
+            }
+            __syncwarp();
+        } else if (nvalid < KS) {
             // tail stage: rows past the range keep stale bytes; zero this head's V slice there
             // so that 0 * stale can never produce NaN.
             for (uint32_t i = lane; i < (KS - nvalid) * 16u; i += 32) {
@@ -523,7 +582,7 @@ decode_attn_kernel(const DecodeParams p) {
             for (int j = 0; j < 2; j++) {
                 const uint32_t key = nb + 4 * (2 * t4 + j);
                 float v = s[nb][j] * QK_SCALE_LOG2;
-                v = (key < nvalid) ? v : -INFINITY;
+                v = (kSinks ? ((vis >> key) & 1u) != 0u : key < nvalid) ? v : -INFINITY;
                 s[nb][j] = v;
                 mx = fmaxf(mx, v);
             }
@@ -561,7 +620,7 @@ decode_attn_kernel(const DecodeParams p) {
             }
         }
         // release the stage (generic writes of a tail stage are ordered before later bulk copies)
-        if (nvalid < KS || owner || (kFused && (desc.z & F_FIRST))) fence_proxy_async_smem();
+        if (nvalid < KS || (kSinks && vis != 0xffffffffu) || owner || (kFused && (desc.z & F_FIRST))) fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty_bar[slot]);
 
@@ -574,14 +633,15 @@ decode_attn_kernel(const DecodeParams p) {
         l_tot += __shfl_xor_sync(0xffffffffu, l_tot, 2);
         if (g >= 4) continue;
         if (nchunks == 1) {
-            const float inv = rcp_approx_ftz(l_tot);
+            float inv = rcp_approx_ftz(l_tot);
             const float sig = p.gate ? sigmoid_ref(h2f(p.gate[(size_t)b * NQ + head])) : 1.0f;
+            if (kSinks) inv *= sig;
             uint16_t* out = p.ctx_out + ((size_t)b * NQ + head) * HD;
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 uint16_t h0 = f2h(__fmul_rn(o[j][0], inv));
                 uint16_t h1 = f2h(__fmul_rn(o[j][1], inv));
-                if (p.gate) {
+                if (!kSinks && p.gate) {
                     h0 = f2h(__fmul_rn(h2f(h0), sig));
                     h1 = f2h(__fmul_rn(h2f(h1), sig));
                 }
@@ -616,7 +676,10 @@ constexpr int MERGE_BLK = 16;            // key ranges per block of loads = per 
 constexpr int MERGE_SLOT = HD + 4;       // floats per slice slot: 128 sums, the weight sum, padding to 16 bytes
 constexpr int MERGE_MAX_Y = 8;
 
-template <bool kSliced>  // false: the workspace holds rows of at most 16 key ranges (no slice scratch)
+// kRule: how a row is cut into key ranges, and how its result is rounded
+constexpr int MERGE_WINDOW = 0;  // row_chunks; the gate on the f16 result, as the reference does
+constexpr int MERGE_SINKS = 1;   // view_chunks; the gate before the one rounding
+template <bool kSliced, int kRule>  // kSliced false: the workspace holds rows of at most 16 key ranges (no slice scratch)
 __global__ void __launch_bounds__(128)
 decode_merge_kernel(const DecodeParams p) {
     pdl_launch_dependents();
@@ -631,7 +694,7 @@ decode_merge_kernel(const DecodeParams p) {
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.work_counter = 0u;
     if (slen == 0u || slen > p.max_seq_len || (kvp & 15ull) != 0ull) return;
     if (p.paged.block_tables && ((slen - 1u) >> p.paged.lbs) >= p.paged.max_blocks) return;
-    const uint32_t nchunks = row_chunks(slen, p.window);
+    const uint32_t nchunks = kRule == MERGE_SINKS ? view_chunks(row_view<dec::GK>(slen, p.window, p.sinks)) : row_chunks(slen, p.window);
     if (nchunks <= 1) return;
     const uint32_t nslices = kSliced ? (nchunks + MERGE_BLK - 1) / MERGE_BLK : 1u;
     // CTAs that work on this row and head group: several only where that saves memory round trips
@@ -733,10 +796,11 @@ decode_merge_kernel(const DecodeParams p) {
             }
         }
     }
-    const float inv = rcp_approx_ftz(l);
+    float inv = rcp_approx_ftz(l);
+    if (kRule != MERGE_WINDOW && p.gate) inv *= sigmoid_ref(gate_f);
     uint16_t h[4] = {f2h(__fmul_rn(acc.x, inv)), f2h(__fmul_rn(acc.y, inv)),
                      f2h(__fmul_rn(acc.z, inv)), f2h(__fmul_rn(acc.w, inv))};
-    if (p.gate) {
+    if (kRule == MERGE_WINDOW && p.gate) {
         const float sig = sigmoid_ref(gate_f);
 #pragma unroll
         for (int i = 0; i < 4; i++) h[i] = f2h(__fmul_rn(h2f(h[i]), sig));
@@ -761,9 +825,10 @@ static dim3 merge_grid(const DecodeWorkspace& ws, uint32_t batch) {
     return dim3(batch * NKV, y);
 }
 
+template <int kRule>
 static cudaError_t launch_merge(cudaStream_t stream, const DecodeWorkspace& ws, uint32_t batch, const DecodeParams& p) {
-    if (ws.merge_acc) return launch_pdl(decode_merge_kernel<true>, merge_grid(ws, batch), dim3(128), 0, stream, p);
-    return launch_pdl(decode_merge_kernel<false>, dim3(batch * NKV), dim3(128), 0, stream, p);
+    if (ws.merge_acc) return launch_pdl(decode_merge_kernel<true, kRule>, merge_grid(ws, batch), dim3(128), 0, stream, p);
+    return launch_pdl(decode_merge_kernel<false, kRule>, dim3(batch * NKV), dim3(128), 0, stream, p);
 }
 
 size_t decode_merge_scratch_bytes(uint32_t max_batch, uint32_t max_chunks) {
@@ -774,16 +839,21 @@ size_t decode_merge_scratch_bytes(uint32_t max_batch, uint32_t max_chunks) {
 uint32_t decode_chunk_keys() { return dec::CHUNK; }
 uint32_t decode_max_rows() { return dec::MAX_ROWS; }
 
-cudaError_t decode_attn_init() {
-    cudaError_t e = cudaFuncSetAttribute(decode_attn_kernel<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)dec::SMEM_BYTES);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(decode_attn_kernel<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dec::SMEM_BYTES);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(decode_attn_kernel<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dec::SMEM_BYTES);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(decode_attn_kernel<true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dec::SMEM_BYTES);
+template <bool kSinks>
+static cudaError_t set_smem() {
+    auto set = [](auto* kernel) {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dec::SMEM_BYTES);
+    };
+    cudaError_t e = set(decode_attn_kernel<false, false, kSinks>);
+    if (e == cudaSuccess) e = set(decode_attn_kernel<true, false, kSinks>);
+    if (e == cudaSuccess) e = set(decode_attn_kernel<false, true, kSinks>);
+    if (e == cudaSuccess) e = set(decode_attn_kernel<true, true, kSinks>);
     return e;
+}
+
+cudaError_t decode_attn_init() {
+    const cudaError_t e = set_smem<false>();
+    return e != cudaSuccess ? e : set_smem<true>();
 }
 
 static DecodeParams make_params(const DecodeWorkspace& ws, void* ctx_out, const void* q, const void* gate,
@@ -810,65 +880,61 @@ static DecodeParams make_params(const DecodeWorkspace& ws, void* ctx_out, const 
     return p;
 }
 
+// The streaming kernel of p's variant and the merge.  sinks == 0: the plain window.
+template <bool kFused, bool kPaged>
+static cudaError_t launch_decode(cudaStream_t stream, const DecodeWorkspace& ws, uint32_t sinks, DecodeParams p) {
+    p.sinks = sinks;
+    cudaError_t e = launch_pdl(sinks ? decode_attn_kernel<kFused, kPaged, true> : decode_attn_kernel<kFused, kPaged, false>,
+                               dim3(ws.num_sms), dim3(dec::THREADS), dec::SMEM_BYTES, stream, p);
+    if (e != cudaSuccess) return e;
+    return sinks ? launch_merge<MERGE_SINKS>(stream, ws, p.batch, p) : launch_merge<MERGE_WINDOW>(stream, ws, p.batch, p);
+}
+
 cudaError_t launch_decode_attn(cudaStream_t stream, const DecodeWorkspace& ws, void* ctx_out,
                                const void* q, const void* gate, const uint64_t* k_ptrs,
                                const uint64_t* v_ptrs, const uint32_t* seq_lens, uint32_t batch,
-                               uint32_t window) {
-    const DecodeParams p = make_params(ws, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, batch, window);
-    cudaError_t e = launch_pdl(decode_attn_kernel<false, false>, dim3(ws.num_sms), dim3(dec::THREADS), dec::SMEM_BYTES,
-                               stream, p);
-    if (e != cudaSuccess) return e;
-    return launch_merge(stream, ws, batch, p);
+                               uint32_t window, uint32_t sinks) {
+    return launch_decode<false, false>(stream, ws, sinks, make_params(ws, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, batch, window));
+}
+
+static void set_fused(DecodeParams& p, const void* k_in, const void* v_in, const void* q_norm_w, const void* k_norm_w,
+                      const void* cos_t, const void* sin_t, float eps) {
+    p.k_in = (const uint16_t*)k_in;
+    p.v_in = (const uint16_t*)v_in;
+    p.q_norm_w = (const uint16_t*)q_norm_w;
+    p.k_norm_w = (const uint16_t*)k_norm_w;
+    p.cos_t = (const uint16_t*)cos_t;
+    p.sin_t = (const uint16_t*)sin_t;
+    p.eps = eps;
 }
 
 cudaError_t launch_append_decode(cudaStream_t stream, const DecodeWorkspace& ws, void* ctx_out, const void* q_io,
                                  const void* k_in, const void* v_in, const void* gate, const void* q_norm_w,
                                  const void* k_norm_w, const void* cos_t, const void* sin_t,
                                  const uint32_t* seq_lens, const uint64_t* k_ptrs, const uint64_t* v_ptrs,
-                                 uint32_t batch, uint32_t window, float eps) {
+                                 uint32_t batch, uint32_t window, float eps, uint32_t sinks) {
     DecodeParams p = make_params(ws, ctx_out, q_io, gate, k_ptrs, v_ptrs, seq_lens, batch, window);
-    p.k_in = (const uint16_t*)k_in;
-    p.v_in = (const uint16_t*)v_in;
-    p.q_norm_w = (const uint16_t*)q_norm_w;
-    p.k_norm_w = (const uint16_t*)k_norm_w;
-    p.cos_t = (const uint16_t*)cos_t;
-    p.sin_t = (const uint16_t*)sin_t;
-    p.eps = eps;
-    cudaError_t e = launch_pdl(decode_attn_kernel<true, false>, dim3(ws.num_sms), dim3(dec::THREADS), dec::SMEM_BYTES,
-                               stream, p);
-    if (e != cudaSuccess) return e;
-    return launch_merge(stream, ws, batch, p);
+    set_fused(p, k_in, v_in, q_norm_w, k_norm_w, cos_t, sin_t, eps);
+    return launch_decode<true, false>(stream, ws, sinks, p);
 }
 
 cudaError_t launch_decode_attn_paged(cudaStream_t stream, const DecodeWorkspace& ws, void* ctx_out, const void* q,
                                      const void* gate, const PagedMap& pm, const uint32_t* seq_lens, uint32_t batch,
-                                     uint32_t window) {
+                                     uint32_t window, uint32_t sinks) {
     DecodeParams p = make_params(ws, ctx_out, q, gate, nullptr, nullptr, seq_lens, batch, window);
     p.paged = pm;
-    cudaError_t e = launch_pdl(decode_attn_kernel<false, true>, dim3(ws.num_sms), dim3(dec::THREADS), dec::SMEM_BYTES,
-                               stream, p);
-    if (e != cudaSuccess) return e;
-    return launch_merge(stream, ws, batch, p);
+    return launch_decode<false, true>(stream, ws, sinks, p);
 }
 
 cudaError_t launch_append_decode_paged(cudaStream_t stream, const DecodeWorkspace& ws, void* ctx_out, const void* q_io,
                                        const void* k_in, const void* v_in, const void* gate, const void* q_norm_w,
                                        const void* k_norm_w, const void* cos_t, const void* sin_t,
                                        const uint32_t* seq_lens, const PagedMap& pm, uint32_t batch, uint32_t window,
-                                       float eps) {
+                                       float eps, uint32_t sinks) {
     DecodeParams p = make_params(ws, ctx_out, q_io, gate, nullptr, nullptr, seq_lens, batch, window);
     p.paged = pm;
-    p.k_in = (const uint16_t*)k_in;
-    p.v_in = (const uint16_t*)v_in;
-    p.q_norm_w = (const uint16_t*)q_norm_w;
-    p.k_norm_w = (const uint16_t*)k_norm_w;
-    p.cos_t = (const uint16_t*)cos_t;
-    p.sin_t = (const uint16_t*)sin_t;
-    p.eps = eps;
-    cudaError_t e = launch_pdl(decode_attn_kernel<true, true>, dim3(ws.num_sms), dim3(dec::THREADS), dec::SMEM_BYTES,
-                               stream, p);
-    if (e != cudaSuccess) return e;
-    return launch_merge(stream, ws, batch, p);
+    set_fused(p, k_in, v_in, q_norm_w, k_norm_w, cos_t, sin_t, eps);
+    return launch_decode<true, true>(stream, ws, sinks, p);
 }
 
 }  // namespace oxi

@@ -41,13 +41,13 @@ cudaError_t decode_attn_init();  // one-time function attributes (dynamic shared
 cudaError_t launch_decode_attn(cudaStream_t stream, const DecodeWorkspace& ws, void* ctx_out,
                                const void* q, const void* gate, const uint64_t* k_ptrs,
                                const uint64_t* v_ptrs, const uint32_t* seq_lens, uint32_t batch,
-                               uint32_t window);
+                               uint32_t window, uint32_t sinks = 0 /* first tokens that stay visible behind the window */);
 // Fused RMSNorm + RoPE + KV append + gated decode attention (positions are seq_lens - 1).
 cudaError_t launch_append_decode(cudaStream_t stream, const DecodeWorkspace& ws, void* ctx_out, const void* q_io,
                                  const void* k_in, const void* v_in, const void* gate, const void* q_norm_w,
                                  const void* k_norm_w, const void* cos_t, const void* sin_t,
                                  const uint32_t* seq_lens, const uint64_t* k_ptrs, const uint64_t* v_ptrs,
-                                 uint32_t batch, uint32_t window, float eps);
+                                 uint32_t batch, uint32_t window, float eps, uint32_t sinks = 0);
 uint32_t decode_chunk_keys();    // keys per split-KV work item
 uint32_t decode_max_rows();      // rows one launch can take
 size_t decode_merge_scratch_bytes(uint32_t max_batch, uint32_t max_chunks);
@@ -100,12 +100,12 @@ cudaError_t launch_append_paged(cudaStream_t stream, void* q_io, const void* k_i
                                 uint32_t batch, float eps, uint32_t* status);
 cudaError_t launch_decode_attn_paged(cudaStream_t stream, const DecodeWorkspace& ws, void* ctx_out, const void* q,
                                      const void* gate, const PagedMap& pm, const uint32_t* seq_lens, uint32_t batch,
-                                     uint32_t window);
+                                     uint32_t window, uint32_t sinks = 0);
 cudaError_t launch_append_decode_paged(cudaStream_t stream, const DecodeWorkspace& ws, void* ctx_out, const void* q_io,
                                        const void* k_in, const void* v_in, const void* gate, const void* q_norm_w,
                                        const void* k_norm_w, const void* cos_t, const void* sin_t,
                                        const uint32_t* seq_lens, const PagedMap& pm, uint32_t batch, uint32_t window,
-                                       float eps);
+                                       float eps, uint32_t sinks = 0);
 
 // 8-bit paged caches, and f16 caches with a sliding window and sinks.
 cudaError_t launch_append_q8(cudaStream_t stream, void* q_out, const void* q_in, const void* k_in, const void* v_in,

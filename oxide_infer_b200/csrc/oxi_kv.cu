@@ -581,8 +581,7 @@ int32_t oxi_decode_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const 
     REQ_PTR(ctx_out && q && k_ptrs && v_ptrs && seq_lens, "oxi_decode_attn_sinks");
     REQ_BATCH(batch, h->max_batch, "oxi_decode_attn_sinks");
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_decode_attn_sinks");
-    OXI_CUDA(launch_attn_sinks((cudaStream_t)stream, ctx_out, q, gate, k_ptrs, v_ptrs, nullptr, nullptr, seq_lens, batch, window,
-                               sinks, h->max_seq_len, h->dws.status),
+    OXI_CUDA(launch_decode_attn((cudaStream_t)stream, take_dws(h), ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, batch, window, sinks),
              "decode_attn_sinks launch");
     return OXI_OK;
 }
@@ -597,9 +596,52 @@ int32_t oxi_decode_attn_paged_sinks(oxi_handle* h, void* stream, void* ctx_out, 
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_decode_attn_paged_sinks");
     PagedMap pm;
     if (int32_t rc = paged_map(layout, "oxi_decode_attn_paged_sinks", &pm)) return rc;
-    OXI_CUDA(launch_attn_sinks((cudaStream_t)stream, ctx_out, q, gate, nullptr, nullptr, &pm, nullptr, seq_lens, batch, window,
-                               sinks, h->max_seq_len, h->dws.status),
+    OXI_CUDA(launch_decode_attn_paged((cudaStream_t)stream, take_dws(h), ctx_out, q, gate, pm, seq_lens, batch, window, sinks),
              "decode_attn_paged_sinks launch");
+    return OXI_OK;
+}
+
+int32_t oxi_append_decode_sinks(oxi_handle* h, void* stream, void* ctx_out, void* q_io, const void* k_in,
+                                const void* v_in, const void* gate, const void* q_norm_w, const void* k_norm_w,
+                                const void* cos_table, const void* sin_table, const uint32_t* pos_ids,
+                                const uint32_t* seq_lens, const uint64_t* k_ptrs, const uint64_t* v_ptrs,
+                                uint32_t batch, uint32_t window, uint32_t sinks, float eps) {
+    if (window == 0u || sinks == 0u)
+        return oxi_append_decode(h, stream, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos_table, sin_table, pos_ids,
+                                 seq_lens, k_ptrs, v_ptrs, batch, window, eps);
+    REQ_HANDLE("oxi_append_decode_sinks");
+    REQ_PTR(ctx_out && q_io && k_in && v_in && q_norm_w && k_norm_w && cos_table && sin_table && pos_ids &&
+                seq_lens && k_ptrs && v_ptrs, "oxi_append_decode_sinks");
+    REQ_BATCH(batch, h->max_batch, "oxi_append_decode_sinks");
+    if (!(eps >= 0.0f)) return fail(OXI_ERR_ARG, "oxi_append_decode_sinks: eps must be >= 0");
+    REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q_io | (uintptr_t)k_in | (uintptr_t)v_in | (uintptr_t)cos_table | (uintptr_t)sin_table,
+                "oxi_append_decode_sinks");
+    OXI_CUDA(launch_append_decode((cudaStream_t)stream, take_dws(h), ctx_out, q_io, k_in, v_in, gate, q_norm_w,
+                                  k_norm_w, cos_table, sin_table, seq_lens, k_ptrs, v_ptrs, batch, window, eps, sinks),
+             "append_decode_sinks launch");
+    return OXI_OK;
+}
+
+int32_t oxi_append_decode_paged_sinks(oxi_handle* h, void* stream, void* ctx_out, void* q_io, const void* k_in,
+                                      const void* v_in, const void* gate, const void* q_norm_w, const void* k_norm_w,
+                                      const void* cos_table, const void* sin_table, const uint32_t* seq_lens,
+                                      const oxi_paged_layout* layout, uint32_t batch, uint32_t window, uint32_t sinks,
+                                      float eps) {
+    if (window == 0u || sinks == 0u)
+        return oxi_append_decode_paged(h, stream, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos_table, sin_table,
+                                       seq_lens, layout, batch, window, eps);
+    REQ_HANDLE("oxi_append_decode_paged_sinks");
+    REQ_PTR(ctx_out && q_io && k_in && v_in && q_norm_w && k_norm_w && cos_table && sin_table && seq_lens,
+            "oxi_append_decode_paged_sinks");
+    REQ_BATCH(batch, h->max_batch, "oxi_append_decode_paged_sinks");
+    if (!(eps >= 0.0f)) return fail(OXI_ERR_ARG, "oxi_append_decode_paged_sinks: eps must be >= 0");
+    REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q_io | (uintptr_t)k_in | (uintptr_t)v_in | (uintptr_t)cos_table | (uintptr_t)sin_table,
+                "oxi_append_decode_paged_sinks");
+    PagedMap pm;
+    if (int32_t rc = paged_map(layout, "oxi_append_decode_paged_sinks", &pm)) return rc;
+    OXI_CUDA(launch_append_decode_paged((cudaStream_t)stream, take_dws(h), ctx_out, q_io, k_in, v_in, gate, q_norm_w,
+                                        k_norm_w, cos_table, sin_table, seq_lens, pm, batch, window, eps, sinks),
+             "append_decode_paged_sinks launch");
     return OXI_OK;
 }
 

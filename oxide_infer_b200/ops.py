@@ -272,6 +272,20 @@ class KvPath:
         _check(self.lib.oxi_decode_attn_paged_sinks(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), C.addressof(layout),
                                                     _p(seq_lens), b, window, sinks), "oxi_decode_attn_paged_sinks")
 
+    def append_decode_sinks(self, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos, sin, pos_ids, seq_lens,
+                            k_ptrs, v_ptrs, window: int, sinks: int, eps: float = 1e-5):
+        _check(self.lib.oxi_append_decode_sinks(self.h, _stream(), _p(ctx_out), _p(q_io), _p(k_in), _p(v_in), _p(gate),
+                                                _p(q_norm_w), _p(k_norm_w), _p(cos), _p(sin), _p(pos_ids), _p(seq_lens),
+                                                _p(k_ptrs), _p(v_ptrs), q_io.shape[0], window, sinks, eps),
+               "oxi_append_decode_sinks")
+
+    def append_decode_paged_sinks(self, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos, sin, seq_lens,
+                                  layout: PagedLayout, window: int, sinks: int, eps: float = 1e-5):
+        _check(self.lib.oxi_append_decode_paged_sinks(self.h, _stream(), _p(ctx_out), _p(q_io), _p(k_in), _p(v_in),
+                                                      _p(gate), _p(q_norm_w), _p(k_norm_w), _p(cos), _p(sin),
+                                                      _p(seq_lens), C.addressof(layout), q_io.shape[0], window, sinks,
+                                                      eps), "oxi_append_decode_paged_sinks")
+
     def prefill_attn_sinks(self, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, window: int, sinks: int,
                            rows: int | None = None):
         n = q.shape[0] if rows is None else rows

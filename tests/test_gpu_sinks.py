@@ -156,6 +156,40 @@ def test_paged_decode_reports_bad_tables(kv):
     assert torch.equal(a[0].view(torch.int16), b[0].view(torch.int16)) and bool((b[2] == 7.0).all())
 
 
+@pytest.mark.parametrize("bs", [0, 16, 256])
+@pytest.mark.parametrize("window,sinks", [(1, 1), (100, 4), (64, 70), (300, 33), (8000, 4)])
+def test_fused_step_is_append_then_decode(kv, bs, window, sinks):
+    lens = [0, 1, 3, 15, 16, 17, 63, 64, 100, 104, 255, 257, 700, 3001]
+    n = len(lens)
+    gen = torch.Generator(device="cuda").manual_seed(80)
+    half = lambda *s: torch.randn(*s, generator=gen, device="cuda").half()  # noqa: E731
+    q, k, v, g = half(n, 16, 128), half(n, 4, 128), half(n, 4, 128), half(n, 16)
+    w = (1 + 0.1 * torch.randn(128, generator=gen, device="cuda")).half()
+    ang = torch.rand(max(lens) + 1, 128, generator=gen, device="cuda") * 6.28
+    cos, sin = ang.cos().half(), ang.sin().half()
+    pos, sl = Q.i32(lens), Q.i32([x + 1 for x in lens])
+    outs = []
+    for fused in (False, True):
+        c = F16Cache(lens, bs, seed=81)
+        qq, ctx = q.clone(), _ctx(n)
+        if bs and fused:
+            kv.append_decode_paged_sinks(ctx, qq, k, v, g, w, w, cos, sin, sl, c.layout(), window, sinks)
+        elif fused:
+            kv.append_decode_sinks(ctx, qq, k, v, g, w, w, cos, sin, pos, sl, c.k_ptrs, c.v_ptrs, window, sinks)
+        else:
+            if bs:
+                kv.append_paged(qq, k, v, w, w, cos, sin, pos, c.layout())
+            else:
+                kv.append(qq, k, v, w, w, cos, sin, pos, c.k_ptrs, c.v_ptrs)
+            c.decode(kv, ctx, qq, g, [x + 1 for x in lens], window, sinks)
+            Q.check_rows(ctx, qq, g, [(i, i, Q.visible(x + 1, window, sinks)) for i, x in enumerate(lens)], c.values)
+        outs.append((ctx, torch.stack([torch.stack(c.values(i, [x])) for i, x in enumerate(lens)])))
+        if fused:
+            assert torch.equal(qq, q)  # read as the raw q
+    assert kv.device_status() == 0
+    assert torch.equal(outs[0][0].view(torch.int16), outs[1][0].view(torch.int16)) and torch.equal(outs[0][1], outs[1][1])
+
+
 WAVES = {
     "one row": [(0, 0, 1)],
     "a row behind a prefix": [(0, 900, 1)],

@@ -20,6 +20,8 @@ def test_null_handles_are_refused_before_cuda_is_touched(lib):
     for window, sinks in ((0, 0), (5, 2)):
         assert lib.oxi_decode_attn_sinks(n, *([n] * 7), 1, window, sinks) == -1
         assert lib.oxi_decode_attn_paged_sinks(n, *([n] * 6), 1, window, sinks) == -1
+        assert lib.oxi_append_decode_sinks(n, *([n] * 14), 1, window, sinks, 1e-5) == -1
+        assert lib.oxi_append_decode_paged_sinks(n, *([n] * 12), 1, window, sinks, 1e-5) == -1
         assert lib.oxi_prefill_attn_sinks(n, *([n] * 7), 1, window, sinks) == -1
         assert lib.oxi_prefill_attn_paged_sinks(n, *([n] * 7), 1, window, sinks) == -1
 
