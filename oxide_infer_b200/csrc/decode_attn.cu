@@ -679,6 +679,7 @@ constexpr int MERGE_MAX_Y = 8;
 // kRule: how a row is cut into key ranges, and how its result is rounded
 constexpr int MERGE_WINDOW = 0;  // row_chunks; the gate on the f16 result, as the reference does
 constexpr int MERGE_SINKS = 1;   // view_chunks; the gate before the one rounding
+constexpr int MERGE_Q8 = 2;      // the 8-bit cache: groups of 8 tokens; the gate before the one rounding
 template <bool kSliced, int kRule>  // kSliced false: the workspace holds rows of at most 16 key ranges (no slice scratch)
 __global__ void __launch_bounds__(128)
 decode_merge_kernel(const DecodeParams p) {
@@ -694,7 +695,9 @@ decode_merge_kernel(const DecodeParams p) {
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.work_counter = 0u;
     if (slen == 0u || slen > p.max_seq_len || (kvp & 15ull) != 0ull) return;
     if (p.paged.block_tables && ((slen - 1u) >> p.paged.lbs) >= p.paged.max_blocks) return;
-    const uint32_t nchunks = kRule == MERGE_SINKS ? view_chunks(row_view<dec::GK>(slen, p.window, p.sinks)) : row_chunks(slen, p.window);
+    const uint32_t nchunks = kRule == MERGE_SINKS ? view_chunks(row_view<dec::GK>(slen, p.window, p.sinks))
+                             : kRule == MERGE_Q8  ? (row_view<8>(slen, p.window, p.sinks).ng + dec::CHUNK / 8 - 1) / (dec::CHUNK / 8)
+                                                  : row_chunks(slen, p.window);
     if (nchunks <= 1) return;
     const uint32_t nslices = kSliced ? (nchunks + MERGE_BLK - 1) / MERGE_BLK : 1u;
     // CTAs that work on this row and head group: several only where that saves memory round trips
@@ -895,6 +898,17 @@ cudaError_t launch_decode_attn(cudaStream_t stream, const DecodeWorkspace& ws, v
                                const uint64_t* v_ptrs, const uint32_t* seq_lens, uint32_t batch,
                                uint32_t window, uint32_t sinks) {
     return launch_decode<false, false>(stream, ws, sinks, make_params(ws, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, batch, window));
+}
+
+cudaError_t launch_decode_merge_q8(cudaStream_t stream, const DecodeWorkspace& ws, void* ctx_out, const void* gate,
+                                   const Q8Map& map, const uint32_t* seq_lens, uint32_t batch, uint32_t window,
+                                   uint32_t sinks) {
+    DecodeParams p = make_params(ws, ctx_out, nullptr, gate, nullptr, nullptr, seq_lens, batch, window);
+    p.sinks = sinks;
+    p.paged.block_tables = map.block_tables;  // which rows are valid goes by the paged layout's limits
+    p.paged.lbs = map.lbs;
+    p.paged.max_blocks = map.max_blocks;
+    return launch_merge<MERGE_Q8>(stream, ws, batch, p);
 }
 
 static void set_fused(DecodeParams& p, const void* k_in, const void* v_in, const void* q_norm_w, const void* k_norm_w,

@@ -112,6 +112,14 @@ cudaError_t launch_append_q8(cudaStream_t stream, void* q_out, const void* q_in,
                              const void* q_norm_w, const void* k_norm_w, const void* cos_t, const void* sin_t,
                              const uint32_t* pos_ids, const uint32_t* row_seq /* may be null */, const Q8Map& map,
                              uint32_t format, uint32_t rows, uint32_t max_seq_len, float eps, uint32_t* status);
+cudaError_t decode_attn_q8_init();
+cudaError_t launch_decode_attn_q8(cudaStream_t stream, const DecodeWorkspace& ws, void* ctx_out, const void* q, const void* gate,
+                                  const Q8Map& map, uint32_t format, const uint32_t* seq_lens, uint32_t batch, uint32_t window,
+                                  uint32_t sinks);
+// merges the partial results of the 8-bit decode kernel (key ranges of decode_chunk_keys() keys)
+cudaError_t launch_decode_merge_q8(cudaStream_t stream, const DecodeWorkspace& ws, void* ctx_out, const void* gate,
+                                   const Q8Map& map, const uint32_t* seq_lens, uint32_t batch, uint32_t window,
+                                   uint32_t sinks);
 cudaError_t launch_attn_q8(cudaStream_t stream, void* ctx_out, const void* q, const void* gate, const Q8Map& map, uint32_t format,
                            const uint32_t* row_seq, const uint32_t* seq_lens, uint32_t rows, uint32_t window, uint32_t sinks,
                            uint32_t max_seq_len, uint32_t* status);

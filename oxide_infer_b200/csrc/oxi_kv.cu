@@ -171,6 +171,7 @@ int32_t oxi_create(oxi_handle** out, int32_t device, uint32_t max_batch, uint32_
     }
     {
         cudaError_t e = decode_attn_init();
+        if (e == cudaSuccess) e = decode_attn_q8_init();
         if (e == cudaSuccess) e = prefill_attn_init();
         if (e == cudaSuccess) e = stream_probe_init();
         if (e == cudaSuccess) e = proj_gemm_init();
@@ -551,8 +552,8 @@ int32_t oxi_decode_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const voi
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_decode_attn_q8");
     Q8Map m;
     if (int32_t rc = paged_q8_map(layout, "oxi_decode_attn_q8: the layout or one of its pointers is null", &m)) return rc;
-    OXI_CUDA(launch_attn_q8((cudaStream_t)stream, ctx_out, q, gate, m, layout->format, nullptr, seq_lens, batch, window, sinks,
-                            h->max_seq_len, h->dws.status),
+    OXI_CUDA(launch_decode_attn_q8((cudaStream_t)stream, take_dws(h), ctx_out, q, gate, m, layout->format, seq_lens, batch, window,
+                                   sinks),
              "decode_attn_q8 launch");
     return OXI_OK;
 }
