@@ -136,7 +136,7 @@ append_q8_kernel(const AppendQ8Params p) {
     const int combo = warp & (COMBOS - 1), part = warp / COMBOS, kvh = combo & (NKV - 1);
     const bool is_v = combo >= NKV;
     float* scale_at = (is_v ? p.map.v_scales : p.map.k_scales) + (size_t)id * p.map.scale_stride + kvh;
-    const float old_scale = slot0 != 0u ? *scale_at : 0.0f;
+    const float old_scale = slot0 != 0u ? __ldcg(scale_at) : 0.0f;
     if (!is_v) load_pairs(p.k_norm_w, lane, wv);
     bool odd = false;  // some value is not a finite f16
     auto load_row = [&](uint32_t i, float (&x)[4]) {
@@ -183,7 +183,7 @@ append_q8_kernel(const AppendQ8Params p) {
     if (scale > old_scale) {  // slots before the segment move to the larger scale
         for (uint32_t t = part; t < slot0; t += PARTS) {
             uint32_t* at = reinterpret_cast<uint32_t*>(base + (size_t)t * Q8_ROW_BYTES) + lane;
-            const uint32_t w = *at;
+            const uint32_t w = __ldcg(at);
             uint32_t o = 0;
 #pragma unroll
             for (int j = 0; j < 4; j++) o |= q8_code<kFmt>(q8_value<kFmt>((w >> (8 * j)) & 0xffu) * old_scale, div) << (8 * j);

@@ -81,7 +81,11 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
                                 const PrefillSplitWs* split = nullptr /* key-range split of small waves */,
                                 uint32_t part_keys = 0 /* keys per part; 0: no split */,
                                 const PrefillSlab* slab = nullptr /* K/V rows inside it are loaded by TMA */,
-                                const WaitFault* fault = nullptr /* test support: a K tile of CTA 0 goes missing */);
+                                const WaitFault* fault = nullptr /* test support: a K tile of CTA 0 goes missing */,
+                                uint32_t sinks = 0 /* first tokens that stay visible behind the window */,
+                                uint32_t max_seq_len = 0 /* with sinks or q8: longer rows are skipped */,
+                                const Q8Map* q8 = nullptr /* 8-bit cache: k_ptrs, v_ptrs and pm unused */,
+                                uint32_t format = 0 /* of q8 */);
 size_t prefill_split_slot_bytes();   // partial-result bytes per slot of PrefillSplitWs::part
 size_t prefill_split_table_bytes();  // bytes of PrefillSplitWs::units
 
@@ -120,12 +124,6 @@ cudaError_t launch_decode_attn_q8(cudaStream_t stream, const DecodeWorkspace& ws
 cudaError_t launch_decode_merge_q8(cudaStream_t stream, const DecodeWorkspace& ws, void* ctx_out, const void* gate,
                                    const Q8Map& map, const uint32_t* seq_lens, uint32_t batch, uint32_t window,
                                    uint32_t sinks);
-cudaError_t launch_attn_q8(cudaStream_t stream, void* ctx_out, const void* q, const void* gate, const Q8Map& map, uint32_t format,
-                           const uint32_t* row_seq, const uint32_t* seq_lens, uint32_t rows, uint32_t window, uint32_t sinks,
-                           uint32_t max_seq_len, uint32_t* status);
-cudaError_t launch_attn_sinks(cudaStream_t stream, void* ctx_out, const void* q, const void* gate, const uint64_t* k_ptrs,
-                              const uint64_t* v_ptrs, const PagedMap* pm, const uint32_t* row_seq, const uint32_t* seq_lens,
-                              uint32_t rows, uint32_t window, uint32_t sinks, uint32_t max_seq_len, uint32_t* status);
 
 // Projection GEMM (tcgen05) with the append operator as its epilogue, and the same GEMM as a plain linear layer.
 cudaError_t proj_gemm_init();

@@ -55,6 +55,7 @@
 // writing output and reports OXI_DEV_WAIT_TIMEOUT in the status word.
 #include "common.cuh"
 #include "kernels.h"
+#include "q8.cuh"
 #include "tc5.cuh"
 
 namespace oxi {
@@ -73,7 +74,11 @@ constexpr int NS = 4;                        // ring stages, for K and for V
 constexpr int DEPTH = 3;                     // tiles a loader keeps in flight
 constexpr int Q_SUB = M * ROW_B;             // one 64-dim half of a query tile in shared memory: 16 KB
 constexpr int Q_BYTES = 2 * Q_SUB;           // 32 KB
+constexpr int STG_TILE = TK * HD;            // a K (or V) tile of 8-bit codes as it arrives: 8 KB
+constexpr int STG = 3;                       // such tiles a loader has in flight
+constexpr int SCL = 8;                       // tiles whose scales are in shared memory (the softmax lags the loader by fewer)
 constexpr size_t SMEM_BYTES = 1024 + Q_BYTES + 2 * NS * KV_TILE;  // + slack for 1024-byte alignment; > half an SM: one CTA per SM
+constexpr size_t SMEM_BYTES_Q8 = SMEM_BYTES + 2 * STG * STG_TILE;
 constexpr uint32_t TMEM_COLS = 512;
 // Q_0 (64) | S_0 S_1 (64 each) | P_0 P_1 (32 each) | O_0 O_1 (128 each); Q_1 does not fit and stays in shared memory
 constexpr uint32_t Q0_COL = 0, S_COL = 64, P_COL = 192, O_COL = 256;  // S + j*64, P + j*32, O + j*128 for query tile j
@@ -103,11 +108,40 @@ struct PfSplit {
     uint32_t target_items;  // items the wave should not exceed (the SM count)
 };
 
+// Sliding window with sinks and the 8-bit cache (kSinks, kFmt of the kernel).
+struct PfView {
+    uint32_t sinks;        // first tokens that stay visible behind the window
+    uint32_t max_seq_len;  // longer rows are skipped
+    const float* k_scales; // 8-bit cache: block i's scales at + i * scale_stride
+    const float* v_scales;
+    uint64_t scale_stride;
+};
+// The 64-key tiles of a run whose rows' windows start at `wlo` or later and whose tokens end at hi: nst tiles of
+// sinks from token 0, then tiles from token lo on.  Tiles of the 8-bit cache start at a multiple of 16 tokens, so
+// that 16 keys of a tile share a block.
+struct PfTiles {
+    uint32_t nst, lo, n;
+    __device__ __forceinline__ uint32_t first_key(uint32_t tile) const { return tile < nst ? tile * pf::TK : lo + (tile - nst) * pf::TK; }
+};
+template <bool kView, bool kAlign>
+__device__ __forceinline__ PfTiles pf_tiles(uint32_t wlo, uint32_t hi, uint32_t sinks) {
+    PfTiles t;
+    t.nst = 0;
+    t.lo = wlo;
+    if (kView) {
+        t.nst = (min(sinks, wlo) + pf::TK - 1) / pf::TK;
+        if (t.nst * pf::TK >= wlo) t.nst = t.lo = 0u;  // the sinks reach the window
+        if (kAlign) t.lo &= ~15u;
+    }
+    t.n = hi > wlo ? t.nst + (hi - t.lo + pf::TK - 1) / pf::TK : 0u;
+    return t;
+}
+
 // Orders the 64-row blocks of the wave by decreasing work (key tiles to scan) with a counting
 // sort, so that the persistent CTAs of the main kernel claim the longest items first, and
 // resets the claim counter.  One CTA.
 __global__ void __launch_bounds__(1024)
-prefill_plan_kernel(const uint32_t* __restrict__ seq_lens, uint32_t rows, uint32_t window,
+prefill_plan_kernel(const uint32_t* __restrict__ seq_lens, uint32_t rows, uint32_t window, uint32_t sinks,
                     uint32_t* __restrict__ order, uint32_t* __restrict__ counter) {
     using namespace pf;
     constexpr int NB = 1024;
@@ -128,7 +162,7 @@ prefill_plan_kernel(const uint32_t* __restrict__ seq_lens, uint32_t rows, uint32
             lo = min(lo, window_start(sl, window));
             hi = max(hi, sl);
         }
-        const uint32_t tiles = hi > lo ? (hi - lo + TK - 1) / TK : 0u;
+        const uint32_t tiles = hi > lo ? pf_tiles<true, false>(lo, hi, sinks).n : 0u;
         return (uint32_t)(NB - 1) - min(tiles, (uint32_t)(NB - 1));  // bucket 0 = most work
     };
     uint32_t my_key[4];  // keys of this thread's first blocks are kept for the scatter pass
@@ -174,7 +208,7 @@ prefill_plan_kernel(const uint32_t* __restrict__ seq_lens, uint32_t rows, uint32
 // atomics, and every block finds its rank by counting the blocks with more work.  Lets the
 // attention kernel, launched as a programmatic dependent, run its prologue meanwhile.
 __global__ void __launch_bounds__(1024)
-prefill_plan_small_kernel(const uint32_t* __restrict__ seq_lens, uint32_t rows, uint32_t window,
+prefill_plan_small_kernel(const uint32_t* __restrict__ seq_lens, uint32_t rows, uint32_t window, uint32_t sinks,
                           uint32_t* __restrict__ order, uint32_t* __restrict__ counter, const PfSplit sp) {
     using namespace pf;
     __shared__ uint32_t s_lo[1024], s_hi[1024], s_key[1024], s_ns[1024];
@@ -198,7 +232,7 @@ prefill_plan_small_kernel(const uint32_t* __restrict__ seq_lens, uint32_t rows, 
     uint32_t key = 0, ns = 1;
     if (tid < nblocks) {
         const uint32_t lo = s_lo[tid], hi = s_hi[tid];
-        key = hi > lo ? (hi - lo + TK - 1) / TK : 0u;
+        key = hi > lo ? pf_tiles<true, false>(lo, hi, sinks).n : 0u;
     }
     if (sp.part_tiles != 0u) {
         // Part size: the smallest P >= part_tiles with sum_b ceil(tiles_b / P) * 4 <= target_items and
@@ -208,7 +242,7 @@ prefill_plan_small_kernel(const uint32_t* __restrict__ seq_lens, uint32_t rows, 
             uint32_t tb = 0u;
             if (tid + 32 < nblocks) {
                 const uint32_t lo2 = s_lo[tid + 32], hi2 = s_hi[tid + 32];
-                tb = hi2 > lo2 ? (hi2 - lo2 + TK - 1) / TK : 0u;
+                tb = hi2 > lo2 ? pf_tiles<true, false>(lo2, hi2, sinks).n : 0u;
             }
             uint32_t tmax = max(t0, tb);
 #pragma unroll
@@ -298,7 +332,15 @@ __device__ __forceinline__ bool pf_next_run(uint32_t& next, uint32_t nruns, cons
 // instantiations carry none of it: the loop is sensitive to a few instructions in its waits and hand-overs
 // (measured 3-5 % on the 4,096-row wave), and there a wait only runs out after an internal error, which the
 // status word reports.
-template <bool kPaged, bool kSplit, bool kTma, bool kFault>
+// kSinks: the window leaves the first tokens visible (PfView); a run's tiles are then PfTiles, keys that no row of the
+// run sees are zero-filled, and the gate is applied before the one rounding of the result.
+// kFmt (with kPaged and kSinks): the 8-bit cache.  The loader warps bring codes into a staging ring (half the bytes
+// from L2) and convert them to the f16 tiles of the ring, exactly: scales never enter the operands.  A tile's four
+// 16-key groups have one K scale and one V scale each; the softmax multiplies the scores of a group by its K scale in
+// the fma that it does anyway and adds log2 of the V scale to the exponent, so that P carries the V scales, and the
+// row sum takes each group's partial sum times 1 / (V scale): 8 instructions a tile more than the f16 cache.
+constexpr uint32_t PF_F16 = 0, PF_INT8 = 1, PF_E4M3 = 2;
+template <bool kPaged, bool kSplit, bool kTma, bool kFault, bool kSinks = false, uint32_t kFmt = PF_F16>
 __global__ void __launch_bounds__(pf::THREADS, 1)
 prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__ q,
                     const uint16_t* __restrict__ gate, const uint64_t* __restrict__ k_ptrs,
@@ -307,8 +349,13 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                     const uint32_t* __restrict__ order, uint32_t* __restrict__ counter,
                     const PagedMap pm, const uint32_t* __restrict__ row_seq, const PfSplit sp,
                     const __grid_constant__ TmaDesc tmap, const uint64_t slab_base, const uint32_t slab_rows,
-                    const WaitFault fault) {
+                    const WaitFault fault, const PfView view) {
     using namespace pf;
+    constexpr bool kQ8 = kFmt != PF_F16;
+    constexpr uint32_t kCodes = kFmt == PF_INT8 ? Q8_INT8 : Q8_E4M3;
+    constexpr int ROWB = kQ8 ? Q8_ROW_BYTES : KV_ROW_BYTES;
+    static_assert(!kQ8 || (kPaged && kSinks && !kTma && !kFault), "variants of the 8-bit cache");
+    auto tiles_of = [&](const PfRun& r) { return pf_tiles<kSinks, kQ8>(r.lo, r.hi, view.sinks); };
     const uint32_t wait_us = kFault ? fault.limit_us : WAIT_LIMIT_US;
     // paged K/V: k_ptrs / v_ptrs are unused, wave row r reads row row_seq[r] of pm.block_tables
     constexpr bool paged = kPaged;
@@ -326,9 +373,12 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
     __shared__ __align__(8) uint64_t bar_sfull[2], bar_sfree[2], bar_pfull[2], bar_pvdone[2], bar_qfull[2], bar_ofull[2];
     __shared__ __align__(8) uint64_t bar_tok[2];  // issue token of MMA warp j
     __shared__ uint32_t s_tmem, s_abort, s_item[2], s_unit[2];
+    // 8-bit cache: scales of a tile's four groups as they arrive (K, then V; all heads), and what the softmax uses:
+    // K scale * log2e / sqrt(128), log2 V scale, 1 / V scale
+    __shared__ __align__(16) float s_raw[kQ8 ? SCL : 1][8][4], s_scl[kQ8 ? SCL : 1][3][4];
 
     const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;  // 1024-byte aligned tiles
-    const uint32_t q1_s = sbase, k_s = sbase + Q_BYTES, v_s = k_s + NS * KV_TILE;
+    const uint32_t q1_s = sbase, k_s = sbase + Q_BYTES, v_s = k_s + NS * KV_TILE, stg_s = v_s + NS * KV_TILE;
     const int tid = threadIdx.x, lane = tid & 31;
     // warp index the compiler can prove uniform: role branches and MMA issue stay in uniform control flow
     const int warp_u = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -410,7 +460,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                 if (((kp[hf] | vp[hf]) & 15ull) != 0ull) {
                     if (kvh == 0) atomicOr(status, DEV_MISALIGNED_PTR);
                     sl[hf] = 0;
-                } else if (sl[hf] == 0u || too_long) {
+                } else if (sl[hf] == 0u || too_long || (kSinks && sl[hf] > view.max_seq_len)) {
                     if (kvh == 0) atomicOr(status, DEV_BAD_SEQ_LEN);
                     sl[hf] = 0;
                 }
@@ -494,7 +544,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
     if (kSplit) {
         uint32_t gt = 0, next = 0;
         PfRun run;
-        while (pf_next_run(next, nruns, c_runs, run)) gt += (run.hi - run.lo + TK - 1) / TK;
+        while (pf_next_run(next, nruns, c_runs, run)) gt += tiles_of(run).n;
         t_lo = (uint32_t)((uint64_t)gt * part / nparts);
         t_hi = (uint32_t)((uint64_t)gt * (part + 1u) / nparts);
     }
@@ -556,7 +606,8 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             // key range that is valid for every row of this query tile (mask-free tiles)
             const uint32_t lo_max = c_tile[j][0], hi_min = c_tile[j][1];
             const bool full = run.r0 <= (uint32_t)(j * TOK) && run.r1 >= (uint32_t)(j * TOK + TOK) && c_tile[j][2] != 0u;
-            const uint32_t ntiles = (run.hi - run.lo + TK - 1) / TK;
+            const PfTiles tl = tiles_of(run);
+            const uint32_t ntiles = tl.n;
             uint32_t tile0 = 0, tile1 = ntiles;  // this unit's tiles of the run
             if (kSplit) {
                 tile0 = min(ntiles, max(t_lo, tflat) - tflat);
@@ -567,44 +618,70 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                 ok &= mbar_wait_bounded(&bar_sfull[j], gk & 1u, &s_abort, wait_us);  // S_j(tile) complete
                 __syncwarp();
                 tc_fence_after();
-                const uint32_t kbeg = run.lo + tile * TK;
+                const uint32_t kbeg = tl.first_key(tile);
                 uint32_t sr[2][32];
                 tmem_ld32(s_t, sr[0]);
                 tmem_ld32(s_t + 32, sr[1]);
                 tmem_wait_ld();
                 tc_fence_before();
+                float xs[4], lv[4], iv[4];  // 8-bit cache: the tile's scales (before S_j is handed back: see SCL)
+                if (kQ8) {
+#pragma unroll
+                    for (int b = 0; b < 4; b++) {
+                        xs[b] = s_scl[gk % SCL][0][b];
+                        lv[b] = s_scl[gk % SCL][1][b];
+                        iv[b] = s_scl[gk % SCL][2][b];
+                    }
+                }
                 mbar_arrive(&bar_sfree[j]);  // the next tile's scores may overwrite S_j now
                 // PV_j of the tile before has long completed as a rule: polled here, needed before P is stored
                 const bool pv_prev_done = mbar_try_wait(&bar_pvdone[j], (gk - 1u) & 1u);
-                const bool interior = full && kbeg >= lo_max && kbeg + TK <= hi_min;
+                const bool interior = full && kbeg + TK <= hi_min && (kbeg >= lo_max || (kSinks && kbeg + TK <= view.sinks));
                 float mxa[4] = {-1.0e30f, -1.0e30f, -1.0e30f, -1.0e30f};
                 if (interior) {
 #pragma unroll
-                    for (int c = 0; c < TK; c++) mxa[c & 3] = fmaxf(mxa[c & 3], __uint_as_float(sr[c >> 5][c & 31]));
+                    for (int c = 0; c < TK; c++) {
+                        const int m = kQ8 ? c >> 4 : c & 3;  // 8-bit cache: a maximum for each group
+                        mxa[m] = fmaxf(mxa[m], __uint_as_float(sr[c >> 5][c & 31]));
+                    }
                 } else {
 #pragma unroll
                     for (int c = 0; c < TK; c++) {
                         const uint32_t key = kbeg + c;
                         float v = __uint_as_float(sr[c >> 5][c & 31]);
-                        v = (key >= rlo && key < rhi) ? v : -INFINITY;
+                        v = ((key >= rlo || (kSinks && key < view.sinks)) && key < rhi) ? v : -INFINITY;
                         sr[c >> 5][c & 31] = __float_as_uint(v);
-                        mxa[c & 3] = fmaxf(mxa[c & 3], v);
+                        const int m = kQ8 ? c >> 4 : c & 3;
+                        mxa[m] = fmaxf(mxa[m], v);
                     }
                 }
+                if (kQ8) {
+#pragma unroll
+                    for (int b = 0; b < 4; b++) mxa[b] = mxa[b] > -1.0e29f ? fmaf(mxa[b], xs[b], lv[b]) : -1.0e30f;
+                }
                 float mx = fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3]));
-                mx = mx > -1.0e29f ? mx * QK_SCALE_LOG2 : -1.0e30f;  // stays -1e30 when the whole row is masked
+                if (!kQ8) mx = mx > -1.0e29f ? mx * QK_SCALE_LOG2 : -1.0e30f;  // stays -1e30 when the whole row is masked
                 const bool raise = mx > m_ref + RESCALE_THRESHOLD;
                 const float corr = raise ? ex2_approx_ftz(m_ref - mx) : 1.0f;
                 if (raise) m_ref = mx;
                 float psa[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 uint32_t pk[32];
                 const float neg_m = -m_ref;
+                if (kQ8) {
+#pragma unroll
+                    for (int b = 0; b < 4; b++) lv[b] += neg_m;
+                }
 #pragma unroll
                 for (int c = 0; c < TK; c += 2) {  // p = 2^(s*scale*log2e - m): one fma + one ex2 per key
-                    const float p0 = ex2_approx_ftz(fmaf(__uint_as_float(sr[c >> 5][c & 31]), QK_SCALE_LOG2, neg_m));
-                    const float p1 = ex2_approx_ftz(fmaf(__uint_as_float(sr[(c + 1) >> 5][(c + 1) & 31]), QK_SCALE_LOG2, neg_m));
-                    psa[(c >> 1) & 3] += p0 + p1;
+                    const float mul = kQ8 ? xs[c >> 4] : QK_SCALE_LOG2, add = kQ8 ? lv[c >> 4] : neg_m;
+                    const float p0 = ex2_approx_ftz(fmaf(__uint_as_float(sr[c >> 5][c & 31]), mul, add));
+                    const float p1 = ex2_approx_ftz(fmaf(__uint_as_float(sr[(c + 1) >> 5][(c + 1) & 31]), mul, add));
+                    psa[kQ8 ? c >> 4 : (c >> 1) & 3] += p0 + p1;
                     pk[c >> 1] = pack_h2(p0, p1);
+                }
+                if (kQ8) {
+#pragma unroll
+                    for (int b = 0; b < 4; b++) psa[b] *= iv[b];
                 }
                 l_run = l_run * corr + ((psa[0] + psa[1]) + (psa[2] + psa[3]));
                 // P_j and O_j are free once PV_j of the tile before is complete (first tile of the CTA: passes)
@@ -672,9 +749,10 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             // nothing is written once a wait of this thread gave up (kFault: or any wait of the CTA - the MMA warp
             // then withholds bar_ofull, so the wait above has failed too)
             const bool write = OXI_IN_BOUNDS(row0 + tok < rows || tok >= nrows, status) && tok < nrows && c_len[tok] != 0 && ok;
-            const float inv = rcp_approx_ftz(l_run);
+            float inv = rcp_approx_ftz(l_run);
             const size_t rh = (size_t)(row0 + (write ? tok : 0u)) * NQ + head;
             const float sig = (gate && write) ? sigmoid_ref(h2f(gate[rh])) : 1.0f;
+            if (kSinks) inv *= sig;
             uint4* out = reinterpret_cast<uint4*>(ctx_out + rh * HD);
 #pragma unroll
             for (int ch = 0; ch < 4; ch++) {
@@ -689,7 +767,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                         for (int jj = 0; jj < 4; jj++) {
                             uint16_t h0 = f2h(__fmul_rn(__uint_as_float(orow[v8 * 8 + 2 * jj]), inv));
                             uint16_t h1 = f2h(__fmul_rn(__uint_as_float(orow[v8 * 8 + 2 * jj + 1]), inv));
-                            if (gate) {
+                            if (!kSinks && gate) {
                                 h0 = f2h(__fmul_rn(h2f(h0), sig));
                                 h1 = f2h(__fmul_rn(h2f(h1), sig));
                             }
@@ -787,7 +865,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             uint32_t next = 0;
             PfRun run;
             while (pf_next_run(next, nruns, c_runs, run)) {
-                const uint32_t ntiles = (run.hi - run.lo + TK - 1) / TK;
+                const uint32_t ntiles = tiles_of(run).n;
                 for (uint32_t tile = 0; tile < ntiles; tile++) {
                     step(nt, nt >= 2, true, false);
                     ++nt;
@@ -816,13 +894,53 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             if (kFault && is_k && blockIdx.x == 0 && g + 1u == fault.skip_plus1) return;
             mbar_arrive(&full[g % NS]);
         };
+        // 8-bit cache: tile number g from the staging ring into the f16 ring.  A lane converts the 16-byte chunks that it
+        // copied itself: chunk cq of rows rq, rq + 4, ... becomes chunks 2 cq and 2 cq + 1 of the f16 row; lanes of the
+        // two 64-dim halves store them in opposite order, so the 8 lanes of a store phase fall in distinct banks.
+        const uint32_t cq = lane & 7u, rq = lane >> 3;
+        const uint32_t stg = stg_s + (is_k ? 0u : (uint32_t)(STG * STG_TILE));
+        auto convert = [&](uint32_t g) {
+            const uint32_t st = g % NS;
+            ok &= mbar_wait_bounded(&empty[st], ((g / NS) & 1u) ^ 1u, &s_abort, wait_us);
+            __syncwarp();
+            const uint32_t src = stg + (g % STG) * STG_TILE + rq * HD + cq * 16;
+            const uint32_t dst = ring + st * KV_TILE + (cq >> 2) * KV_SUB;
+            const uint32_t odd = cq >> 2;  // 1: the odd chunk first
+            const uint32_t ch = (2u * cq) & 7u;
+#pragma unroll 4
+            for (int k = 0; k < TK / 4; k++) {
+                const uint32_t row = rq + 4 * k;
+                uint32_t w[4], h[8];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src + k * 4 * HD) : "memory");
+#pragma unroll
+                for (int i = 0; i < 4; i++) codes_to_f16<kCodes>(w[i], h[2 * i], h[2 * i + 1]);
+#pragma unroll
+                for (uint32_t i = 0; i < 2; i++) {
+                    const bool hi = (i ^ odd) != 0u;
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + row * ROW_B + (((ch + (hi ? 1u : 0u)) ^ (row & 7u)) << 4)),
+                                 "r"(hi ? h[4] : h[0]), "r"(hi ? h[5] : h[1]), "r"(hi ? h[6] : h[2]), "r"(hi ? h[7] : h[3]) : "memory");
+                }
+            }
+            if (is_k && lane < 4) {
+                const float ks = s_raw[g % SCL][lane][kvh], vs = s_raw[g % SCL][4 + lane][kvh];
+                const float l2 = fminf(fmaxf(__log2f(vs), -100.0f), 100.0f);  // finite even for the scale of a block without visible keys
+                s_scl[g % SCL][0][lane] = fmaxf(ks * QK_SCALE_LOG2, 1.0e-30f);  // a masked score stays -inf under a zero scale
+                s_scl[g % SCL][1][lane] = l2;
+                s_scl[g % SCL][2][lane] = exp2f(-l2);
+            }
+            fence_proxy_async_smem();
+            publish(g);
+        };
         uint32_t tflat = 0;    // tiles of the block's runs before this one (key-range split)
         uint32_t next = 0;
         PfRun run;
         while (pf_next_run(next, nruns, c_runs, run)) {
-            const char* base = paged ? reinterpret_cast<const char*>(is_k ? pm.k_pool : pm.v_pool) + kvh * (HD * 2)
+            const char* base = paged ? reinterpret_cast<const char*>(is_k ? pm.k_pool : pm.v_pool) + kvh * (ROWB / NKV)
                                      : reinterpret_cast<const char*>(is_k ? c_kp[run.r0] : c_vp[run.r0]) + kvh * (HD * 2);
-            const uint32_t ntiles = (run.hi - run.lo + TK - 1) / TK;
+            const PfTiles tl = tiles_of(run);
+            const uint32_t ntiles = tl.n;
+            // keys that no row of the run sees are zero-filled
+            auto seen = [&](uint32_t tkn) { return tkn < run.hi && (!kSinks || tkn >= run.lo || tkn < view.sinks); };
             // paged: lane l holds the block of page (tile's first page + l); a 64-key tile spans at most 5
             // blocks of >= 16 tokens; the next tile's entries are fetched while this tile is copied
             const uint32_t* trow = paged ? pm.block_tables + (size_t)((c_kp[run.r0] >> 4) - 1ull) * pm.max_blocks : nullptr;
@@ -845,7 +963,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                 tile1 = min(ntiles, max(t_hi, tflat) - tflat);
                 tflat += ntiles;
             }
-            uint32_t pg_next = (paged && tile0 < tile1) ? fetch_pages(run.lo + tile0 * TK) : 0u;
+            uint32_t pg_next = (paged && tile0 < tile1) ? fetch_pages(tl.first_key(tile0)) : 0u;
             // Rows of a registered slab (at a whole number of 1024-byte rows from its base) come through the
             // TMA unit: two boxes per full tile, written in the same swizzled layout, completion counted on
             // the stage's barrier.  The run's ragged last tile keeps the zero-filling copies below.
@@ -863,10 +981,42 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                 }
             }
             for (uint32_t tile = tile0; tile < tile1; tile++) {
+                if (kQ8) {
+                    // four groups of 16 keys, each inside one block; lanes 0-3 (4-7) also bring the groups' K (V) scales
+                    const uint32_t kbeg = tl.first_key(tile), p0 = kbeg >> pm.lbs, mask = (1u << pm.lbs) - 1u;
+                    const uint32_t pg_cur = pg_next;
+                    if (tile + 1 < tile1) pg_next = fetch_pages(tl.first_key(tile + 1));
+                    const uint32_t dst = stg + (gk % STG) * STG_TILE + rq * HD + cq * 16;
+                    uint64_t off[4];
+#pragma unroll
+                    for (int b = 0; b < 4; b++) {
+                        const uint32_t t = kbeg + 16 * b;
+                        const uint32_t pid = __shfl_sync(0xffffffffu, pg_cur, ((t >> pm.lbs) - p0) & 31u);
+                        off[b] = (uint64_t)pid * pm.block_stride + (uint64_t)(t & mask) * ROWB;
+                        if (is_k && (lane & 3) == b && lane < 8)
+                            cp_async_16(smem_u32(&s_raw[gk % SCL][lane][0]), (lane < 4 ? view.k_scales : view.v_scales) + (uint64_t)pid * view.scale_stride,
+                                        t < run.hi);
+                    }
+#pragma unroll
+                    for (int k = 0; k < TK / 4; k++) {
+                        const uint32_t row = rq + 4 * k;
+                        const bool valid = seen(kbeg + row);
+                        cp_async_16(dst + k * 4 * HD, valid ? base + off[k >> 2] + (row & 15u) * ROWB + cq * 16 : base, valid);
+                    }
+                    cp_async_commit();
+                    ++pending;
+                    ++gk;
+                    if (pending == STG) {
+                        cp_async_wait<STG - 1>();
+                        convert(gk - STG);
+                        --pending;
+                    }
+                    continue;
+                }
                 const uint32_t st = gk % NS;
                 // the MMAs that read this stage's previous tile have completed (first use: passes at once)
                 ok &= mbar_wait_bounded(&empty[st], ((gk / NS) & 1u) ^ 1u, &s_abort, wait_us);
-                const uint32_t kbeg = run.lo + tile * TK;
+                const uint32_t kbeg = tl.first_key(tile);
                 if (kTma && tma_run && kbeg + TK <= run.hi) {
                     if (lane == 0 && ok) {  // after a wait gave up nothing more is copied
                         mbar_arrive_expect_tx(&full[st], (uint32_t)KV_TILE);
@@ -882,18 +1032,18 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                 const char* src = base + (size_t)(kbeg + r0) * KV_ROW_BYTES + c * 16;
                 if (paged) {
                     const uint32_t pg_cur = pg_next;
-                    if (tile + 1 < tile1) pg_next = fetch_pages(kbeg + TK);
+                    if (tile + 1 < tile1) pg_next = fetch_pages(tl.first_key(tile + 1));
                     const uint32_t p0 = kbeg >> pm.lbs, mask = (1u << pm.lbs) - 1u;
 #pragma unroll 8
                     for (int k = 0; k < TK / 2; k++) {
                         const uint32_t row = r0 + 2 * k, tkn = kbeg + row;
                         const uint32_t pid = __shfl_sync(0xffffffffu, pg_cur, ((tkn >> pm.lbs) - p0) & 31u);
-                        const bool valid = tkn < run.hi;  // rows past the run's last key are zero-filled
+                        const bool valid = seen(tkn);  // rows past the run's last key are zero-filled
                         cp_async_16(dst + row * ROW_B + (((c & 7u) ^ (row & 7u)) << 4),
                                     valid ? base + (size_t)pid * pm.block_stride + (size_t)(tkn & mask) * KV_ROW_BYTES + c * 16 : base,
                                     valid);
                     }
-                } else if (kbeg + TK <= run.hi) {
+                } else if (kbeg + TK <= run.hi && (!kSinks || kbeg >= run.lo || kbeg + TK <= view.sinks)) {
 #pragma unroll
                     for (int k = 0; k < TK / 2; k++) {
                         const uint32_t row = r0 + 2 * k;
@@ -903,7 +1053,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
 #pragma unroll
                     for (int k = 0; k < TK / 2; k++) {
                         const uint32_t row = r0 + 2 * k;
-                        const bool valid = kbeg + row < run.hi;  // rows past the run's last key are zero-filled
+                        const bool valid = seen(kbeg + row);  // rows past the run's last key are zero-filled
                         cp_async_16(dst + row * ROW_B + (((c & 7u) ^ (row & 7u)) << 4),
                                     valid ? src + (size_t)k * 2 * KV_ROW_BYTES : base, valid);
                     }
@@ -925,8 +1075,12 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             }
         }
         cp_async_wait<0>();
-        fence_proxy_async_smem();
-        for (; pending > 0; --pending) publish(gk - pending);
+        if (kQ8) {
+            for (; pending > 0; --pending) convert(gk - pending);
+        } else {
+            fence_proxy_async_smem();
+            for (; pending > 0; --pending) publish(gk - pending);
+        }
         // all tiles of this item are on their way to the tensor core: claim the next item and prepare its
         // tables while the other roles work through the last tiles
         if (is_k) prepare_item(buf ^ 1u);
@@ -947,6 +1101,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
 // of a row holds O_s = sum_k 2^(x_k - m_s) v_k and l_s = sum_k 2^(x_k - m_s); the row's result is
 // sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s with m = max_s m_s, rounded to f16 and gated like
 // the unsplit epilogue.
+template <bool kOnce>  // the gate before the one rounding (kSinks), else on the f16 result
 __global__ void __launch_bounds__(128)
 prefill_merge_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__ gate,
                      uint32_t rows, const PfSplit sp) {
@@ -1001,11 +1156,12 @@ prefill_merge_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict_
             acc.w = fmaf(w[u], o[u].w, acc.w);
         }
     }
-    const float inv = rcp_approx_ftz(lsum);
+    float inv = rcp_approx_ftz(lsum);
     const size_t rh = (size_t)(row0 + tok) * NQ + head;
+    if (kOnce && gate) inv *= sigmoid_ref(h2f(gate[rh]));
     uint16_t h[4] = {f2h(__fmul_rn(acc.x, inv)), f2h(__fmul_rn(acc.y, inv)), f2h(__fmul_rn(acc.z, inv)),
                      f2h(__fmul_rn(acc.w, inv))};
-    if (gate) {
+    if (!kOnce && gate) {
         const float sig = sigmoid_ref(h2f(gate[rh]));
 #pragma unroll
         for (int e = 0; e < 4; e++) h[e] = f2h(__fmul_rn(h2f(h[e]), sig));
@@ -1017,10 +1173,10 @@ prefill_merge_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict_
 size_t prefill_split_table_bytes() { return (size_t)3 * 1024 * PF_MAX_SPLIT * sizeof(uint32_t); }
 size_t prefill_split_slot_bytes() { return (size_t)NKV * 2 * pf::M * (HD + 2) * sizeof(float); }
 
-template <bool kPaged, bool kSplit, bool kTma, bool kFault = false>
+template <bool kPaged, bool kSplit, bool kTma, bool kFault = false, bool kSinks = false, uint32_t kFmt = PF_F16>
 static cudaError_t pf_set_smem() {
-    return cudaFuncSetAttribute(prefill_attn_kernel<kPaged, kSplit, kTma, kFault>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)pf::SMEM_BYTES);
+    return cudaFuncSetAttribute(prefill_attn_kernel<kPaged, kSplit, kTma, kFault, kSinks, kFmt>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)(kFmt != PF_F16 ? pf::SMEM_BYTES_Q8 : pf::SMEM_BYTES));
 }
 
 cudaError_t prefill_attn_init() {
@@ -1031,18 +1187,28 @@ cudaError_t prefill_attn_init() {
     if ((e = pf_set_smem<true, true, false>())) return e;
     if ((e = pf_set_smem<false, false, true>())) return e;
     if ((e = pf_set_smem<false, false, false, true>())) return e;
+    if ((e = pf_set_smem<false, false, false, false, true>())) return e;
+    if ((e = pf_set_smem<true, false, false, false, true>())) return e;
+    if ((e = pf_set_smem<false, true, false, false, true>())) return e;
+    if ((e = pf_set_smem<true, true, false, false, true>())) return e;
+    if ((e = pf_set_smem<true, false, false, false, true, PF_INT8>())) return e;
+    if ((e = pf_set_smem<true, true, false, false, true, PF_INT8>())) return e;
+    if ((e = pf_set_smem<true, false, false, false, true, PF_E4M3>())) return e;
+    if ((e = pf_set_smem<true, true, false, false, true, PF_E4M3>())) return e;
     return pf_set_smem<false, true, true>();
 }
 
-template <bool kPaged, bool kSplit, bool kTma, bool kFault = false>
+template <bool kPaged, bool kSplit, bool kTma, bool kFault = false, bool kSinks = false, uint32_t kFmt = PF_F16>
 static cudaError_t launch_pf(cudaStream_t stream, uint32_t grid, void* ctx_out, const void* q, const void* gate,
                              const uint64_t* k_ptrs, const uint64_t* v_ptrs, const uint32_t* seq_lens, uint32_t rows,
                              uint32_t window, uint32_t* status, uint32_t* order, uint32_t* counter, const PagedMap& pm,
-                             const uint32_t* row_seq, const PfSplit& sp, const PrefillSlab& slab, const WaitFault& fault) {
+                             const uint32_t* row_seq, const PfSplit& sp, const PrefillSlab& slab, const WaitFault& fault,
+                             const PfView& view) {
     // programmatic dependent of the plan kernel: TMEM allocation and barrier set-up overlap it
-    return launch_pdl(prefill_attn_kernel<kPaged, kSplit, kTma, kFault>, dim3(grid), dim3(pf::THREADS), pf::SMEM_BYTES, stream,
+    return launch_pdl(prefill_attn_kernel<kPaged, kSplit, kTma, kFault, kSinks, kFmt>, dim3(grid), dim3(pf::THREADS),
+                      kFmt != PF_F16 ? pf::SMEM_BYTES_Q8 : pf::SMEM_BYTES, stream,
                       (uint16_t*)ctx_out, (const uint16_t*)q, (const uint16_t*)gate, k_ptrs, v_ptrs, seq_lens, rows,
-                      window, status, (const uint32_t*)order, counter, pm, row_seq, sp, slab.map, slab.base, slab.rows, fault);
+                      window, status, (const uint32_t*)order, counter, pm, row_seq, sp, slab.map, slab.base, slab.rows, fault, view);
 }
 
 cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* q,
@@ -1050,12 +1216,19 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
                                 const uint32_t* seq_lens, uint32_t rows, uint32_t window,
                                 uint32_t* status, int num_sms, uint32_t* order, uint32_t* counter,
                                 const PagedMap* pm, const uint32_t* row_seq, const PrefillSplitWs* ws,
-                                uint32_t part_keys, const PrefillSlab* slab, const WaitFault* fault) {
+                                uint32_t part_keys, const PrefillSlab* slab, const WaitFault* fault, uint32_t sinks,
+                                uint32_t max_seq_len, const Q8Map* q8, uint32_t format) {
+    const PfView view{sinks, max_seq_len, q8 ? q8->k_scales : nullptr, q8 ? q8->v_scales : nullptr, q8 ? q8->scale_stride : 0};
+    PagedMap q8pm{};
+    if (q8) {
+        q8pm = PagedMap{q8->k_pool, q8->v_pool, q8->block_tables, q8->block_stride, q8->max_blocks, q8->lbs, q8->num_blocks};
+        pm = &q8pm;
+    }
     const WaitFault flt = fault ? *fault : WaitFault{};
     const uint32_t nblocks = (rows + pf::BLK - 1) / pf::BLK;
     // the split is for waves that leave SMs idle; larger waves balance by claiming longest first
     // an armed test fault runs the plain instantiation: pointer tables, unsplit, per-thread copies
-    const bool armed = flt.skip_plus1 != 0u && !pm;
+    const bool armed = flt.skip_plus1 != 0u && !pm && !sinks;
     const bool split = !armed && ws && ws->max_slots != 0u && part_keys != 0u && nblocks * NKV < (uint32_t)num_sms;
     PfSplit sp{};
     if (split) {
@@ -1069,19 +1242,23 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
         sp.target_items = (uint32_t)num_sms;
     }
     if (nblocks <= 1024u)
-        (void)launch_pdl(prefill_plan_small_kernel, dim3(1), dim3(1024), 0, stream, seq_lens, rows, window, order, counter, sp);
+        (void)launch_pdl(prefill_plan_small_kernel, dim3(1), dim3(1024), 0, stream, seq_lens, rows, window, sinks, order, counter, sp);
     else
-        prefill_plan_kernel<<<1, 1024, 0, stream>>>(seq_lens, rows, window, order, counter);
+        prefill_plan_kernel<<<1, 1024, 0, stream>>>(seq_lens, rows, window, sinks, order, counter);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const PagedMap map = pm ? *pm : PagedMap{};
     const PrefillSlab none{};
-    const bool tma = !armed && !pm && slab && slab->rows != 0u;
+    const bool tma = !armed && !pm && !sinks && slab && slab->rows != 0u;
     const PrefillSlab& sl = tma ? *slab : none;
-#define OXI_PF_ARGS ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, rows, window, status, order, counter, map, row_seq, sp, sl, flt
+#define OXI_PF_ARGS ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, rows, window, status, order, counter, map, row_seq, sp, sl, flt, view
     if (!split) {
         const uint32_t nitems = nblocks * NKV;
         const uint32_t grid = nitems < (uint32_t)num_sms ? nitems : (uint32_t)num_sms;
+        if (q8) return format == Q8_INT8 ? launch_pf<true, false, false, false, true, PF_INT8>(stream, grid, OXI_PF_ARGS)
+                                         : launch_pf<true, false, false, false, true, PF_E4M3>(stream, grid, OXI_PF_ARGS);
+        if (sinks) return pm ? launch_pf<true, false, false, false, true>(stream, grid, OXI_PF_ARGS)
+                             : launch_pf<false, false, false, false, true>(stream, grid, OXI_PF_ARGS);
         if (pm) return launch_pf<true, false, false>(stream, grid, OXI_PF_ARGS);
         if (armed) return launch_pf<false, false, false, true>(stream, grid, OXI_PF_ARGS);
         return tma ? launch_pf<false, false, true>(stream, grid, OXI_PF_ARGS)
@@ -1089,12 +1266,17 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
     }
     // the unit count is only known on the device: one CTA per SM, those without a unit leave at once
     const uint32_t grid = (uint32_t)num_sms;
-    if (pm) e = launch_pf<true, true, false>(stream, grid, OXI_PF_ARGS);
+    if (q8) e = format == Q8_INT8 ? launch_pf<true, true, false, false, true, PF_INT8>(stream, grid, OXI_PF_ARGS)
+                                  : launch_pf<true, true, false, false, true, PF_E4M3>(stream, grid, OXI_PF_ARGS);
+    else if (sinks) e = pm ? launch_pf<true, true, false, false, true>(stream, grid, OXI_PF_ARGS)
+                           : launch_pf<false, true, false, false, true>(stream, grid, OXI_PF_ARGS);
+    else if (pm) e = launch_pf<true, true, false>(stream, grid, OXI_PF_ARGS);
     else e = tma ? launch_pf<false, true, true>(stream, grid, OXI_PF_ARGS) : launch_pf<false, true, false>(stream, grid, OXI_PF_ARGS);
 #undef OXI_PF_ARGS
     if (e != cudaSuccess) return e;
     // a plain launch: as a programmatic dependent it measured no faster
-    prefill_merge_kernel<<<nblocks * 8 * 32, 128, 0, stream>>>((uint16_t*)ctx_out, (const uint16_t*)gate, rows, sp);
+    if (q8 || sinks) prefill_merge_kernel<true><<<nblocks * 8 * 32, 128, 0, stream>>>((uint16_t*)ctx_out, (const uint16_t*)gate, rows, sp);
+    else prefill_merge_kernel<false><<<nblocks * 8 * 32, 128, 0, stream>>>((uint16_t*)ctx_out, (const uint16_t*)gate, rows, sp);
     return cudaGetLastError();
 }
 

@@ -34,4 +34,21 @@ __device__ __forceinline__ float q8_value(uint32_t code) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)code, __NV_E4M3)));
 }
 
+// the four codes of w as two f16 pairs, exact
+template <uint32_t kFmt>
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if (kFmt == Q8_E4M3) {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(lo), "=r"(hi) : "r"(w));
+    } else {
+        // c + 128 as the low bits of the f16 1024 + (c + 128), minus 1152
+        const uint32_t u = w ^ 0x80808080u;
+        const __half2 k = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+        uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), k), y = __hsub2(*reinterpret_cast<__half2*>(&b), k);
+        lo = *reinterpret_cast<const uint32_t*>(&x);
+        hi = *reinterpret_cast<const uint32_t*>(&y);
+    }
+}
+
 }  // namespace oxi

@@ -361,6 +361,26 @@ def test_prefill_attention_ignores_later_tokens_and_idle_blocks(kv):
     assert torch.equal(base.view(torch.int16), again.view(torch.int16)) and kv.device_status() == 0
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), 1e38, 0.0])
+def test_prefill_attention_ignores_keys_between_sinks_and_windows(kv, fmt, bad):
+    """Tokens that no row of the wave sees: any codes; blocks without a visible token: any scales."""
+    c = Q.Q8Cache([700, 300], fmt, 16, seed=46)
+    chunks, window, sinks = [(0, 600, 90), (1, 250, 40)], 70, 21
+    base, *_ = _prefill(kv, c, chunks, window, sinks)
+    for s, p, n in chunks:
+        t = np.arange(sinks, p + 1 - window)
+        tt = torch.from_numpy(t).cuda()
+        blk = c.dtables[s].long()[tt // 16]
+        for x in (c.kp, c.vp):
+            x.view(torch.uint8)[blk, tt % 16] = 0x7f if fmt == "e4m3" else 0x80
+        hidden = [b for b in range(2, (p + 1 - window) // 16)]
+        for x in (c.ks, c.vs):
+            x[c.dtables[s].long()[torch.tensor(hidden, device="cuda")]] = bad
+    again, *_ = _prefill(kv, c, chunks, window, sinks)
+    assert torch.equal(base.view(torch.int16), again.view(torch.int16)) and kv.device_status() == 0
+
+
 def test_prefill_attention_skips_rows_and_reports_blocks(kv):
     c = Q.Q8Cache([100, 40], "int8", 16, seed=44)
     row_seq, lens = [0, 0, 1, 1, 0], [5, 0, 40, 16 * c.max_blocks + 1, 100]

@@ -231,6 +231,22 @@ def test_prefill_without_window_or_sinks_is_the_plain_entry_point(kv, bs):
         assert torch.equal(a.view(torch.int16), b.view(torch.int16))
 
 
+@pytest.mark.parametrize("bs", [0, 16])
+@pytest.mark.parametrize("window,sinks", [(70, 21), (70, 64), (20, 130)])
+def test_prefill_ignores_what_no_row_sees(kv, bs, window, sinks):
+    c = F16Cache([700, 300], bs, seed=79)
+    chunks = [(0, 600, 90), (1, 250, 40)]
+    row_seq, pos = Q.wave(chunks)
+    q, g = Q.activations(len(pos), 82)
+    a, b = _ctx(len(pos)), _ctx(len(pos))
+    c.prefill(kv, a, q, g, row_seq, pos + 1, window, sinks)
+    for s, p, n in chunks:
+        c.poison(s, np.arange(sinks, p + 1 - window))
+        c.poison(s, np.arange(p + n, c.lens[s]))
+    c.prefill(kv, b, q, g, row_seq, pos + 1, window, sinks)
+    assert torch.equal(a.view(torch.int16), b.view(torch.int16)) and kv.device_status() == 0
+
+
 def test_prefill_skips_rows(kv):
     c = F16Cache([100, 40], 16, seed=74)
     row_seq, lens = [0, 0, 1, 1, 0], [5, 0, 40, 16 * c.max_blocks + 1, 100]
