@@ -5,25 +5,25 @@
 //   q_out = f16(z);   k code = round(z / s_k),   v code = round(v / s_v)
 //
 // with s the scale of the token's (block, KV head).  A scale belongs to a whole block, so the rows of a run that
-// fall into one block are handled together by the CTA of the first of them (the segment's leader): largest
-// magnitude over the segment, the block's new scale, requantised codes of the slots before the segment if the
-// scale grew, then the segment's codes.  Nothing waits on another CTA: the leader reads the whole segment, the
-// CTAs of the other rows only do their q.
+// fall into one block (a segment) need their largest magnitude first; then the block's new scale, requantised codes
+// of the slots before the segment if the scale grew, and the segment's codes.  Nothing waits on another CTA.
 //
-// grid = rows, 16 warps: warp w does q head w; in a leader's CTA warp w then does every second row of the
-// segment for (K or V, KV head) = w mod 8.  Lane l holds dims 2l, 2l+1, 64+2l, 65+2l, so that both members of
-// every rotation pair sit in one lane.
+// Two kernels, by what the caller passes: without row_seq every row is a segment of its own (append_q8_step_kernel),
+// with it rows may form runs (append_q8_wave_kernel).
+//
+// Dims are spread over lanes so that both members of every rotation pair are in one lane and all accesses of a warp
+// are contiguous.
 #include "kernels.h"
 #include "q8.cuh"
 
 namespace oxi {
 
 namespace aq {
-constexpr int WARPS = 16, THREADS = WARPS * 32;
-constexpr int COMBOS = 2 * NKV;             // K or V of a KV head
-constexpr int PARTS = WARPS / COMBOS;       // warps that share a combination's rows
-constexpr int KEEP = 8;                     // rows a warp keeps in registers between the two passes
 constexpr float F16_MAX = 65504.0f;
+constexpr int COMBOS = 2 * NKV;                    // K or V of a KV head
+constexpr int STEP_THREADS = (NQ + COMBOS) * 32;   // a warp for each head of the row
+constexpr int WAVE_WARPS = 16, WAVE_THREADS = WAVE_WARPS * 32;
+constexpr int KV_PAIRS = NKV;                      // pairs of K or V heads of a row: K 0-1, K 2-3, V 0-1, V 2-3
 }  // namespace aq
 
 struct AppendQ8Params {
@@ -67,145 +67,388 @@ __device__ __forceinline__ void norm_rope_pairs(float (&x)[4], const float (&w)[
     x[3] = fmaf(y[3], c[3], y[1] * s[3]);
 }
 
-template <uint32_t kFmt>
-__global__ void __launch_bounds__(aq::THREADS)
-append_q8_kernel(const AppendQ8Params p) {
-    using namespace aq;
-    __shared__ uint32_t s_len, s_conflict;
-    __shared__ float s_amax[PARTS][COMBOS];
-    const uint32_t r = blockIdx.x;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    pdl_launch_dependents();
-    if (tid == 0) {
-        s_len = 0xffffffffu;
-        s_conflict = 0u;
+// Infinite and NaN values and values beyond f16 are stored as +-65504 and 0; returns whether there were any.
+__device__ __forceinline__ bool make_finite(float (&x)[4]) {
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (!(fabsf(x[j]) <= aq::F16_MAX)) {
+            odd = true;
+            x[j] = x[j] != x[j] ? 0.0f : copysignf(aq::F16_MAX, x[j]);
+        }
     }
+    return odd;
+}
+
+__device__ __forceinline__ float abs_max(const float (&x)[4]) {
+    return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+    return v;
+}
+
+__device__ __forceinline__ void store_q(uint16_t* head, int lane, const float (&x)[4]) {
+    reinterpret_cast<uint32_t*>(head)[lane] = pack_h2(x[0], x[1]);
+    reinterpret_cast<uint32_t*>(head)[32 + lane] = pack_h2(x[2], x[3]);
+}
+
+template <uint32_t kFmt>
+__device__ __forceinline__ void store_codes(unsigned char* at, int lane, const float (&x)[4], float inv) {
+    reinterpret_cast<uint16_t*>(at)[lane] = (uint16_t)q8_codes2<kFmt>(x[0], x[1], inv);
+    reinterpret_cast<uint16_t*>(at)[32 + lane] = (uint16_t)q8_codes2<kFmt>(x[2], x[3], inv);
+}
+
+// Slots first, first + step, ... < slots of a block (one head's 128 codes at base) move from scale `from` to `to`.
+template <uint32_t kFmt>
+__device__ __forceinline__ void requantise(unsigned char* base, uint32_t first, uint32_t step, uint32_t slots, int lane, float from, float to) {
+#pragma unroll 4
+    for (uint32_t t = first; t < slots; t += step) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(base + (size_t)t * Q8_ROW_BYTES) + lane;
+        const uint32_t w = __ldcg(at);
+        uint32_t o = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) o |= q8_code<kFmt>(q8_value<kFmt>((w >> (8 * j)) & 0xffu) * from, to) << (8 * j);
+        *at = o;
+    }
+}
+
+// Row r is a token of table row r.  grid = rows, a warp for each query head, K head and V head.
+template <uint32_t kFmt>
+__global__ void __launch_bounds__(aq::STEP_THREADS)
+append_q8_step_kernel(const AppendQ8Params p) {
+    using namespace aq;
+    const uint32_t r = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_launch_dependents();
     // the step's tables, norm weights and rotary rows are not written by any kernel: read while the preceding
     // kernel is still draining
-    const uint32_t lbs = p.map.lbs, bs = 1u << lbs;
-    const uint32_t pos = p.pos_ids[r];
-    const uint32_t seq = p.row_seq ? p.row_seq[r] : r;
-    const uint32_t blk = pos >> lbs, slot0 = pos & (bs - 1u);
+    const uint32_t lbs = p.map.lbs, pos = p.pos_ids[r], blk = pos >> lbs, slot = pos & ((1u << lbs) - 1u);
     if (pos >= p.max_seq_len || blk >= p.map.max_blocks) {
-        if (tid == 0) atomicOr(p.status, DEV_BAD_SEQ_LEN);
+        if (threadIdx.x == 0) atomicOr(p.status, DEV_BAD_SEQ_LEN);
         pdl_wait();
         return;
     }
-    bool leader = slot0 == 0u || r == 0u || !p.row_seq;
-    if (!leader) leader = p.row_seq[r - 1] != seq || p.pos_ids[r - 1] + 1u != pos;
-    __syncthreads();
-    uint32_t n = 1u, id = 0u;
-    if (leader) {
-        if (p.row_seq) {
-            // length of the segment: rows that go on with the next position of the same sequence inside the block
-            for (uint32_t i = 1u + tid; slot0 + i <= bs; i += THREADS) {
-                const bool same = slot0 + i < bs && r + i < p.rows && p.row_seq[r + i] == seq && p.pos_ids[r + i] == pos + i &&
-                                  pos + i < p.max_seq_len;
-                if (!same) {
-                    atomicMin(&s_len, i);
-                    break;
-                }
-            }
-            __syncthreads();
-            n = s_len;
-            // another run of this call in the same block would race with this one
-            for (uint32_t j = tid; j < p.rows; j += THREADS)
-                if ((j < r || j >= r + n) && p.row_seq[j] == seq && (p.pos_ids[j] >> lbs) == blk && p.pos_ids[j] < p.max_seq_len) s_conflict = 1u;
-        }
-        id = p.map.block_tables[(size_t)seq * p.map.max_blocks + blk];
+    const int combo = warp - NQ;  // >= 0: K or V head
+    const bool is_v = combo >= NKV;
+    const uint32_t id = combo >= 0 ? p.map.block_tables[(size_t)r * p.map.max_blocks + blk] : 0u;
+    float wv[4], cv[4], sv[4], x[4];
+    if (!is_v) {
+        load_pairs(combo < 0 ? p.q_norm_w : p.k_norm_w, lane, wv);
+        load_pairs(p.cos_t + (size_t)pos * HD, lane, cv);
+        load_pairs(p.sin_t + (size_t)pos * HD, lane, sv);
     }
-    float wv[4], cv[4], sv[4];
-    load_pairs(p.q_norm_w, lane, wv);
-    load_pairs(p.cos_t + (size_t)pos * HD, lane, cv);
-    load_pairs(p.sin_t + (size_t)pos * HD, lane, sv);
     pdl_wait();  // q, k, v come from the preceding kernel; the cache may still be read by it
-    {
-        float x[4];
+    if (combo < 0) {
         const size_t at = ((size_t)r * NQ + warp) * HD;
         load_pairs(p.q_in + at, lane, x);
         norm_rope_pairs(x, wv, cv, sv, p.eps);
-        reinterpret_cast<uint32_t*>(p.q_out + at)[lane] = pack_h2(x[0], x[1]);
-        reinterpret_cast<uint32_t*>(p.q_out + at)[32 + lane] = pack_h2(x[2], x[3]);
-    }
-    if (!leader) return;
-    __syncthreads();
-    if (id >= p.map.num_blocks || s_conflict) {
-        if (tid == 0) atomicOr(p.status, s_conflict ? DEV_BLOCK_CONFLICT : DEV_BAD_BLOCK);
+        store_q(p.q_out + at, lane, x);
         return;
     }
-    const int combo = warp & (COMBOS - 1), part = warp / COMBOS, kvh = combo & (NKV - 1);
-    const bool is_v = combo >= NKV;
+    if (id >= p.map.num_blocks) {
+        if (combo == 0 && lane == 0) atomicOr(p.status, DEV_BAD_BLOCK);
+        return;
+    }
+    const int kvh = combo & (NKV - 1);
     float* scale_at = (is_v ? p.map.v_scales : p.map.k_scales) + (size_t)id * p.map.scale_stride + kvh;
-    const float old_scale = slot0 != 0u ? __ldcg(scale_at) : 0.0f;
-    if (!is_v) load_pairs(p.k_norm_w, lane, wv);
-    bool odd = false;  // some value is not a finite f16
-    auto load_row = [&](uint32_t i, float (&x)[4]) {
-        load_pairs((is_v ? p.v_in : p.k_in) + ((size_t)(r + i) * NKV + kvh) * HD, lane, x);
-        if (!is_v) {
-            load_pairs(p.cos_t + (size_t)(pos + i) * HD, lane, cv);
-            load_pairs(p.sin_t + (size_t)(pos + i) * HD, lane, sv);
-            norm_rope_pairs(x, wv, cv, sv, p.eps);
-        }
+    const float old_scale = slot != 0u ? __ldcg(scale_at) : 0.0f;
+    load_pairs((is_v ? p.v_in : p.k_in) + ((size_t)r * NKV + kvh) * HD, lane, x);
+    if (!is_v) norm_rope_pairs(x, wv, cv, sv, p.eps);
+    if (__any_sync(0xffffffffu, make_finite(x)) && lane == 0) atomicOr(p.status, DEV_NONFINITE);
+    const float scale = fmaxf(q8_scale<kFmt>(warp_max(abs_max(x))), old_scale);
+    unsigned char* base = (is_v ? p.map.v_pool : p.map.k_pool) + (size_t)id * p.map.block_stride + kvh * HD;
+    if (scale > old_scale) requantise<kFmt>(base, 0u, 1u, slot, lane, old_scale, scale);
+    store_codes<kFmt>(base + (size_t)slot * Q8_ROW_BYTES, lane, x, q8_inverse<kFmt>(scale));
+    if (lane == 0) *scale_at = scale;
+}
+
+// ---- the wave kernel's unit is a PAIR of heads of one row in a warp: lanes 0-15 hold the first, lanes 16-31 the second,
+// lane j (mod 16) dims 4j .. 4j+3 and 64+4j .. 64+4j+3: eight-byte loads, and one reduction serves two heads.
+__device__ __forceinline__ void load_dims(const uint16_t* head, int j, float (&x)[8]) {
+    const uint2 a = reinterpret_cast<const uint2*>(head)[j], b = reinterpret_cast<const uint2*>(head)[16 + j];
+    const uint32_t w[4] = {a.x, a.y, b.x, b.y};
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (!(fabsf(x[j]) <= F16_MAX)) {
-                odd = true;
-                x[j] = x[j] != x[j] ? 0.0f : copysignf(F16_MAX, x[j]);
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+// the same 8 dims of a norm weight, cos or sin row, kept as f16 pairs (registers)
+struct Dims {
+    uint32_t w[4];
+    __device__ __forceinline__ float operator[](int i) const {
+        const __half2 h = *reinterpret_cast<const __half2*>(&w[i >> 1]);
+        return i & 1 ? __high2float(h) : __low2float(h);
+    }
+};
+__device__ __forceinline__ Dims dims_of(const uint16_t* head, int j) {
+    const uint2 a = reinterpret_cast<const uint2*>(head)[j], b = reinterpret_cast<const uint2*>(head)[16 + j];
+    return Dims{{a.x, a.y, b.x, b.y}};
+}
+__device__ __forceinline__ void norm_rope_dims(float (&x)[8], const Dims& w, const Dims& c, const Dims& s, float eps) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum = fmaf(x[i], x[i], sum);
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    const float r = rsqrtf(fmaf(sum, 1.0f / HD, eps));
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = x[i] * r * w[i];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float lo = x[i], hi = x[4 + i];
+        x[i] = fmaf(lo, c[i], -hi * s[i]);
+        x[4 + i] = fmaf(hi, c[4 + i], lo * s[4 + i]);
+    }
+}
+// largest magnitude of the lane's head; infinite, NaN and too large values are replaced as in make_finite
+__device__ __forceinline__ float head_max(float (&x)[8], bool& odd) {
+    float m = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        bad |= !(fabsf(x[i]) <= aq::F16_MAX);
+        m = fmaxf(m, fabsf(x[i]));
+    }
+    if (bad) {
+        odd = true;
+        m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (!(fabsf(x[i]) <= aq::F16_MAX)) x[i] = x[i] != x[i] ? 0.0f : copysignf(aq::F16_MAX, x[i]);
+            m = fmaxf(m, fabsf(x[i]));
+        }
+    }
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    return m;
+}
+template <uint32_t kFmt>
+__device__ __forceinline__ void store_dims(unsigned char* head, int j, const float (&x)[8], float inv) {
+    reinterpret_cast<uint32_t*>(head)[j] = q8_codes2<kFmt>(x[0], x[1], inv) | (q8_codes2<kFmt>(x[2], x[3], inv) << 16);
+    reinterpret_cast<uint32_t*>(head)[16 + j] = q8_codes2<kFmt>(x[4], x[5], inv) | (q8_codes2<kFmt>(x[6], x[7], inv) << 16);
+}
+
+// Row r is a token of table row row_seq[r].  A CTA takes a window of 16 rows and one of kSplit groups of heads: the
+// query heads of its rows, and for its K and V heads the segments that BEGIN in its window, to their end: rows behind
+// the window (its last segment may go on for up to 255 rows) are read twice, once for the scale and once for the
+// codes.  Rows at the window's start that go on with a segment of the window before are left to that CTA.  Warp w owns
+// row w of the window; all its K and V loads are in flight together.
+template <uint32_t kFmt, int kSplit>
+__global__ void __launch_bounds__(aq::WAVE_THREADS, 2)
+append_q8_wave_kernel(const AppendQ8Params p) {
+    using namespace aq;
+    constexpr int ROWS = WAVE_WARPS;             // a warp for each row of the window
+    constexpr int NP = KV_PAIRS / kSplit;        // K / V pairs of a warp; it does twice as many query pairs
+    // per row of the window; a segment is named by its first row
+    __shared__ uint32_t s_pos[ROWS], s_seq[ROWS], s_id[ROWS], s_end[ROWS], s_bad[ROWS];
+    __shared__ int s_lead[ROWS];  // the row's segment, -1: not of this CTA
+    __shared__ float s_amax[ROWS][COMBOS], s_old[ROWS][COMBOS], s_scale[ROWS][COMBOS], s_tailmax[ROWS][COMBOS];
+    __shared__ uint32_t s_leaders, s_tail;
+    const uint32_t row0 = blockIdx.x * ROWS;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = lane >> 4, j = lane & 15;
+    const int w = warp;                          // this warp's row of the window
+    const int pair0 = (int)blockIdx.y * NP;      // and its first K / V pair
+    const uint32_t lbs = p.map.lbs, bs = 1u << lbs;
+    pdl_launch_dependents();
+    if (tid == 0) s_tail = 256u;
+    if (warp == 0) {
+        const uint32_t r = row0 + (uint32_t)lane;
+        uint32_t pos = 0, seq = 0, ppos = 0, pseq = 0;
+        const bool there = lane < ROWS && r < p.rows;
+        if (there) {
+            pos = p.pos_ids[r];
+            seq = p.row_seq[r];
+            if (r > 0u) {
+                ppos = p.pos_ids[r - 1u];
+                pseq = p.row_seq[r - 1u];
             }
         }
+        const bool valid = there && pos < p.max_seq_len && (pos >> lbs) < p.map.max_blocks;
+        if (there && !valid && blockIdx.y == 0) atomicOr(p.status, DEV_BAD_SEQ_LEN);
+        const bool leader = valid && ((pos & (bs - 1u)) == 0u || r == 0u || pseq != seq || ppos + 1u != pos);
+        const uint32_t leaders = __ballot_sync(0xffffffffu, leader), valids = __ballot_sync(0xffffffffu, valid);
+        if (lane < ROWS) {
+            // a valid row that is no leader goes on with the row before; the row after one that is not valid is a leader
+            const uint32_t upto = leaders & (0xffffffffu >> (31 - lane));
+            s_lead[lane] = valid && upto ? 31 - __clz(upto) : -1;
+            s_pos[lane] = valid ? pos : 0xffffffffu;
+            s_seq[lane] = seq;
+            // where the segment that begins here ends inside the window: the next leader or row that is not valid
+            const uint32_t stop = (leaders | ~valids) & ~(0xffffffffu >> (31 - lane));
+            s_end[lane] = min((uint32_t)ROWS, stop ? (uint32_t)__ffs((int)stop) - 1u : 32u);
+            s_id[lane] = leader ? p.map.block_tables[(size_t)seq * p.map.max_blocks + (pos >> lbs)] : 0u;
+            s_bad[lane] = 0u;
+        }
+        if (lane == 0) s_leaders = leaders;
+    }
+    if (tid < ROWS * COMBOS) {
+        s_amax[tid / COMBOS][tid % COMBOS] = 0.0f;
+        s_tailmax[tid / COMBOS][tid % COMBOS] = 0.0f;
+    }
+    __syncthreads();
+    const uint32_t leaders = s_leaders, pos = s_pos[w];
+    const bool there = pos != 0xffffffffu;  // a row that is skipped is not read either
+    const int last = s_lead[ROWS - 1];
+    const Dims cv = dims_of(p.cos_t + (size_t)(there ? pos : 0u) * HD, j), sv = dims_of(p.sin_t + (size_t)(there ? pos : 0u) * HD, j);
+    const Dims kw = dims_of(p.k_norm_w, j), qw = dims_of(p.q_norm_w, j);
+    if (tid < 256) {
+        // rows behind the window that go on with its last row's segment: the first that does not ends the tail
+        const uint32_t i = 1u + (uint32_t)tid, r = row0 + ROWS - 1u + i, lp = s_pos[ROWS - 1];
+        const bool same = last >= 0 && (lp & (bs - 1u)) + i < bs && r < p.rows && p.row_seq[r] == s_seq[ROWS - 1] &&
+                          p.pos_ids[r] == lp + i && lp + i < p.max_seq_len;
+        if (!same) atomicMin(&s_tail, i - 1u);
+    }
+    __syncthreads();
+    const uint32_t tail = s_tail;
+    // another run of this call in a segment's block would race with it: both are refused
+    for (uint32_t m = leaders; m; m &= m - 1u) {
+        const int li = __ffs((int)m) - 1;
+        const uint32_t seq = s_seq[li], blk = s_pos[li] >> lbs, first = row0 + li, end = row0 + s_end[li] + (li == last ? tail : 0u);
+        auto look = [&](uint32_t r) {
+            if (r < first || r >= end) {
+                const uint32_t q = p.pos_ids[r];
+                if ((q >> lbs) == blk && q < p.max_seq_len) s_bad[li] = 1u;
+            }
+        };
+        const uint32_t quads = (((uintptr_t)p.row_seq) & 15u) == 0u ? p.rows / 4u : 0u;
+        for (uint32_t i = tid; i < quads; i += WAVE_THREADS) {
+            const uint4 q = reinterpret_cast<const uint4*>(p.row_seq)[i];
+            if (q.x == seq) look(4u * i);
+            if (q.y == seq) look(4u * i + 1u);
+            if (q.z == seq) look(4u * i + 2u);
+            if (q.w == seq) look(4u * i + 3u);
+        }
+        for (uint32_t i = 4u * quads + tid; i < p.rows; i += WAVE_THREADS)
+            if (p.row_seq[i] == seq) look(i);
+    }
+    pdl_wait();  // q, k, v come from the preceding kernel; the cache may still be read by it
+    // heads of pair i: K (i < 2) or V, heads 2 (i mod 2) and + 1; combination (K 0-3, V 0-3) of this lane's head
+    auto combo_of = [&](int i) { return 2 * i + half; };
+    auto kv_head = [&](int i, size_t row) {
+        return (i < KV_PAIRS / 2 ? p.k_in : p.v_in) + (row * NKV + 2 * (i % (KV_PAIRS / 2)) + half) * HD;
     };
-    float keep[KEEP][4], amax = 0.0f;
+    const size_t row = there ? row0 + w : 0u;
+    float x[NP][8], y[8];
 #pragma unroll
-    for (int k = 0; k < KEEP; k++) {
-        const uint32_t i = part + k * PARTS;
-        if (i < n) {
-            load_row(i, keep[k]);
+    for (int k = 0; k < NP; k++) load_dims(kv_head(pair0 + k, row), j, x[k]);
+    if (tid < ROWS * COMBOS) {  // a segment that begins behind slot 0 starts from the block's scale
+        const int li = tid / COMBOS, c = tid % COMBOS;
+        const bool read = ((leaders >> li) & 1u) && s_id[li] < p.map.num_blocks && (s_pos[li] & (bs - 1u)) != 0u;
+        s_old[li][c] = read ? __ldcg((c < NKV ? p.map.k_scales : p.map.v_scales) + (size_t)s_id[li] * p.map.scale_stride + (c & (NKV - 1))) : 0.0f;
+    }
+    bool odd = false;
 #pragma unroll
-            for (int j = 0; j < 4; j++) amax = fmaxf(amax, fabsf(keep[k][j]));
+    for (int k = 0; k < NP; k++) {
+        if (pair0 + k < KV_PAIRS / 2) norm_rope_dims(x[k], kw, cv, sv, p.eps);
+        bool o = false;
+        const float a = head_max(x[k], o);
+        if (there && s_lead[w] >= 0) {
+            odd |= o;
+            if (j == 0) s_amax[w][combo_of(pair0 + k)] = a;
         }
     }
-    for (uint32_t i = part + KEEP * PARTS; i < n; i += PARTS) {
-        float x[4];
-        load_row(i, x);
+    // rows behind the window: row t of the tail by warp t mod 16
+    auto tail_row = [&](uint32_t t, int i, float (&v)[8]) {
+        load_dims(kv_head(i, row0 + ROWS + t), j, v);
+        if (i < KV_PAIRS / 2) {
+            const size_t at = s_pos[ROWS - 1] + 1u + t;
+            norm_rope_dims(v, kw, dims_of(p.cos_t + at * HD, j), dims_of(p.sin_t + at * HD, j), p.eps);
+        }
+        return head_max(v, odd);
+    };
 #pragma unroll
-        for (int j = 0; j < 4; j++) amax = fmaxf(amax, fabsf(x[j]));
+    for (int k = 0; k < NP; k++) {
+        float m = 0.0f;
+#pragma unroll 2
+        for (uint32_t t = w; t < tail; t += ROWS) {
+            float v[8];
+            m = fmaxf(m, tail_row(t, pair0 + k, v));
+        }
+        if (j == 0) s_tailmax[w][combo_of(pair0 + k)] = m;
     }
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-    if (lane == 0) s_amax[part][combo] = amax;
     if (__any_sync(0xffffffffu, odd) && lane == 0) atomicOr(p.status, DEV_NONFINITE);
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < PARTS; k++) amax = fmaxf(amax, s_amax[k][combo]);
-    const float scale = fmaxf(q8_scale<kFmt>(amax), old_scale);
-    const float div = scale > 0.0f ? scale : 1.0f;
-    unsigned char* base = (is_v ? p.map.v_pool : p.map.k_pool) + (size_t)id * p.map.block_stride + kvh * HD;
-    if (scale > old_scale) {  // slots before the segment move to the larger scale
-        for (uint32_t t = part; t < slot0; t += PARTS) {
-            uint32_t* at = reinterpret_cast<uint32_t*>(base + (size_t)t * Q8_ROW_BYTES) + lane;
-            const uint32_t w = __ldcg(at);
-            uint32_t o = 0;
-#pragma unroll
-            for (int j = 0; j < 4; j++) o |= q8_code<kFmt>(q8_value<kFmt>((w >> (8 * j)) & 0xffu) * old_scale, div) << (8 * j);
-            *at = o;
+    if (tid < ROWS * COMBOS && ((leaders >> (tid / COMBOS)) & 1u)) {
+        const int li = tid / COMBOS, c = tid % COMBOS;
+        float amax = 0.0f;
+        for (uint32_t i = li; i < s_end[li]; i++) amax = fmaxf(amax, s_amax[i][c]);
+        if (li == last)
+            for (int i = 0; i < ROWS; i++) amax = fmaxf(amax, s_tailmax[i][c]);
+        const float scale = fmaxf(q8_scale<kFmt>(amax), s_old[li][c]);
+        s_scale[li][c] = scale;
+        const bool no_block = s_id[li] >= p.map.num_blocks;
+        if (no_block || s_bad[li]) {
+            if (c == 0 && blockIdx.y == 0) atomicOr(p.status, no_block ? DEV_BAD_BLOCK : DEV_BLOCK_CONFLICT);
+        } else if (c / (COMBOS / kSplit) == (int)blockIdx.y) {
+            ((c < NKV ? p.map.k_scales : p.map.v_scales) + (size_t)s_id[li] * p.map.scale_stride)[c & (NKV - 1)] = scale;
         }
     }
-    auto store_row = [&](uint32_t i, const float (&x)[4]) {
-        uint16_t* at = reinterpret_cast<uint16_t*>(base + (size_t)(slot0 + i) * Q8_ROW_BYTES);
-        at[lane] = (uint16_t)(q8_code<kFmt>(x[0], div) | (q8_code<kFmt>(x[1], div) << 8));
-        at[32 + lane] = (uint16_t)(q8_code<kFmt>(x[2], div) | (q8_code<kFmt>(x[3], div) << 8));
+    // the query heads, while the scales settle
+    if (there) {
+#pragma unroll 4
+        for (int k = 0; k < 2 * NP; k++) {
+            const size_t at = (row * NQ + 2 * (2 * pair0 + k) + half) * HD;
+            load_dims(p.q_in + at, j, y);
+            norm_rope_dims(y, qw, cv, sv, p.eps);
+            reinterpret_cast<uint2*>(p.q_out + at)[j] = make_uint2(pack_h2(y[0], y[1]), pack_h2(y[2], y[3]));
+            reinterpret_cast<uint2*>(p.q_out + at)[16 + j] = make_uint2(pack_h2(y[4], y[5]), pack_h2(y[6], y[7]));
+        }
+    }
+    __syncthreads();
+    auto usable = [&](int li) { return s_id[li] < p.map.num_blocks && s_bad[li] == 0u; };
+    auto head_codes = [&](int li, int c) {  // this head's codes in the segment's block
+        return (c < NKV ? p.map.k_pool : p.map.v_pool) + (size_t)s_id[li] * p.map.block_stride + (c & (NKV - 1)) * HD;
     };
+    for (uint32_t m = leaders; m; m &= m - 1u) {
+        const int li = __ffs((int)m) - 1;
+        const uint32_t slots = s_pos[li] & (bs - 1u);
+        if (slots == 0u || !usable(li)) continue;
+        for (int k = 0; k < 2 * NP; k++) {
+            const int c = 2 * pair0 + k;
+            if (s_scale[li][c] > s_old[li][c]) requantise<kFmt>(head_codes(li, c), w, ROWS, slots, lane, s_old[li][c], s_scale[li][c]);
+        }
+    }
+    const int li = there ? s_lead[w] : -1;
+    if (li >= 0 && usable(li)) {
 #pragma unroll
-    for (int k = 0; k < KEEP; k++) {
-        const uint32_t i = part + k * PARTS;
-        if (i < n) store_row(i, keep[k]);
+        for (int k = 0; k < NP; k++) {
+            const int c = combo_of(pair0 + k);
+            store_dims<kFmt>(head_codes(li, c) + (size_t)(pos & (bs - 1u)) * Q8_ROW_BYTES, j, x[k], q8_inverse<kFmt>(s_scale[li][c]));
+        }
     }
-    for (uint32_t i = part + KEEP * PARTS; i < n; i += PARTS) {
-        float x[4];
-        load_row(i, x);
-        store_row(i, x);
+    if (tail != 0u && usable(last)) {
+#pragma unroll
+        for (int k = 0; k < NP; k++) {
+            const int c = combo_of(pair0 + k);
+            const float inv = q8_inverse<kFmt>(s_scale[last][c]);
+#pragma unroll 2
+            for (uint32_t t = w; t < tail; t += ROWS) {
+                float v[8];
+                tail_row(t, pair0 + k, v);
+                store_dims<kFmt>(head_codes(last, c) + (size_t)((s_pos[ROWS - 1] + 1u + t) & (bs - 1u)) * Q8_ROW_BYTES, j, v, inv);
+            }
+        }
     }
-    if (part == 0 && lane == 0) *scale_at = scale;
+}
+
+template <uint32_t kFmt, int kSplit>
+static cudaError_t launch_wave(cudaStream_t stream, const AppendQ8Params& p) {
+    return launch_pdl(append_q8_wave_kernel<kFmt, kSplit>, dim3((p.rows + aq::WAVE_WARPS - 1) / aq::WAVE_WARPS, kSplit), dim3(aq::WAVE_THREADS), 0,
+                      stream, p);
+}
+
+template <uint32_t kFmt>
+static cudaError_t launch_fmt(cudaStream_t stream, const AppendQ8Params& p) {
+    if (!p.row_seq) return launch_pdl(append_q8_step_kernel<kFmt>, dim3(p.rows), dim3(aq::STEP_THREADS), 0, stream, p);
+    // two CTAs fit an SM: four groups of heads while all CTAs are resident at once, else two (fewer CTAs repeat a window's
+    // set-up).  Measured, us: 128 rows in one run, blocks of 16 / 256: 3.5 / 12.2 with four groups, 4.9 / 22.0 with two;
+    // 2,048 rows 10.3 / 16.5 against 7.3 / 27.2; 4,096 rows 23.2 / 28.2 against 17.8 / 32.4.
+    return p.rows <= 1184u ? launch_wave<kFmt, 4>(stream, p) : launch_wave<kFmt, 2>(stream, p);
 }
 
 cudaError_t launch_append_q8(cudaStream_t stream, void* q_out, const void* q_in, const void* k_in, const void* v_in,
@@ -228,8 +471,7 @@ cudaError_t launch_append_q8(cudaStream_t stream, void* q_out, const void* q_in,
     p.max_seq_len = max_seq_len;
     p.eps = eps;
     p.status = status;
-    return launch_pdl(format == Q8_INT8 ? append_q8_kernel<Q8_INT8> : append_q8_kernel<Q8_E4M3>, dim3(rows), dim3(aq::THREADS), 0,
-                      stream, p);
+    return format == Q8_INT8 ? launch_fmt<Q8_INT8>(stream, p) : launch_fmt<Q8_E4M3>(stream, p);
 }
 
 }  // namespace oxi

@@ -28,6 +28,19 @@ __device__ __forceinline__ uint32_t q8_code(float x, float s) {
     return (uint32_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
 }
 
+// What values are multiplied with before they are rounded to codes: 1 / scale, exact for e4m3; for int8 the quotient
+// x / s is off by up to 2^-22 of itself, i.e. a value within 2^-15 of a step from a tie may go to the other side.
+template <uint32_t kFmt>
+__device__ __forceinline__ float q8_inverse(float scale) {
+    return scale > 0.0f ? fminf(__fdiv_rn(1.0f, scale), 3.0e38f) : 0.0f;
+}
+// Codes of a (low byte) and b at inv = q8_inverse of a scale that covers them.
+template <uint32_t kFmt>
+__device__ __forceinline__ uint32_t q8_codes2(float a, float b, float inv) {
+    if (kFmt == Q8_INT8) return (uint32_t)(__float2int_rn(a * inv) & 0xff) | ((uint32_t)(__float2int_rn(b * inv) & 0xff) << 8);
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
+}
+
 template <uint32_t kFmt>
 __device__ __forceinline__ float q8_value(uint32_t code) {
     if (kFmt == Q8_INT8) return (float)(int8_t)(uint8_t)code;
