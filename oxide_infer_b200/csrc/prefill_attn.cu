@@ -55,6 +55,8 @@
 // writing output and reports OXI_DEV_WAIT_TIMEOUT in the status word.
 #include "common.cuh"
 #include "kernels.h"
+#include <type_traits>
+
 #include "q8.cuh"
 #include "tc5.cuh"
 
@@ -74,11 +76,12 @@ constexpr int NS = 4;                        // ring stages, for K and for V
 constexpr int DEPTH = 3;                     // tiles a loader keeps in flight
 constexpr int Q_SUB = M * ROW_B;             // one 64-dim half of a query tile in shared memory: 16 KB
 constexpr int Q_BYTES = 2 * Q_SUB;           // 32 KB
-constexpr int STG_TILE = TK * HD;            // a K (or V) tile of 8-bit codes as it arrives: 8 KB
-constexpr int STG = 3;                       // such tiles a loader has in flight
+constexpr int NL = 3;                        // 8-bit cache: loader warps for K and for V (tiles in turn)
+constexpr int THREADS_Q8 = 512;              // four loader warps more; 128 registers a thread at launch, of which
+constexpr int REGS_SOFTMAX = 160, REGS_OTHER = 96;  // warps 8-15 give up 32 each for the softmax warps
+static_assert(256 * (REGS_SOFTMAX + REGS_OTHER) == THREADS_Q8 * 128, "the split hands out what the block was launched with");
 constexpr int SCL = 8;                       // tiles whose scales are in shared memory (the softmax lags the loader by fewer)
 constexpr size_t SMEM_BYTES = 1024 + Q_BYTES + 2 * NS * KV_TILE;  // + slack for 1024-byte alignment; > half an SM: one CTA per SM
-constexpr size_t SMEM_BYTES_Q8 = SMEM_BYTES + 2 * STG * STG_TILE;
 constexpr uint32_t TMEM_COLS = 512;
 // Q_0 (64) | S_0 S_1 (64 each) | P_0 P_1 (32 each) | O_0 O_1 (128 each); Q_1 does not fit and stays in shared memory
 constexpr uint32_t Q0_COL = 0, S_COL = 64, P_COL = 192, O_COL = 256;  // S + j*64, P + j*32, O + j*128 for query tile j
@@ -334,14 +337,16 @@ __device__ __forceinline__ bool pf_next_run(uint32_t& next, uint32_t nruns, cons
 // status word reports.
 // kSinks: the window leaves the first tokens visible (PfView); a run's tiles are then PfTiles, keys that no row of the
 // run sees are zero-filled, and the gate is applied before the one rounding of the result.
-// kFmt (with kPaged and kSinks): the 8-bit cache.  The loader warps bring codes into a staging ring (half the bytes
-// from L2) and convert them to the f16 tiles of the ring, exactly: scales never enter the operands.  A tile's four
+// kFmt (with kPaged and kSinks): the 8-bit cache.  Loader warps (three for K, three for V: a conversion takes one warp longer
+// than a tile's MMAs take) hold the next tile's codes in registers while they convert the current one to an f16 tile of the
+// ring, exactly: scales never enter the operands.  A tile's four
 // 16-key groups have one K scale and one V scale each; the softmax multiplies the scores of a group by its K scale in
 // the fma that it does anyway and adds log2 of the V scale to the exponent, so that P carries the V scales, and the
 // row sum takes each group's partial sum times 1 / (V scale): 8 instructions a tile more than the f16 cache.
 constexpr uint32_t PF_F16 = 0, PF_INT8 = 1, PF_E4M3 = 2;
+constexpr int pf_threads(uint32_t fmt) { return fmt == PF_F16 ? pf::THREADS : pf::THREADS_Q8; }
 template <bool kPaged, bool kSplit, bool kTma, bool kFault, bool kSinks = false, uint32_t kFmt = PF_F16>
-__global__ void __launch_bounds__(pf::THREADS, 1)
+__global__ void __launch_bounds__(pf_threads(kFmt), 1)
 prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__ q,
                     const uint16_t* __restrict__ gate, const uint64_t* __restrict__ k_ptrs,
                     const uint64_t* __restrict__ v_ptrs, const uint32_t* __restrict__ seq_lens,
@@ -373,12 +378,11 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
     __shared__ __align__(8) uint64_t bar_sfull[2], bar_sfree[2], bar_pfull[2], bar_pvdone[2], bar_qfull[2], bar_ofull[2];
     __shared__ __align__(8) uint64_t bar_tok[2];  // issue token of MMA warp j
     __shared__ uint32_t s_tmem, s_abort, s_item[2], s_unit[2];
-    // 8-bit cache: scales of a tile's four groups as they arrive (K, then V; all heads), and what the softmax uses:
-    // K scale * log2e / sqrt(128), log2 V scale, 1 / V scale
-    __shared__ __align__(16) float s_raw[kQ8 ? SCL : 1][8][4], s_scl[kQ8 ? SCL : 1][3][4];
+    // 8-bit cache: a tile's four groups' K scale * log2e / sqrt(128), log2 of the V scale, 1 / V scale
+    __shared__ __align__(16) float s_scl[kQ8 ? SCL : 1][3][4];
 
     const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;  // 1024-byte aligned tiles
-    const uint32_t q1_s = sbase, k_s = sbase + Q_BYTES, v_s = k_s + NS * KV_TILE, stg_s = v_s + NS * KV_TILE;
+    const uint32_t q1_s = sbase, k_s = sbase + Q_BYTES, v_s = k_s + NS * KV_TILE;
     const int tid = threadIdx.x, lane = tid & 31;
     // warp index the compiler can prove uniform: role branches and MMA issue stay in uniform control flow
     const int warp_u = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -520,6 +524,10 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
     if (warp_u == W_KLOAD) prepare_item(0u);
 
   // ======== persistent loop over (64-row block, KV head) items, longest first ========
+  // kRole 0: every warp runs this loop and branches to its role; 1, 2, 3: the loop of the softmax, MMA and loader
+  // warps alone (the 8-bit cache, where the roles have different register counts and must not share code)
+  auto run_items = [&](auto role) {
+  constexpr int kRole = decltype(role)::value;
   for (uint32_t it = 0;; ++it) {
     // every role is done with the previous item; this item's tables (written by the K loader) are visible
     __syncthreads();
@@ -549,7 +557,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
         t_hi = (uint32_t)((uint64_t)gt * (part + 1u) / nparts);
     }
 
-    if (warp_u < 8) {
+    if (kRole == 0 ? warp_u < 8 : kRole == 1) {
         // ================= softmax warps: query tile j, accumulator row (head hw, token lane) =================
         const int j = warp_u >> 2, hw = warp_u & 3;
         const uint32_t tok = (uint32_t)(j * TOK + lane);
@@ -778,7 +786,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                 }
             }
         }
-    } else if (warp_u == W_MMA0 || warp_u == W_MMA1) {
+    } else if (kRole == 0 ? warp_u == W_MMA0 || warp_u == W_MMA1 : kRole == 2) {
         // ================= MMA warps: warp W_MMAj issues the MMAs of query tile j =================
         // One elected lane issues, the whole warp waits.  The tensor pipe accepts an MMA only when
         // the one before has started, so the issuing thread is held for about the MMAs' execution
@@ -878,6 +886,125 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             step(nt + 1, true, false, true);
             ++n_o;
         }
+    } else if (kQ8) {
+        // ================= loader warps of the 8-bit cache: warps 9, 12, 14 for K, 10, 13, 15 for V =================
+        // Warp idx of a kind takes the tiles g with g % NL == idx.  It holds the codes of its next tile in registers
+        // (quarter b: the 16 keys of a group, which lie in one block) and, quarter by quarter, converts the current
+        // tile and requests the next one's.  A lane's 16-byte chunk cq of row rr + 4k becomes chunks 2 cq and
+        // 2 cq + 1 of the f16 row; the 8 lanes of a store phase (4 chunks of two neighbouring rows) fall in distinct
+        // banks of the swizzled tile.
+        const bool is_k = warp_u == W_KLOAD || warp_u == 12 || warp_u == 14;
+        const uint32_t idx = warp_u < 12 ? 0u : (uint32_t)(warp_u - 10) / 2u;
+        uint64_t* full = is_k ? bar_kfull : bar_vfull;
+        uint64_t* empty = is_k ? bar_kempty : bar_vempty;
+        const uint32_t cq = (lane & 3u) + 4u * ((lane >> 3) & 1u), rr = ((lane >> 2) & 1u) + 2u * ((lane >> 4) & 1u);
+        const char* const base = reinterpret_cast<const char*>(is_k ? pm.k_pool : pm.v_pool) + kvh * HD + cq * 16;
+        const uint32_t ch = (2u * cq) & 7u, pos0 = (ch ^ rr) << 4, pos1 = ((ch + 1u) ^ rr) << 4;
+        const uint32_t dst0 = (is_k ? k_s : v_s) + (cq >> 2) * KV_SUB + rr * ROW_B;
+        uint32_t next = 0, tflat = 0, tile = 0, tile1 = 0, gi = gk, last_page = 0;
+        const uint32_t* trow = nullptr;
+        PfRun run;
+        PfTiles tl;
+        // moves to this warp's next tile, at or behind (run, tile), whose number is gi; at the end gi counts all tiles
+        auto seek = [&]() -> bool {
+            for (;;) {
+                const uint32_t skip = (idx + NL - gi % NL) % NL;
+                if (tile + skip < tile1) {
+                    tile += skip;
+                    gi += skip;
+                    return true;
+                }
+                gi += tile1 - tile;
+                tile = tile1 = 0;
+                if (!pf_next_run(next, nruns, c_runs, run)) return false;
+                tl = tiles_of(run);
+                tile1 = tl.n;
+                if (kSplit) {
+                    tile = min(tl.n, max(t_lo, tflat) - tflat);
+                    tile1 = min(tl.n, max(t_hi, tflat) - tflat);
+                    tflat += tl.n;
+                }
+                trow = pm.block_tables + (size_t)((c_kp[run.r0] >> 4) - 1ull) * pm.max_blocks;
+                last_page = (run.hi - 1u) >> pm.lbs;
+            }
+        };
+        // lane l: the block of page (tile's first page + l), at most 4 pages
+        auto fetch_pages = [&]() -> uint32_t {
+            const uint32_t pg = (tl.first_key(tile) >> pm.lbs) + (uint32_t)lane;
+            uint32_t id = 0;
+            if (lane < 4 && pg <= last_page) {
+                id = __ldg(trow + pg);
+                if (id >= pm.num_blocks) {
+                    atomicOr(status, DEV_BAD_BLOCK);
+                    id = 0;
+                }
+            }
+            return id;
+        };
+        uint4 d[4][4];
+        auto request = [&](int b, uint32_t pages) {  // quarter b of tile (run, tile); keys that no row sees: zeros
+            const uint32_t kbeg = tl.first_key(tile), t = kbeg + 16 * b;
+            const uint32_t pid = __shfl_sync(0xffffffffu, pages, ((t >> pm.lbs) - (kbeg >> pm.lbs)) & 31u);
+            const char* src = base + (uint64_t)pid * pm.block_stride + (uint64_t)((t & ((1u << pm.lbs) - 1u)) + rr) * ROWB;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t tkn = t + rr + 4 * k;
+                const bool seen = tkn < run.hi && (tkn >= run.lo || tkn < view.sinks);
+                // written by the append kernel before: not through L1
+                d[b][k] = seen ? __ldcg(reinterpret_cast<const uint4*>(src + (size_t)k * 4 * ROWB)) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        };
+        // K loaders: lane l < 4 the K scale of group l, lanes 4-7 the V scales
+        auto request_scale = [&](uint32_t pages) -> float {
+            const uint32_t kbeg = tl.first_key(tile), t = kbeg + 16u * (lane & 3u);
+            const uint32_t pid = __shfl_sync(0xffffffffu, pages, ((t >> pm.lbs) - (kbeg >> pm.lbs)) & 31u);
+            return is_k && lane < 8 && t < run.hi ? __ldcg((lane < 4 ? view.k_scales : view.v_scales) + (uint64_t)pid * view.scale_stride + kvh) : 0.0f;
+        };
+        float scale = 0.0f;
+        bool more = seek();
+        if (more) {
+            const uint32_t pages = fetch_pages();
+#pragma unroll
+            for (int b = 0; b < 4; b++) request(b, pages);
+            scale = request_scale(pages);
+        }
+        while (more) {
+            const uint32_t g = gi, st = g % NS;
+            ++tile;
+            ++gi;
+            more = seek();
+            const uint32_t pages = more ? fetch_pages() : 0u;
+            ok &= mbar_wait_bounded(&empty[st], ((g / NS) & 1u) ^ 1u, &s_abort, wait_us);
+            __syncwarp();
+            const uint32_t dst = dst0 + st * KV_TILE;
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t w[4] = {d[b][k].x, d[b][k].y, d[b][k].z, d[b][k].w};
+                    uint32_t h[8];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) codes_to_f16<kCodes>(w[i], h[2 * i], h[2 * i + 1]);
+                    const uint32_t at = dst + (uint32_t)(16 * b + 4 * k) * ROW_B, flip = (k & 1) << 6;  // row & 7 = rr + 4 (k & 1)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (pos0 ^ flip)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (pos1 ^ flip)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                }
+                if (more) request(b, pages);
+            }
+            if (is_k) {
+                const float l2 = fminf(fmaxf(__log2f(scale), -100.0f), 100.0f);  // finite even for the scale of a block without visible keys
+                if (lane < 4) s_scl[g % SCL][0][lane] = fmaxf(scale * QK_SCALE_LOG2, 1.0e-30f);  // a masked score stays -inf under a zero scale
+                else if (lane < 8) {
+                    s_scl[g % SCL][1][lane - 4] = l2;
+                    s_scl[g % SCL][2][lane - 4] = exp2f(-l2);
+                }
+                if (more) scale = request_scale(pages);
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&full[st]);
+        }
+        gk = gi;
+        if (warp_u == W_KLOAD) prepare_item(buf ^ 1u);
     } else if (warp_u == W_KLOAD || warp_u == W_VLOAD) {
         // ================= loader warps: one for the K ring, one for the V ring =================
         const bool is_k = warp_u == W_KLOAD;
@@ -893,43 +1020,6 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
         auto publish = [&](uint32_t g) {
             if (kFault && is_k && blockIdx.x == 0 && g + 1u == fault.skip_plus1) return;
             mbar_arrive(&full[g % NS]);
-        };
-        // 8-bit cache: tile number g from the staging ring into the f16 ring.  A lane converts the 16-byte chunks that it
-        // copied itself: chunk cq of rows rq, rq + 4, ... becomes chunks 2 cq and 2 cq + 1 of the f16 row; lanes of the
-        // two 64-dim halves store them in opposite order, so the 8 lanes of a store phase fall in distinct banks.
-        const uint32_t cq = lane & 7u, rq = lane >> 3;
-        const uint32_t stg = stg_s + (is_k ? 0u : (uint32_t)(STG * STG_TILE));
-        auto convert = [&](uint32_t g) {
-            const uint32_t st = g % NS;
-            ok &= mbar_wait_bounded(&empty[st], ((g / NS) & 1u) ^ 1u, &s_abort, wait_us);
-            __syncwarp();
-            const uint32_t src = stg + (g % STG) * STG_TILE + rq * HD + cq * 16;
-            const uint32_t dst = ring + st * KV_TILE + (cq >> 2) * KV_SUB;
-            const uint32_t odd = cq >> 2;  // 1: the odd chunk first
-            const uint32_t ch = (2u * cq) & 7u;
-#pragma unroll 4
-            for (int k = 0; k < TK / 4; k++) {
-                const uint32_t row = rq + 4 * k;
-                uint32_t w[4], h[8];
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src + k * 4 * HD) : "memory");
-#pragma unroll
-                for (int i = 0; i < 4; i++) codes_to_f16<kCodes>(w[i], h[2 * i], h[2 * i + 1]);
-#pragma unroll
-                for (uint32_t i = 0; i < 2; i++) {
-                    const bool hi = (i ^ odd) != 0u;
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + row * ROW_B + (((ch + (hi ? 1u : 0u)) ^ (row & 7u)) << 4)),
-                                 "r"(hi ? h[4] : h[0]), "r"(hi ? h[5] : h[1]), "r"(hi ? h[6] : h[2]), "r"(hi ? h[7] : h[3]) : "memory");
-                }
-            }
-            if (is_k && lane < 4) {
-                const float ks = s_raw[g % SCL][lane][kvh], vs = s_raw[g % SCL][4 + lane][kvh];
-                const float l2 = fminf(fmaxf(__log2f(vs), -100.0f), 100.0f);  // finite even for the scale of a block without visible keys
-                s_scl[g % SCL][0][lane] = fmaxf(ks * QK_SCALE_LOG2, 1.0e-30f);  // a masked score stays -inf under a zero scale
-                s_scl[g % SCL][1][lane] = l2;
-                s_scl[g % SCL][2][lane] = exp2f(-l2);
-            }
-            fence_proxy_async_smem();
-            publish(g);
         };
         uint32_t tflat = 0;    // tiles of the block's runs before this one (key-range split)
         uint32_t next = 0;
@@ -981,38 +1071,6 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                 }
             }
             for (uint32_t tile = tile0; tile < tile1; tile++) {
-                if (kQ8) {
-                    // four groups of 16 keys, each inside one block; lanes 0-3 (4-7) also bring the groups' K (V) scales
-                    const uint32_t kbeg = tl.first_key(tile), p0 = kbeg >> pm.lbs, mask = (1u << pm.lbs) - 1u;
-                    const uint32_t pg_cur = pg_next;
-                    if (tile + 1 < tile1) pg_next = fetch_pages(tl.first_key(tile + 1));
-                    const uint32_t dst = stg + (gk % STG) * STG_TILE + rq * HD + cq * 16;
-                    uint64_t off[4];
-#pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        const uint32_t t = kbeg + 16 * b;
-                        const uint32_t pid = __shfl_sync(0xffffffffu, pg_cur, ((t >> pm.lbs) - p0) & 31u);
-                        off[b] = (uint64_t)pid * pm.block_stride + (uint64_t)(t & mask) * ROWB;
-                        if (is_k && (lane & 3) == b && lane < 8)
-                            cp_async_16(smem_u32(&s_raw[gk % SCL][lane][0]), (lane < 4 ? view.k_scales : view.v_scales) + (uint64_t)pid * view.scale_stride,
-                                        t < run.hi);
-                    }
-#pragma unroll
-                    for (int k = 0; k < TK / 4; k++) {
-                        const uint32_t row = rq + 4 * k;
-                        const bool valid = seen(kbeg + row);
-                        cp_async_16(dst + k * 4 * HD, valid ? base + off[k >> 2] + (row & 15u) * ROWB + cq * 16 : base, valid);
-                    }
-                    cp_async_commit();
-                    ++pending;
-                    ++gk;
-                    if (pending == STG) {
-                        cp_async_wait<STG - 1>();
-                        convert(gk - STG);
-                        --pending;
-                    }
-                    continue;
-                }
                 const uint32_t st = gk % NS;
                 // the MMAs that read this stage's previous tile have completed (first use: passes at once)
                 ok &= mbar_wait_bounded(&empty[st], ((gk / NS) & 1u) ^ 1u, &s_abort, wait_us);
@@ -1075,24 +1133,39 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             }
         }
         cp_async_wait<0>();
-        if (kQ8) {
-            for (; pending > 0; --pending) convert(gk - pending);
-        } else {
-            fence_proxy_async_smem();
-            for (; pending > 0; --pending) publish(gk - pending);
-        }
+        fence_proxy_async_smem();
+        for (; pending > 0; --pending) publish(gk - pending);
         // all tiles of this item are on their way to the tensor core: claim the next item and prepare its
         // tables while the other roles work through the last tiles
         if (is_k) prepare_item(buf ^ 1u);
     }
   }  // item loop
-
-    if (!ok) atomicOr(status, DEV_WAIT_TIMEOUT);
-    tc_fence_before();
-    __syncthreads();
-    if (warp_u == W_MMA0) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+  };
+    auto finish = [&]() {
+        if (!ok) atomicOr(status, DEV_WAIT_TIMEOUT);
+        tc_fence_before();
+        __syncthreads();
+        if (warp_u == W_MMA0) {
+            tc_fence_after();
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+        }
+    };
+    if constexpr (!kQ8) {
+        run_items(std::integral_constant<int, 0>{});
+        finish();
+    } else if (warp_u < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+        run_items(std::integral_constant<int, 1>{});
+        finish();
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHER));
+        if (warp_u == W_MMA0 || warp_u == W_MMA1) {
+            run_items(std::integral_constant<int, 2>{});
+            finish();
+        } else {
+            run_items(std::integral_constant<int, 3>{});
+            finish();
+        }
     }
 }
 
@@ -1176,7 +1249,7 @@ size_t prefill_split_slot_bytes() { return (size_t)NKV * 2 * pf::M * (HD + 2) * 
 template <bool kPaged, bool kSplit, bool kTma, bool kFault = false, bool kSinks = false, uint32_t kFmt = PF_F16>
 static cudaError_t pf_set_smem() {
     return cudaFuncSetAttribute(prefill_attn_kernel<kPaged, kSplit, kTma, kFault, kSinks, kFmt>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)(kFmt != PF_F16 ? pf::SMEM_BYTES_Q8 : pf::SMEM_BYTES));
+                                (int)pf::SMEM_BYTES);
 }
 
 cudaError_t prefill_attn_init() {
@@ -1205,8 +1278,8 @@ static cudaError_t launch_pf(cudaStream_t stream, uint32_t grid, void* ctx_out, 
                              const uint32_t* row_seq, const PfSplit& sp, const PrefillSlab& slab, const WaitFault& fault,
                              const PfView& view) {
     // programmatic dependent of the plan kernel: TMEM allocation and barrier set-up overlap it
-    return launch_pdl(prefill_attn_kernel<kPaged, kSplit, kTma, kFault, kSinks, kFmt>, dim3(grid), dim3(pf::THREADS),
-                      kFmt != PF_F16 ? pf::SMEM_BYTES_Q8 : pf::SMEM_BYTES, stream,
+    return launch_pdl(prefill_attn_kernel<kPaged, kSplit, kTma, kFault, kSinks, kFmt>, dim3(grid), dim3(pf_threads(kFmt)),
+                      pf::SMEM_BYTES, stream,
                       (uint16_t*)ctx_out, (const uint16_t*)q, (const uint16_t*)gate, k_ptrs, v_ptrs, seq_lens, rows,
                       window, status, (const uint32_t*)order, counter, pm, row_seq, sp, slab.map, slab.base, slab.rows, fault, view);
 }
