@@ -76,9 +76,10 @@ constexpr int NS = 4;                        // ring stages, for K and for V
 constexpr int DEPTH = 3;                     // tiles a loader keeps in flight
 constexpr int Q_SUB = M * ROW_B;             // one 64-dim half of a query tile in shared memory: 16 KB
 constexpr int Q_BYTES = 2 * Q_SUB;           // 32 KB
-constexpr int NL = 3;                        // 8-bit cache: loader warps for K and for V (tiles in turn)
-constexpr int THREADS_Q8 = 512;              // four loader warps more; 128 registers a thread at launch, of which
-constexpr int REGS_SOFTMAX = 160, REGS_OTHER = 96;  // warps 8-15 give up 32 each for the softmax warps
+constexpr int NL = 2;                        // 8-bit cache: loader warps for K and for V (tiles in turn)
+constexpr int W_KLOAD2 = 14, W_VLOAD2 = 13;  // with warps 9 and 10 on the two schedulers that issue no MMAs
+constexpr int THREADS_Q8 = 512;              // warps 12 and 15 only meet the barriers; 128 registers a thread at launch,
+constexpr int REGS_SOFTMAX = 136, REGS_OTHER = 120;  // of which warps 8-15 give up 8 for the softmax warps
 static_assert(256 * (REGS_SOFTMAX + REGS_OTHER) == THREADS_Q8 * 128, "the split hands out what the block was launched with");
 constexpr int SCL = 8;                       // tiles whose scales are in shared memory (the softmax lags the loader by fewer)
 constexpr size_t SMEM_BYTES = 1024 + Q_BYTES + 2 * NS * KV_TILE;  // + slack for 1024-byte alignment; > half an SM: one CTA per SM
@@ -337,8 +338,8 @@ __device__ __forceinline__ bool pf_next_run(uint32_t& next, uint32_t nruns, cons
 // status word reports.
 // kSinks: the window leaves the first tokens visible (PfView); a run's tiles are then PfTiles, keys that no row of the
 // run sees are zero-filled, and the gate is applied before the one rounding of the result.
-// kFmt (with kPaged and kSinks): the 8-bit cache.  Loader warps (three for K, three for V: a conversion takes one warp longer
-// than a tile's MMAs take) hold the next tile's codes in registers while they convert the current one to an f16 tile of the
+// kFmt (with kPaged and kSinks): the 8-bit cache.  Loader warps (two for K, two for V: a conversion takes one warp about as long
+// as a tile's MMAs and softmax; three each measured 3 % slower: they take issue slots from the softmax) hold the next tile's codes in registers while they convert the current one to an f16 tile of the
 // ring, exactly: scales never enter the operands.  A tile's four
 // 16-key groups have one K scale and one V scale each; the softmax multiplies the scores of a group by its K scale in
 // the fma that it does anyway and adds log2 of the V scale to the exponent, so that P carries the V scales, and the
@@ -634,12 +635,11 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                 tc_fence_before();
                 float xs[4], lv[4], iv[4];  // 8-bit cache: the tile's scales (before S_j is handed back: see SCL)
                 if (kQ8) {
-#pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        xs[b] = s_scl[gk % SCL][0][b];
-                        lv[b] = s_scl[gk % SCL][1][b];
-                        iv[b] = s_scl[gk % SCL][2][b];
-                    }
+                    const float4* scl = reinterpret_cast<const float4*>(s_scl[gk % SCL]);
+                    const float4 a = scl[0], b = scl[1], c = scl[2];
+                    xs[0] = a.x, xs[1] = a.y, xs[2] = a.z, xs[3] = a.w;
+                    lv[0] = b.x, lv[1] = b.y, lv[2] = b.z, lv[3] = b.w;
+                    iv[0] = c.x, iv[1] = c.y, iv[2] = c.z, iv[3] = c.w;
                 }
                 mbar_arrive(&bar_sfree[j]);  // the next tile's scores may overwrite S_j now
                 // PV_j of the tile before has long completed as a rule: polled here, needed before P is stored
@@ -887,14 +887,14 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             ++n_o;
         }
     } else if (kQ8) {
-        // ================= loader warps of the 8-bit cache: warps 9, 12, 14 for K, 10, 13, 15 for V =================
+        // ================= loader warps of the 8-bit cache: warps 9, 14 for K, 10, 13 for V =================
         // Warp idx of a kind takes the tiles g with g % NL == idx.  It holds the codes of its next tile in registers
         // (quarter b: the 16 keys of a group, which lie in one block) and, quarter by quarter, converts the current
         // tile and requests the next one's.  A lane's 16-byte chunk cq of row rr + 4k becomes chunks 2 cq and
         // 2 cq + 1 of the f16 row; the 8 lanes of a store phase (4 chunks of two neighbouring rows) fall in distinct
         // banks of the swizzled tile.
-        const bool is_k = warp_u == W_KLOAD || warp_u == 12 || warp_u == 14;
-        const uint32_t idx = warp_u < 12 ? 0u : (uint32_t)(warp_u - 10) / 2u;
+        const bool is_k = warp_u == W_KLOAD || warp_u == W_KLOAD2;
+        const uint32_t idx = warp_u < 12 ? 0u : 1u;
         uint64_t* full = is_k ? bar_kfull : bar_vfull;
         uint64_t* empty = is_k ? bar_kempty : bar_vempty;
         const uint32_t cq = (lane & 3u) + 4u * ((lane >> 3) & 1u), rr = ((lane >> 2) & 1u) + 2u * ((lane >> 4) & 1u);
@@ -946,6 +946,11 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             const uint32_t kbeg = tl.first_key(tile), t = kbeg + 16 * b;
             const uint32_t pid = __shfl_sync(0xffffffffu, pages, ((t >> pm.lbs) - (kbeg >> pm.lbs)) & 31u);
             const char* src = base + (uint64_t)pid * pm.block_stride + (uint64_t)((t & ((1u << pm.lbs) - 1u)) + rr) * ROWB;
+            if (kbeg >= run.lo && kbeg + TK <= run.hi) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) d[b][k] = __ldcg(reinterpret_cast<const uint4*>(src + k * 4 * ROWB));
+                return;
+            }
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const uint32_t tkn = t + rr + 4 * k;
@@ -961,7 +966,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             return is_k && lane < 8 && t < run.hi ? __ldcg((lane < 4 ? view.k_scales : view.v_scales) + (uint64_t)pid * view.scale_stride + kvh) : 0.0f;
         };
         float scale = 0.0f;
-        bool more = seek();
+        bool more = (is_k || warp_u == W_VLOAD || warp_u == W_VLOAD2) && seek();
         if (more) {
             const uint32_t pages = fetch_pages();
 #pragma unroll
