@@ -10,8 +10,7 @@
 //
 // Work decomposition, claiming, merge and failure paths are those of decode_attn.cu: items are fixed ranges of
 // CHUNK keys of the row's own view (a row's arithmetic does not depend on the batch), 148 persistent CTAs claim
-// them, one producer warp streams stages of 64 keys with 4 KB bulk copies through a three-stage ring, consumer
-// warp h serves KV head h.  What differs:
+// them, one producer warp streams stages of 64 keys with 4 KB bulk copies through a three-stage ring.  What differs:
 //
 // * The view is a list of aligned groups of 8 tokens (RowView), so a copy never straddles pages and all keys of a
 //   group share their scales.
@@ -26,6 +25,10 @@
 // * V codes are transposed by ldmatrix on pairs of dims; one byte permutation then pairs the keys, which leaves the
 //   output dims of a tile in the order 0, 2, ..., 14, 1, 3, ..., 15.  Group pitch + 16 bytes.
 // * P^T reaches its B fragment with one movmatrix per 8 keys.
+// * The maximum is only raised when an exponent exceeds it by more than 8 (a factor of 256 in w, within f16's range):
+//   the usual stage needs no reduction over lanes at all.
+// * Consumer warp h serves KV head h.  Two warps per head (half of every group's tokens each) measured 2 us slower
+//   at every size: a scheduler's two warps then wait for the same pipes in the same phases.
 #include "../../include/oxi_kv.h"
 #include "kernels.h"
 #include "q8.cuh"
@@ -56,6 +59,7 @@ constexpr size_t SMEM_BYTES = (size_t)NSTAGE * STAGE_BYTES + NTABLE * TABLE_BYTE
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 static_assert(STAGE_BYTES % 16 == 0 && KPITCH % 128 == 64 && VPITCH % 128 == 16, "alignment and bank offsets");
 constexpr float X_SCALE = ATTN_SCALE * LOG2E;
+constexpr float RAISE = 8.0f;                     // log2 units by which exponents may exceed the maximum in use
 constexpr uint32_t F_FIRST = 1u << 16, F_LAST = 1u << 17, F_END = 1u << 18;
 }  // namespace dq
 
@@ -68,6 +72,12 @@ struct DecodeQ8Params {
     DecodeWorkspace ws;
     uint32_t batch, window, sinks;
 };
+
+// mma.m16n8k16, free to be scheduled among independent ones
+__device__ __forceinline__ void mma_free(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
     uint32_t d;
@@ -147,11 +157,12 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
         };
         auto open_item = [&](uint32_t item) -> Item {
             Item it;
-            uint32_t lo = 0, hi = p.batch;
-            while (hi - lo > 1) {
-                const uint32_t mid = (lo + hi) >> 1;
-                if (prefix[mid] <= item) lo = mid; else hi = mid;
-            }
+            // the row: the last b with prefix[b] <= item, by two looks of the whole warp (batch <= 32 * 32)
+            const uint32_t step = (p.batch + 31u) / 32u;
+            const uint32_t above = __ballot_sync(0xffffffffu, (uint32_t)lane * step < p.batch && prefix[min(lane * step, p.batch)] <= item);
+            const uint32_t lo0 = (31u - __clz(above)) * step;
+            const uint32_t in = __ballot_sync(0xffffffffu, (uint32_t)lane < step && lo0 + lane < p.batch && prefix[min(lo0 + lane, p.batch)] <= item);
+            const uint32_t lo = lo0 + 31u - __clz(in);
             it.row = lo;
             it.range = item - prefix[lo];
             it.slen = s_len[lo];
@@ -167,51 +178,56 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
                               ((uint32_t)lane < it.npa ? it.pa + lane : it.pw + lane - it.npa));
             return it;
         };
-        auto load_scales = [&](Item& it, float4& ks, float4& vs) {
-            if ((uint32_t)lane < it.np && it.id >= p.map.num_blocks) {
-                atomicOr(status, DEV_BAD_BLOCK);
-                it.id = 0;
-            }
-            ks = vs = make_float4(0.f, 0.f, 0.f, 0.f);
-            if ((uint32_t)lane < it.np) {  // written by the append kernel before: not the read-only path
-                ks = __ldcg(reinterpret_cast<const float4*>(p.map.k_scales + (size_t)it.id * p.map.scale_stride));
-                vs = __ldcg(reinterpret_cast<const float4*>(p.map.v_scales + (size_t)it.id * p.map.scale_stride));
-            }
+        // Order of the items: the first rounds go round the CTAs (item k of this CTA is blockIdx + k * grid), the last ones
+        // are claimed from a counter, since SMs do not get equal shares of the memory bandwidth.  Under a saturated
+        // memory pipe a round trip takes about as long as an item, and one that the producer had to wait for would
+        // leave stages empty: `c` is streamed now, the pages of `n` and `m` after it have been requested, and a claim
+        // behind them is in flight.
+        const uint32_t rounds = total_items / gridDim.x;
+        const uint32_t fixed = rounds <= 8u ? min(rounds, 4u) : rounds - 4u;  // rounds in fixed order
+        uint32_t asked = 0, claim = 0;  // items of this CTA so far, the claim in flight
+        auto ask = [&]() {
+            // in PTX: the compiler's warp-aggregated form of atomicAdd waits for the result at once
+            if (asked >= max(fixed, 1u) && lane == 0)
+                asm volatile("atom.global.add.u32 %0, [%1], 1;" : "=r"(claim) : "l"(p.ws.work_counter) : "memory");
         };
-        uint32_t cur = blockIdx.x, claim = 0;
-        Item c{}, n{};
-        float4 cks, cvs, nks, nvs;
+        auto answer = [&]() -> uint32_t {  // the item asked for last; total_items: none
+            const uint32_t k = asked++;
+            if (k < max(fixed, 1u)) return min(blockIdx.x + k * gridDim.x, total_items);
+            const uint32_t i = __shfl_sync(0xffffffffu, claim, 0);
+            return min(total_items, max(fixed, 1u) * gridDim.x + min(i, total_items));
+        };
+        Item c{}, n{}, m{};
+        ask();
+        uint32_t cur = answer(), nxt = total_items, nxt2 = total_items;
+        ask();
         if (cur < total_items) {
-            if (lane == 0) claim = atomicAdd(p.ws.work_counter, 1u);
             c = open_item(cur);
-            load_scales(c, cks, cvs);
+            nxt = answer();
+            if (nxt < total_items) {
+                ask();
+                n = open_item(nxt);
+                nxt2 = answer();
+                if (nxt2 < total_items) {
+                    ask();
+                    m = open_item(nxt2);
+                }
+            }
         }
         while (cur < total_items && ok) {
-            uint32_t nxt = __shfl_sync(0xffffffffu, claim, 0);
-            nxt = (nxt >= total_items) ? total_items : min(nxt + gridDim.x, total_items);
-            claim = 0xffffffffu;
-            if (nxt < total_items) {
-                if (lane == 0) claim = atomicAdd(p.ws.work_counter, 1u);
-                n = open_item(nxt);
+            if ((uint32_t)lane < c.np && c.id >= p.map.num_blocks) {
+                atomicOr(status, DEV_BAD_BLOCK);
+                c.id = 0;
             }
             const uint32_t nchunks = prefix[c.row + 1] - prefix[c.row];
             const RowView rv = row_view<GK>(c.slen, p.window, p.sinks);
             const uint32_t v0 = c.range * CHUNK_G, v1 = min(v0 + CHUNK_G, rv.ng);
             unsigned char* table = tables + (nitem % NTABLE) * TABLE_BYTES;
             for (uint32_t v = v0; v < v1; v += NGROUP, ++fill) {
+                // Whatever does not need the slot comes before the wait for it: a slot's refill starts when its last
+                // consumer lets go.  Lanes 0..7 have the K groups, lanes 8..15 the V groups, lane 16 the q row.
                 const uint32_t slot = fill % NSTAGE;
-                if (fill >= NSTAGE && !mbar_wait_bounded(&empty_bar[slot], ((fill / NSTAGE) & 1u) ^ 1u, abort_flag, wait_us)) {
-                    ok = false;
-                    break;
-                }
                 const bool first = v == v0, last = v + NGROUP >= v1;
-                // test support: this CTA's stage goes missing
-                if (fault.skip_plus1 && blockIdx.x == 0 && fill + 1u == fault.skip_plus1) {
-                    if (first && nxt < total_items) load_scales(n, nks, nvs);  // (checks the next item's pages)
-                    continue;
-                }
-                unsigned char* sb = smem + (size_t)slot * STAGE_BYTES;
-                // lanes 0..7 the K groups, lanes 8..15 the V groups, lane 16 the q row
                 const uint32_t g = lane & (NGROUP - 1), vg = v + g;
                 const bool live = vg < v1;
                 const uint32_t tok = live ? rv.token<GK>(vg) : 0u;
@@ -219,48 +235,62 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
                 const uint32_t id = __shfl_sync(0xffffffffu, c.id, ps & 31u);
                 const uint32_t nk = live ? min(GK, c.slen - tok) : 0u;
                 const uint32_t vis = live ? rv.visible_bits<GK>(tok) : 0u;
-                const uint32_t mine = lane < NGROUP ? nk * 2u * Q8_ROW_BYTES : 0u;
-                const uint32_t bytes = __reduce_add_sync(0xffffffffu, mine) + (first ? Q_BYTES : 0);
-                if (lane < NGROUP) {
-                    sb[DESC_OFF + 16 + lane] = (unsigned char)vis;
-                    sb[DESC_OFF + 24 + lane] = (unsigned char)ps;
+                // only a row's last group is shorter than 8 tokens
+                const uint32_t keys = last ? (v1 - v) * GK - (v1 == rv.ng ? (0u - c.slen) & (GK - 1u) : 0u) : (uint32_t)KS;
+                const uint32_t bytes = keys * 2u * Q8_ROW_BYTES + (first ? Q_BYTES : 0);
+                const bool is_v = lane >= NGROUP;
+                const unsigned char* src = (is_v ? p.map.v_pool : p.map.k_pool) + (size_t)id * p.map.block_stride + (size_t)(tok & bs_mask) * Q8_ROW_BYTES;
+                unsigned char* sb = smem + (size_t)slot * STAGE_BYTES;
+                const uint32_t sbase = smem_u32(sb), dst = sbase + (is_v ? V_OFF + g * VPITCH : g * KPITCH);
+                if (fill >= NSTAGE && !mbar_wait_bounded(&empty_bar[slot], ((fill / NSTAGE) & 1u) ^ 1u, abort_flag, wait_us)) {
+                    ok = false;
+                    break;
                 }
-                if (lane == 0) {
-                    *reinterpret_cast<uint4*>(sb + DESC_OFF) =
-                        make_uint4(c.row, c.range | (nchunks << 16), (nitem % NTABLE) | (first ? F_FIRST : 0u) | (last ? F_LAST : 0u), 0u);
+                // test support: this CTA's stage goes missing
+                if (fault.skip_plus1 && blockIdx.x == 0 && fill + 1u == fault.skip_plus1) continue;
+                if (lane == 0)
                     asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full_bar[slot])), "r"(bytes) : "memory");
-                }
                 __syncwarp();
-                const uint32_t sbase = smem_u32(sb);
                 if (lane < 2 * NGROUP) {
-                    const bool is_v = lane >= NGROUP;
                     if (live) {
-                        const unsigned char* pool = is_v ? p.map.v_pool : p.map.k_pool;
-                        const uint32_t dst = sbase + (is_v ? V_OFF + g * VPITCH : g * KPITCH);
                         if (!OXI_IN_BOUNDS(c.row < p.batch && tok + nk <= c.slen && ps < (uint32_t)PAGES && id < p.map.num_blocks, status))
                             asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full_bar[slot])),
                                          "r"(nk * Q8_ROW_BYTES) : "memory");
                         else
-                            bulk_g2s_hint(dst, pool + (size_t)id * p.map.block_stride + (size_t)(tok & bs_mask) * Q8_ROW_BYTES,
-                                          nk * Q8_ROW_BYTES, &full_bar[slot], policy);
+                            bulk_g2s_hint(dst, src, nk * Q8_ROW_BYTES, &full_bar[slot], policy);
                     }
                 } else if (first && lane == 2 * NGROUP) {
                     bulk_g2s(sbase + Q_OFF, reinterpret_cast<const char*>(p.q) + (size_t)c.row * Q_BYTES, Q_BYTES, &full_bar[slot]);
                 }
-                if (first) {  // the item's scales (their loads may still be in flight; the copies are not held up)
-                    if ((uint32_t)lane < c.np && lane < PAGES) {
-                        reinterpret_cast<float4*>(table)[2 * lane] = cks;
-                        reinterpret_cast<float4*>(table)[2 * lane + 1] = cvs;
-                    }
-                    __syncwarp();
+                if (lane < NGROUP) {
+                    sb[DESC_OFF + 16 + lane] = (unsigned char)vis;
+                    sb[DESC_OFF + 24 + lane] = (unsigned char)ps;
                 }
+                if (lane == 0)
+                    *reinterpret_cast<uint4*>(sb + DESC_OFF) =
+                        make_uint4(c.row, c.range | (nchunks << 16), (nitem % NTABLE) | (first ? F_FIRST : 0u) | (last ? F_LAST : 0u), 0u);
+                if (first) {
+                    // the item's scales; the stage is full when they too have arrived
+                    if ((uint32_t)lane < c.np && lane < PAGES) {
+                        const uint32_t to = smem_u32(table + 32 * lane);
+                        const size_t at = (size_t)c.id * p.map.scale_stride;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p.map.k_scales + at) : "memory");
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16u), "l"(p.map.v_scales + at) : "memory");
+                    }
+                    asm volatile("cp.async.mbarrier.arrive.shared::cta.b64 [%0];" ::"r"(smem_u32(&full_bar[slot])) : "memory");
+                }
+                __syncwarp();
                 if (lane == 0) mbar_arrive(&full_bar[slot]);
-                if (first && nxt < total_items) load_scales(n, nks, nvs);
             }
             cur = nxt;
+            nxt = nxt2;
             c = n;
-            cks = nks;
-            cvs = nvs;
+            n = m;
+            nxt2 = nxt < total_items ? answer() : total_items;
+            if (nxt2 < total_items) {
+                ask();
+                m = open_item(nxt2);
+            }
             ++nitem;
         }
         if (ok) {
@@ -336,26 +366,38 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
         const float lv = fmaxf(__log2f(vs), -100.0f), ivs = exp2f(-lv);
 
         // ---- S^T: tile i holds token 2i of the 8 groups in rows 0-7 and token 2i + 1 in rows 8-15
+        // (the four tiles side by side: their accumulations are independent)
         float s[4][4];
         const unsigned char* krow = sb + g * KPITCH + kvh * HD + t4 * 16;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+        for (int i = 0; i < 4; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                const uint4 a = *reinterpret_cast<const uint4*>(krow + (2 * i) * Q8_ROW_BYTES + hf * 64);
-                const uint4 b = *reinterpret_cast<const uint4*>(krow + (2 * i + 1) * Q8_ROW_BYTES + hf * 64);
-                const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+        for (int hf = 0; hf < 2; hf++) {
+            uint4 kc[8];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
+            for (int i = 0; i < 8; i++) kc[i] = *reinterpret_cast<const uint4*>(krow + i * Q8_ROW_BYTES + hf * 64);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t aw = j == 0 ? kc[2 * i].x : j == 1 ? kc[2 * i].y : j == 2 ? kc[2 * i].z : kc[2 * i].w;
+                    const uint32_t bw = j == 0 ? kc[2 * i + 1].x : j == 1 ? kc[2 * i + 1].y : j == 2 ? kc[2 * i + 1].z : kc[2 * i + 1].w;
                     uint32_t a0, a1, a2, a3;
-                    codes_to_f16<kFmt>(aw[j], a0, a2);
-                    codes_to_f16<kFmt>(bw[j], a1, a3);
-                    mma_16816(s[i], a0, a1, a2, a3, qb[4 * hf + j][0], qb[4 * hf + j][1]);
+                    codes_to_f16<kFmt>(aw, a0, a2);
+                    codes_to_f16<kFmt>(bw, a1, a3);
+                    mma_free(s[i], a0, a1, a2, a3, qb[4 * hf + j][0], qb[4 * hf + j][1]);
                 }
             }
         }
-        // ---- exponents, maxima of the two heads
+        // the first V codes, while the scores settle: k-step i of PV holds tokens 2i (k 0-7) and 2i + 1 (k 8-15)
+        const uint32_t vaddr = smem_u32(sb) + V_OFF + (lane & 7) * VPITCH + (lane >> 3) * Q8_ROW_BYTES + kvh * HD;
+        uint32_t r[4][4];
+        auto load_v = [&](int i2, int d4) {
+#pragma unroll
+            for (int d = 0; d < 4; d++) ldmatrix_x4_trans(vaddr + i2 * 4 * Q8_ROW_BYTES + (d4 + d) * 16, r[d][0], r[d][1], r[d][2], r[d][3]);
+        };
+        load_v(0, 0);
+        // ---- exponents; the maxima of the two heads only where one of them has to be raised
         float n0 = -INFINITY, n1 = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -367,14 +409,14 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
             n0 = fmaxf(n0, fmaxf(s[i][0], s[i][2]));
             n1 = fmaxf(n1, fmaxf(s[i][1], s[i][3]));
         }
+        if (__any_sync(0xffffffffu, n0 > m0 + RAISE || n1 > m1 + RAISE)) {
 #pragma unroll
-        for (int off = 4; off <= 16; off <<= 1) {
-            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, off));
-            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, off));
-        }
-        n0 = fmaxf(n0, m0);
-        n1 = fmaxf(n1, m1);
-        if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
+            for (int off = 4; off <= 16; off <<= 1) {
+                n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, off));
+                n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, off));
+            }
+            n0 = fmaxf(n0, m0);
+            n1 = fmaxf(n1, m1);
             const float c0 = ex2_approx_ftz(m0 - n0), c1 = ex2_approx_ftz(m1 - n1);
             m0 = n0;
             m1 = n1;
@@ -402,18 +444,22 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
         }
         l0 = fmaf(p0, ivs, l0);
         l1 = fmaf(p1, ivs, l1);
-        // ---- O^T += V^T P^T: k-step i holds tokens 2i (k 0-7) and 2i + 1 (k 8-15) of the 8 groups
-        const uint32_t vaddr = smem_u32(sb) + V_OFF + (lane & 7) * VPITCH + (lane >> 3) * Q8_ROW_BYTES + kvh * HD;
+        // ---- O^T += V^T P^T
 #pragma unroll
-        for (int d = 0; d < 8; d++) {
+        for (int i2 = 0; i2 < 2; i2++) {
 #pragma unroll
-            for (int i2 = 0; i2 < 2; i2++) {
-                uint32_t r[4], a[4][2];
-                ldmatrix_x4_trans(vaddr + i2 * 4 * Q8_ROW_BYTES + d * 16, r[0], r[1], r[2], r[3]);
+            for (int d4 = 0; d4 < 8; d4 += 4) {
+                if (i2 + d4 > 0) load_v(i2, d4);
 #pragma unroll
-                for (int j = 0; j < 4; j++) codes_to_f16<kFmt>(__byte_perm(r[j], 0u, 0x3120), a[j][0], a[j][1]);
-                mma_16816(o[d], a[0][0], a[0][1], a[1][0], a[1][1], pb[2 * i2][0], pb[2 * i2][1]);
-                mma_16816(o[d], a[2][0], a[2][1], a[3][0], a[3][1], pb[2 * i2 + 1][0], pb[2 * i2 + 1][1]);
+                for (int j = 0; j < 2; j++) {
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {
+                        uint32_t a0, a1, a2, a3;
+                        codes_to_f16<kFmt>(__byte_perm(r[d][2 * j], 0u, 0x3120), a0, a1);
+                        codes_to_f16<kFmt>(__byte_perm(r[d][2 * j + 1], 0u, 0x3120), a2, a3);
+                        mma_free(o[d4 + d], a0, a1, a2, a3, pb[2 * i2 + j][0], pb[2 * i2 + j][1]);
+                    }
+                }
             }
         }
         if (!whole) fence_proxy_async_smem();  // the zeros above, before the next copy into this stage
