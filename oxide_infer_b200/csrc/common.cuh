@@ -260,7 +260,7 @@ struct RowView {
     uint32_t sinks, start, slen;
     template <uint32_t G>
     __device__ __forceinline__ uint32_t token(uint32_t v) const { return (v < gs ? v : v - gs + gw) * G; }
-    // bit i: token t0 + i is visible (i < G <= 8)
+    // bit i: token t0 + i is visible (i < G <= 16)
     template <uint32_t G>
     __device__ __forceinline__ uint32_t visible_bits(uint32_t t0) const {
         const uint32_t all = (1u << G) - 1u;

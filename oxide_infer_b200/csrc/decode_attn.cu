@@ -679,7 +679,7 @@ constexpr int MERGE_MAX_Y = 8;
 // kRule: how a row is cut into key ranges, and how its result is rounded
 constexpr int MERGE_WINDOW = 0;  // row_chunks; the gate on the f16 result, as the reference does
 constexpr int MERGE_SINKS = 1;   // view_chunks; the gate before the one rounding
-constexpr int MERGE_Q8 = 2;      // the 8-bit cache: groups of 8 tokens; the gate before the one rounding
+constexpr int MERGE_Q8 = 2;      // the 8-bit cache: groups of 16 tokens; the gate before the one rounding
 template <bool kSliced, int kRule>  // kSliced false: the workspace holds rows of at most 16 key ranges (no slice scratch)
 __global__ void __launch_bounds__(128)
 decode_merge_kernel(const DecodeParams p) {
@@ -696,7 +696,7 @@ decode_merge_kernel(const DecodeParams p) {
     if (slen == 0u || slen > p.max_seq_len || (kvp & 15ull) != 0ull) return;
     if (p.paged.block_tables && ((slen - 1u) >> p.paged.lbs) >= p.paged.max_blocks) return;
     const uint32_t nchunks = kRule == MERGE_SINKS ? view_chunks(row_view<dec::GK>(slen, p.window, p.sinks))
-                             : kRule == MERGE_Q8  ? (row_view<8>(slen, p.window, p.sinks).ng + dec::CHUNK / 8 - 1) / (dec::CHUNK / 8)
+                             : kRule == MERGE_Q8  ? (row_view<16>(slen, p.window, p.sinks).ng + dec::CHUNK / 16 - 1) / (dec::CHUNK / 16)
                                                   : row_chunks(slen, p.window);
     if (nchunks <= 1) return;
     const uint32_t nslices = kSliced ? (nchunks + MERGE_BLK - 1) / MERGE_BLK : 1u;

@@ -10,20 +10,22 @@
 //
 // Work decomposition, claiming, merge and failure paths are those of decode_attn.cu: items are fixed ranges of
 // CHUNK keys of the row's own view (a row's arithmetic does not depend on the batch), 148 persistent CTAs claim
-// them, one producer warp streams stages of 64 keys with 4 KB bulk copies through a three-stage ring.  What differs:
+// them, one producer warp streams stages of 64 keys with 8 KB bulk copies through a three-stage ring.  What differs:
 //
-// * The view is a list of aligned groups of 8 tokens (RowView), so a copy never straddles pages and all keys of a
-//   group share their scales.
+// * The view is a list of aligned groups of 16 tokens (RowView), so a copy never straddles pages and all keys of a
+//   group share their scales.  (Groups of 8 tokens: a copy costs the producer about 87 clocks to issue, 16 copies and
+//   the bookkeeping of a stage took it longer than the memory needs for the stage.)
 // * The products are transposed: S^T = K Q^T and O^T = V^T P^T.  The cache is the M = 16 operand and the four
 //   query heads are half of N = 8 columns: half the tensor instructions of the f16 kernel, whose M = 16 rows are a
 //   quarter filled - this kernel has to digest twice the keys per second.
-// * An m16 tile of S^T takes its rows from the 8 groups of the stage (token 2i and 2i+1 of each), so ALL keys of
-//   a thread lie in group lane/4: one K scale and one V scale per thread and stage.
+// * An m16 tile i of S^T takes its rows from the 4 groups of the stage: row r is token 4i + r/4 of group r mod 4.  ALL
+//   keys of a thread therefore lie in group (lane/4) mod 4: one K scale and one V scale per thread and stage.
 // * K codes go from shared memory to fragments with 16-byte loads: the order of the 128 dims inside the products is
 //   permuted so that a thread's 16 consecutive bytes are its operand for four k-steps (q is loaded in the same
 //   order).  Group pitch + 64 bytes: the 8 lanes of a load phase fall in distinct banks.
 // * V codes are transposed by ldmatrix on pairs of dims; one byte permutation then pairs the keys, which leaves the
-//   output dims of a tile in the order 0, 2, ..., 14, 1, 3, ..., 15.  Group pitch + 16 bytes.
+//   output dims of a tile in the order 0, 2, ..., 14, 1, 3, ..., 15.  Group pitch + 16 bytes (two of the 8 rows of a
+//   load phase still share a bank).
 // * P^T reaches its B fragment with one movmatrix per 8 keys.
 // * The maximum is only raised when an exponent exceeds it by more than 8 (a factor of 256 in w, within f16's range):
 //   the usual stage needs no reduction over lanes at all.
@@ -38,9 +40,9 @@ namespace oxi {
 namespace dq {
 constexpr int KS = 64;                            // keys per stage
 constexpr int NSTAGE = 3;
-constexpr uint32_t GK = 8;                        // tokens per group = per bulk copy
-constexpr int NGROUP = KS / (int)GK;              // 8
-constexpr int GROUP_BYTES = (int)GK * Q8_ROW_BYTES;  // 4096
+constexpr uint32_t GK = 16;                       // tokens per group = per bulk copy
+constexpr int NGROUP = KS / (int)GK;              // 4
+constexpr int GROUP_BYTES = (int)GK * Q8_ROW_BYTES;  // 8192
 constexpr int KPITCH = GROUP_BYTES + 64, VPITCH = GROUP_BYTES + 16;
 constexpr int V_OFF = NGROUP * KPITCH;
 constexpr int Q_OFF = V_OFF + NGROUP * VPITCH;
@@ -225,7 +227,7 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
             unsigned char* table = tables + (nitem % NTABLE) * TABLE_BYTES;
             for (uint32_t v = v0; v < v1; v += NGROUP, ++fill) {
                 // Whatever does not need the slot comes before the wait for it: a slot's refill starts when its last
-                // consumer lets go.  Lanes 0..7 have the K groups, lanes 8..15 the V groups, lane 16 the q row.
+                // consumer lets go.  Lanes 0..3 have the K groups, lanes 4..7 the V groups, lane 8 the q row.
                 const uint32_t slot = fill % NSTAGE;
                 const bool first = v == v0, last = v + NGROUP >= v1;
                 const uint32_t g = lane & (NGROUP - 1), vg = v + g;
@@ -235,7 +237,7 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
                 const uint32_t id = __shfl_sync(0xffffffffu, c.id, ps & 31u);
                 const uint32_t nk = live ? min(GK, c.slen - tok) : 0u;
                 const uint32_t vis = live ? rv.visible_bits<GK>(tok) : 0u;
-                // only a row's last group is shorter than 8 tokens
+                // only a row's last group is shorter than 16 tokens
                 const uint32_t keys = last ? (v1 - v) * GK - (v1 == rv.ng ? (0u - c.slen) & (GK - 1u) : 0u) : (uint32_t)KS;
                 const uint32_t bytes = keys * 2u * Q8_ROW_BYTES + (first ? Q_BYTES : 0);
                 const bool is_v = lane >= NGROUP;
@@ -263,7 +265,7 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
                     bulk_g2s(sbase + Q_OFF, reinterpret_cast<const char*>(p.q) + (size_t)c.row * Q_BYTES, Q_BYTES, &full_bar[slot]);
                 }
                 if (lane < NGROUP) {
-                    sb[DESC_OFF + 16 + lane] = (unsigned char)vis;
+                    reinterpret_cast<uint16_t*>(sb + DESC_OFF + 16)[lane] = (uint16_t)vis;
                     sb[DESC_OFF + 24 + lane] = (unsigned char)ps;
                 }
                 if (lane == 0)
@@ -334,7 +336,8 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
         if (desc.z & F_END) break;
         const uint2 vis2 = *reinterpret_cast<const uint2*>(sb + DESC_OFF + 16);
         const bool whole = (vis2.x & vis2.y) == 0xffffffffu;
-        const uint32_t vis = sb[DESC_OFF + 16 + g], ps = sb[DESC_OFF + 24 + g];
+        const uint32_t gg = g & 3u, gt = g >> 2;  // this thread's group, and its first token in it
+        const uint32_t vis = reinterpret_cast<const uint16_t*>(sb + DESC_OFF + 16)[gg], ps = sb[DESC_OFF + 24 + gg];
 
         if (desc.z & F_FIRST) {
             const unsigned char* qrow = sb + Q_OFF + (kvh * 4 + (g & 3)) * (HD * 2);
@@ -357,7 +360,7 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
             for (uint32_t i = lane; i < KS * 8u; i += 32) {
                 const uint32_t key = i >> 3;
                 if (!(((key < 32u ? vis2.x : vis2.y) >> (key & 31u)) & 1u))
-                    *reinterpret_cast<uint4*>(sb + V_OFF + (key >> 3) * VPITCH + (key & 7u) * Q8_ROW_BYTES + kvh * HD + (i & 7u) * 16u) =
+                    *reinterpret_cast<uint4*>(sb + V_OFF + (key / GK) * VPITCH + (key % GK) * Q8_ROW_BYTES + kvh * HD + (i & 7u) * 16u) =
                         make_uint4(0, 0, 0, 0);
             }
             __syncwarp();
@@ -365,17 +368,17 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
         const float xs = ks * X_SCALE;
         const float lv = fmaxf(__log2f(vs), -100.0f), ivs = exp2f(-lv);
 
-        // ---- S^T: tile i holds token 2i of the 8 groups in rows 0-7 and token 2i + 1 in rows 8-15
+        // ---- S^T: tile i holds tokens 4i and 4i + 1 of the 4 groups in rows 0-7 and tokens 4i + 2 and 4i + 3 in rows 8-15
         // (the four tiles side by side: their accumulations are independent)
         float s[4][4];
-        const unsigned char* krow = sb + g * KPITCH + kvh * HD + t4 * 16;
+        const unsigned char* krow = sb + gg * KPITCH + gt * Q8_ROW_BYTES + kvh * HD + t4 * 16;
 #pragma unroll
         for (int i = 0; i < 4; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
 #pragma unroll
         for (int hf = 0; hf < 2; hf++) {
             uint4 kc[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) kc[i] = *reinterpret_cast<const uint4*>(krow + i * Q8_ROW_BYTES + hf * 64);
+            for (int i = 0; i < 8; i++) kc[i] = *reinterpret_cast<const uint4*>(krow + 2 * i * Q8_ROW_BYTES + hf * 64);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
 #pragma unroll
@@ -389,12 +392,12 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
                 }
             }
         }
-        // the first V codes, while the scores settle: k-step i of PV holds tokens 2i (k 0-7) and 2i + 1 (k 8-15)
-        const uint32_t vaddr = smem_u32(sb) + V_OFF + (lane & 7) * VPITCH + (lane >> 3) * Q8_ROW_BYTES + kvh * HD;
+        // the first V codes, while the scores settle: k-step i of PV has the keys of tile i in the same order
+        const uint32_t vaddr = smem_u32(sb) + V_OFF + (lane & 3) * VPITCH + (((lane >> 2) & 1) + 2 * (lane >> 3)) * Q8_ROW_BYTES + kvh * HD;
         uint32_t r[4][4];
         auto load_v = [&](int i2, int d4) {
 #pragma unroll
-            for (int d = 0; d < 4; d++) ldmatrix_x4_trans(vaddr + i2 * 4 * Q8_ROW_BYTES + (d4 + d) * 16, r[d][0], r[d][1], r[d][2], r[d][3]);
+            for (int d = 0; d < 4; d++) ldmatrix_x4_trans(vaddr + i2 * 8 * Q8_ROW_BYTES + (d4 + d) * 16, r[d][0], r[d][1], r[d][2], r[d][3]);
         };
         load_v(0, 0);
         // ---- exponents; the maxima of the two heads only where one of them has to be raised
@@ -404,7 +407,7 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const float e = fmaf(s[i][j], xs, lv);
-                s[i][j] = (whole || ((vis >> (2 * i + (j >> 1))) & 1u)) ? e : -INFINITY;
+                s[i][j] = (whole || ((vis >> (4 * i + 2 * (j >> 1) + gt)) & 1u)) ? e : -INFINITY;
             }
             n0 = fmaxf(n0, fmaxf(s[i][0], s[i][2]));
             n1 = fmaxf(n1, fmaxf(s[i][1], s[i][3]));
