@@ -144,9 +144,9 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
     }
     __syncthreads();
     const uint32_t total_items = prefix[p.batch];
-    pdl_wait();  // codes, scales and q written by the preceding kernel are visible from here on
-
-    if (warp == N_CONSUMER_WARPS) {
+    if (warp != N_CONSUMER_WARPS) {
+        pdl_wait();  // codes, scales and q written by the preceding kernel are visible from here on
+    } else {
         // =========================== producer warp ===========================
         const uint64_t policy = l2_policy_evict_first();
         const uint32_t lbs = p.map.lbs, bs_mask = (1u << lbs) - 1u;
@@ -200,11 +200,24 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
             return min(total_items, max(fixed, 1u) * gridDim.x + min(i, total_items));
         };
         Item c{}, n{}, m{};
-        ask();
-        uint32_t cur = answer(), nxt = total_items, nxt2 = total_items;
+        uint32_t cur = answer(), nxt = total_items, nxt2 = total_items;  // (the first item is in the fixed order)
+        if (cur < total_items) {
+            // block tables are inputs of the step: the first item's pages, and their blocks into L2, while the
+            // preceding kernel drains (what it may still write there is read after the wait, and L2 has it then)
+            c = open_item(cur);
+            const RowView rv = row_view<GK>(c.slen, p.window, p.sinks);
+            const uint32_t v = c.range * CHUNK_G + (lane & 15u), v1 = min((c.range + 1u) * CHUNK_G, rv.ng);
+            const uint32_t tok = v < v1 ? rv.token<GK>(v) : 0u;
+            const uint32_t ps = v >= v1 ? 0u : v < rv.gs ? (tok >> lbs) - c.pa : c.npa + (tok >> lbs) - c.pw;
+            const uint32_t id = __shfl_sync(0xffffffffu, c.id, ps & 31u);
+            if (v < v1 && (lane & 15) < NSTAGE * NGROUP && id < p.map.num_blocks) {
+                const unsigned char* src = (lane >= 16 ? p.map.v_pool : p.map.k_pool) + (size_t)id * p.map.block_stride + (size_t)(tok & bs_mask) * Q8_ROW_BYTES;
+                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(min(GK, c.slen - tok) * Q8_ROW_BYTES) : "memory");
+            }
+        }
+        pdl_wait();
         ask();
         if (cur < total_items) {
-            c = open_item(cur);
             nxt = answer();
             if (nxt < total_items) {
                 ask();
