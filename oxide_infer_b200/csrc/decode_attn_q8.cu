@@ -57,7 +57,7 @@ constexpr int TABLE_BYTES = PAGES * 32;           // per page: 4 K scales, 4 V s
 constexpr int N_CONSUMER_WARPS = NKV;
 constexpr int THREADS = (N_CONSUMER_WARPS + 1) * 32;
 constexpr int MAX_ROWS = 1024;
-constexpr size_t SMEM_BYTES = (size_t)NSTAGE * STAGE_BYTES + NTABLE * TABLE_BYTES + 2 * NSTAGE * 8 + 16 + (2 * MAX_ROWS + 1) * 4;
+constexpr size_t SMEM_BYTES = (size_t)NSTAGE * STAGE_BYTES + NTABLE * TABLE_BYTES + 4 * NSTAGE * 8 + 16 + (2 * MAX_ROWS + 1) * 4;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 static_assert(STAGE_BYTES % 16 == 0 && KPITCH % 128 == 64 && VPITCH % 128 == 16, "alignment and bank offsets");
 constexpr float X_SCALE = ATTN_SCALE * LOG2E;
@@ -93,9 +93,13 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
     using namespace dq;
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char* tables = smem + (size_t)NSTAGE * STAGE_BYTES;
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(tables + NTABLE * TABLE_BYTES);
-    uint64_t* empty_bar = full_bar + NSTAGE;
-    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(empty_bar + NSTAGE);
+    // K (with q, descriptor and scales) and V of a stage are handed over separately: a K slot is refilled while the
+    // consumers are still at the stage's V
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(tables + NTABLE * TABLE_BYTES);
+    uint64_t* v_full = k_full + NSTAGE;
+    uint64_t* k_empty = v_full + NSTAGE;
+    uint64_t* v_empty = k_empty + NSTAGE;
+    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(v_empty + NSTAGE);
     uint32_t* prefix = const_cast<uint32_t*>(abort_flag) + 4;
     uint32_t* s_len = prefix + MAX_ROWS + 1;
 
@@ -108,8 +112,10 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
     // ---- prologue: barriers, items per row, prefix sum (reads only the step's tables)
     if (threadIdx.x == 0) {
         for (int s = 0; s < NSTAGE; s++) {
-            mbar_init(&full_bar[s], 1);
-            mbar_init(&empty_bar[s], N_CONSUMER_WARPS);
+            mbar_init(&k_full[s], 1);
+            mbar_init(&v_full[s], 1);
+            mbar_init(&k_empty[s], N_CONSUMER_WARPS);
+            mbar_init(&v_empty[s], N_CONSUMER_WARPS);
         }
         *abort_flag = 0u;
         prefix[0] = 0u;
@@ -252,30 +258,33 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
                 const uint32_t vis = live ? rv.visible_bits<GK>(tok) : 0u;
                 // only a row's last group is shorter than 16 tokens
                 const uint32_t keys = last ? (v1 - v) * GK - (v1 == rv.ng ? (0u - c.slen) & (GK - 1u) : 0u) : (uint32_t)KS;
-                const uint32_t bytes = keys * 2u * Q8_ROW_BYTES + (first ? Q_BYTES : 0);
+                const uint32_t bytes = keys * Q8_ROW_BYTES;
                 const bool is_v = lane >= NGROUP;
                 const unsigned char* src = (is_v ? p.map.v_pool : p.map.k_pool) + (size_t)id * p.map.block_stride + (size_t)(tok & bs_mask) * Q8_ROW_BYTES;
                 unsigned char* sb = smem + (size_t)slot * STAGE_BYTES;
                 const uint32_t sbase = smem_u32(sb), dst = sbase + (is_v ? V_OFF + g * VPITCH : g * KPITCH);
-                if (fill >= NSTAGE && !mbar_wait_bounded(&empty_bar[slot], ((fill / NSTAGE) & 1u) ^ 1u, abort_flag, wait_us)) {
+                const uint32_t parity = ((fill / NSTAGE) & 1u) ^ 1u;
+                auto open_stage = [&](uint64_t* full, uint32_t tx) {
+                    if (lane == 0) asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(full)), "r"(tx) : "memory");
+                    __syncwarp();
+                };
+                auto copy_group = [&](uint64_t* full) {
+                    if (!OXI_IN_BOUNDS(c.row < p.batch && tok + nk <= c.slen && ps < (uint32_t)PAGES && id < p.map.num_blocks, status))
+                        asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(full)), "r"(nk * Q8_ROW_BYTES) : "memory");
+                    else
+                        bulk_g2s_hint(dst, src, nk * Q8_ROW_BYTES, full, policy);
+                };
+                if (fill >= NSTAGE && !mbar_wait_bounded(&k_empty[slot], parity, abort_flag, wait_us)) {
                     ok = false;
                     break;
                 }
                 // test support: this CTA's stage goes missing
                 if (fault.skip_plus1 && blockIdx.x == 0 && fill + 1u == fault.skip_plus1) continue;
-                if (lane == 0)
-                    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full_bar[slot])), "r"(bytes) : "memory");
-                __syncwarp();
-                if (lane < 2 * NGROUP) {
-                    if (live) {
-                        if (!OXI_IN_BOUNDS(c.row < p.batch && tok + nk <= c.slen && ps < (uint32_t)PAGES && id < p.map.num_blocks, status))
-                            asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full_bar[slot])),
-                                         "r"(nk * Q8_ROW_BYTES) : "memory");
-                        else
-                            bulk_g2s_hint(dst, src, nk * Q8_ROW_BYTES, &full_bar[slot], policy);
-                    }
+                open_stage(&k_full[slot], bytes + (first ? Q_BYTES : 0));
+                if (lane < NGROUP) {
+                    if (live) copy_group(&k_full[slot]);
                 } else if (first && lane == 2 * NGROUP) {
-                    bulk_g2s(sbase + Q_OFF, reinterpret_cast<const char*>(p.q) + (size_t)c.row * Q_BYTES, Q_BYTES, &full_bar[slot]);
+                    bulk_g2s(sbase + Q_OFF, reinterpret_cast<const char*>(p.q) + (size_t)c.row * Q_BYTES, Q_BYTES, &k_full[slot]);
                 }
                 if (lane < NGROUP) {
                     reinterpret_cast<uint16_t*>(sb + DESC_OFF + 16)[lane] = (uint16_t)vis;
@@ -292,10 +301,18 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p.map.k_scales + at) : "memory");
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16u), "l"(p.map.v_scales + at) : "memory");
                     }
-                    asm volatile("cp.async.mbarrier.arrive.shared::cta.b64 [%0];" ::"r"(smem_u32(&full_bar[slot])) : "memory");
+                    asm volatile("cp.async.mbarrier.arrive.shared::cta.b64 [%0];" ::"r"(smem_u32(&k_full[slot])) : "memory");
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&full_bar[slot]);
+                if (lane == 0) mbar_arrive(&k_full[slot]);
+                if (fill >= NSTAGE && !mbar_wait_bounded(&v_empty[slot], parity, abort_flag, wait_us)) {
+                    ok = false;
+                    break;
+                }
+                open_stage(&v_full[slot], bytes);
+                if (is_v && lane < 2 * NGROUP && live) copy_group(&v_full[slot]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[slot]);
             }
             cur = nxt;
             nxt = nxt2;
@@ -310,12 +327,11 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
         }
         if (ok) {
             const uint32_t slot = fill % NSTAGE;
-            if (fill < NSTAGE || mbar_wait_bounded(&empty_bar[slot], ((fill / NSTAGE) & 1u) ^ 1u, abort_flag, wait_us)) {
+            if (fill < NSTAGE || mbar_wait_bounded(&k_empty[slot], ((fill / NSTAGE) & 1u) ^ 1u, abort_flag, wait_us)) {
                 if (lane == 0) {
                     *reinterpret_cast<uint4*>(smem + (size_t)slot * STAGE_BYTES + DESC_OFF) = make_uint4(0u, 0u, F_END, 0u);
-                    mbar_arrive(&full_bar[slot]);
+                    mbar_arrive(&k_full[slot]);
                 }
-                ++fill;
             } else {
                 ok = false;
             }
@@ -323,8 +339,10 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
         if (!ok) {
             // give the copies already issued a bounded time to land before this CTA's shared memory is released
             if (lane == 0) atomicOr(status, DEV_WAIT_TIMEOUT);
-            for (uint32_t k = fill > NSTAGE ? fill - NSTAGE : 0; k < fill; ++k)
-                mbar_wait_drain(&full_bar[k % NSTAGE], (k / NSTAGE) & 1u, wait_us);
+            for (uint32_t k = fill > NSTAGE ? fill - NSTAGE : 0; k <= fill; ++k) {
+                mbar_wait_drain(&k_full[k % NSTAGE], (k / NSTAGE) & 1u, wait_us);
+                mbar_wait_drain(&v_full[k % NSTAGE], (k / NSTAGE) & 1u, wait_us);
+            }
         }
         return;
     }
@@ -340,7 +358,7 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
 
     for (uint32_t take = 0;; ++take) {
         const uint32_t slot = take % NSTAGE;
-        if (!mbar_wait_bounded(&full_bar[slot], (take / NSTAGE) & 1u, abort_flag, wait_us)) {
+        if (!mbar_wait_bounded(&k_full[slot], (take / NSTAGE) & 1u, abort_flag, wait_us)) {
             if (lane == 0) atomicOr(status, DEV_WAIT_TIMEOUT);
             break;
         }
@@ -369,14 +387,6 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
         float ks = table[0], vs = table[4];
         if (!whole) {
             if (vis == 0u) ks = vs = 0.0f;  // no group: its scales are not in the table
-            // codes that are not visible may be anything (an e4m3 NaN times the weight 0 would be a NaN)
-            for (uint32_t i = lane; i < KS * 8u; i += 32) {
-                const uint32_t key = i >> 3;
-                if (!(((key < 32u ? vis2.x : vis2.y) >> (key & 31u)) & 1u))
-                    *reinterpret_cast<uint4*>(sb + V_OFF + (key / GK) * VPITCH + (key % GK) * Q8_ROW_BYTES + kvh * HD + (i & 7u) * 16u) =
-                        make_uint4(0, 0, 0, 0);
-            }
-            __syncwarp();
         }
         const float xs = ks * X_SCALE;
         const float lv = fmaxf(__log2f(vs), -100.0f), ivs = exp2f(-lv);
@@ -404,6 +414,22 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
                     mma_free(s[i], a0, a1, a2, a3, qb[4 * hf + j][0], qb[4 * hf + j][1]);
                 }
             }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&k_empty[slot]);
+        if (!mbar_wait_bounded(&v_full[slot], (take / NSTAGE) & 1u, abort_flag, wait_us)) {
+            if (lane == 0) atomicOr(status, DEV_WAIT_TIMEOUT);
+            break;
+        }
+        if (!whole) {
+            // codes that are not visible may be anything (an e4m3 NaN times the weight 0 would be a NaN)
+            for (uint32_t i = lane; i < KS * 8u; i += 32) {
+                const uint32_t key = i >> 3;
+                if (!(((key < 32u ? vis2.x : vis2.y) >> (key & 31u)) & 1u))
+                    *reinterpret_cast<uint4*>(sb + V_OFF + (key / GK) * VPITCH + (key % GK) * Q8_ROW_BYTES + kvh * HD + (i & 7u) * 16u) =
+                        make_uint4(0, 0, 0, 0);
+            }
+            __syncwarp();
         }
         // the first V codes, while the scores settle: k-step i of PV has the keys of tile i in the same order
         const uint32_t vaddr = smem_u32(sb) + V_OFF + (lane & 3) * VPITCH + (((lane >> 2) & 1) + 2 * (lane >> 3)) * Q8_ROW_BYTES + kvh * HD;
@@ -480,7 +506,7 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
         }
         if (!whole) fence_proxy_async_smem();  // the zeros above, before the next copy into this stage
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty_bar[slot]);
+        if (lane == 0) mbar_arrive(&v_empty[slot]);
         if (!(desc.z & F_LAST)) continue;
 
         // ---- the item is complete
