@@ -522,6 +522,14 @@ static int32_t paged_q8_map(const oxi_paged_q8_layout* l, const char* who, Q8Map
     m->num_blocks = l->num_blocks;
     return OXI_OK;
 }
+// Launches go to the calling thread's current device: another one than the handle's is refused (its stream would be
+// another device's, and the handle's workspace is not mapped there).
+static bool wrong_device(const oxi_handle* h) {
+    int dev = -1;
+    return cudaGetDevice(&dev) != cudaSuccess || dev != h->device;
+}
+#define REQ_DEVICE(name) \
+    if (wrong_device(h)) return fail(OXI_ERR_NO_DEVICE, name ": the handle's device is not the current one")
 #define REQ_ALIGNED(bits, name) \
     if (((uintptr_t)(bits) & 15u) != 0u) return fail(OXI_ERR_ARG, name ": tensors must be 16-byte aligned")
 
@@ -530,6 +538,7 @@ int32_t oxi_append_q8(oxi_handle* h, void* stream, void* q_out, const void* q_in
                       const uint32_t* pos_ids, const oxi_paged_q8_layout* layout, const uint32_t* row_seq, uint32_t rows,
                       float eps) {
     REQ_HANDLE("oxi_append_q8");
+    REQ_DEVICE("oxi_append_q8");
     REQ_PTR(q_out && q_in && k_in && v_in && q_norm_w && k_norm_w && cos_table && sin_table && pos_ids, "oxi_append_q8");
     REQ_BATCH(rows, (h->max_batch > h->max_prefill_rows ? h->max_batch : h->max_prefill_rows), "oxi_append_q8");
     if (!(eps >= 0.0f)) return fail(OXI_ERR_ARG, "oxi_append_q8: eps must be >= 0");
@@ -547,6 +556,7 @@ int32_t oxi_decode_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const voi
                            const oxi_paged_q8_layout* layout, const uint32_t* seq_lens, uint32_t batch, uint32_t window,
                            uint32_t sinks) {
     REQ_HANDLE("oxi_decode_attn_q8");
+    REQ_DEVICE("oxi_decode_attn_q8");
     REQ_PTR(ctx_out && q && seq_lens, "oxi_decode_attn_q8");
     REQ_BATCH(batch, h->max_batch, "oxi_decode_attn_q8");
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_decode_attn_q8");
@@ -562,6 +572,7 @@ int32_t oxi_prefill_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const vo
                             const oxi_paged_q8_layout* layout, const uint32_t* row_seq, const uint32_t* seq_lens,
                             uint32_t rows, uint32_t window, uint32_t sinks) {
     REQ_HANDLE("oxi_prefill_attn_q8");
+    REQ_DEVICE("oxi_prefill_attn_q8");
     REQ_PTR(ctx_out && q && row_seq && seq_lens, "oxi_prefill_attn_q8");
     REQ_BATCH(rows, h->max_prefill_rows, "oxi_prefill_attn_q8");
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_prefill_attn_q8");
@@ -581,6 +592,7 @@ int32_t oxi_decode_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const 
                               uint32_t window, uint32_t sinks) {
     if (window == 0u || sinks == 0u) return oxi_decode_attn(h, stream, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, batch, window);
     REQ_HANDLE("oxi_decode_attn_sinks");
+    REQ_DEVICE("oxi_decode_attn_sinks");
     REQ_PTR(ctx_out && q && k_ptrs && v_ptrs && seq_lens, "oxi_decode_attn_sinks");
     REQ_BATCH(batch, h->max_batch, "oxi_decode_attn_sinks");
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_decode_attn_sinks");
@@ -594,6 +606,7 @@ int32_t oxi_decode_attn_paged_sinks(oxi_handle* h, void* stream, void* ctx_out, 
                                     uint32_t window, uint32_t sinks) {
     if (window == 0u || sinks == 0u) return oxi_decode_attn_paged(h, stream, ctx_out, q, gate, layout, seq_lens, batch, window);
     REQ_HANDLE("oxi_decode_attn_paged_sinks");
+    REQ_DEVICE("oxi_decode_attn_paged_sinks");
     REQ_PTR(ctx_out && q && seq_lens, "oxi_decode_attn_paged_sinks");
     REQ_BATCH(batch, h->max_batch, "oxi_decode_attn_paged_sinks");
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_decode_attn_paged_sinks");
@@ -613,6 +626,7 @@ int32_t oxi_append_decode_sinks(oxi_handle* h, void* stream, void* ctx_out, void
         return oxi_append_decode(h, stream, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos_table, sin_table, pos_ids,
                                  seq_lens, k_ptrs, v_ptrs, batch, window, eps);
     REQ_HANDLE("oxi_append_decode_sinks");
+    REQ_DEVICE("oxi_append_decode_sinks");
     REQ_PTR(ctx_out && q_io && k_in && v_in && q_norm_w && k_norm_w && cos_table && sin_table && pos_ids &&
                 seq_lens && k_ptrs && v_ptrs, "oxi_append_decode_sinks");
     REQ_BATCH(batch, h->max_batch, "oxi_append_decode_sinks");
@@ -634,6 +648,7 @@ int32_t oxi_append_decode_paged_sinks(oxi_handle* h, void* stream, void* ctx_out
         return oxi_append_decode_paged(h, stream, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos_table, sin_table,
                                        seq_lens, layout, batch, window, eps);
     REQ_HANDLE("oxi_append_decode_paged_sinks");
+    REQ_DEVICE("oxi_append_decode_paged_sinks");
     REQ_PTR(ctx_out && q_io && k_in && v_in && q_norm_w && k_norm_w && cos_table && sin_table && seq_lens,
             "oxi_append_decode_paged_sinks");
     REQ_BATCH(batch, h->max_batch, "oxi_append_decode_paged_sinks");
@@ -653,6 +668,7 @@ int32_t oxi_prefill_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const
                                uint32_t window, uint32_t sinks) {
     if (window == 0u || sinks == 0u) return oxi_prefill_attn(h, stream, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, rows, window);
     REQ_HANDLE("oxi_prefill_attn_sinks");
+    REQ_DEVICE("oxi_prefill_attn_sinks");
     REQ_PTR(ctx_out && q && k_ptrs && v_ptrs && seq_lens, "oxi_prefill_attn_sinks");
     REQ_BATCH(rows, h->max_prefill_rows, "oxi_prefill_attn_sinks");
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_prefill_attn_sinks");
@@ -669,6 +685,7 @@ int32_t oxi_prefill_attn_paged_sinks(oxi_handle* h, void* stream, void* ctx_out,
                                      uint32_t rows, uint32_t window, uint32_t sinks) {
     if (window == 0u || sinks == 0u) return oxi_prefill_attn_paged(h, stream, ctx_out, q, gate, layout, row_seq, seq_lens, rows, window);
     REQ_HANDLE("oxi_prefill_attn_paged_sinks");
+    REQ_DEVICE("oxi_prefill_attn_paged_sinks");
     REQ_PTR(ctx_out && q && row_seq && seq_lens, "oxi_prefill_attn_paged_sinks");
     REQ_BATCH(rows, h->max_prefill_rows, "oxi_prefill_attn_paged_sinks");
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_prefill_attn_paged_sinks");

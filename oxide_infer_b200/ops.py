@@ -123,6 +123,19 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def _ptrs(*tensors):
+    """Device addresses of contiguous tensors (None stays None)."""
+    out = []
+    for t in tensors:
+        if t is None:
+            out.append(None)
+        elif t.is_contiguous():
+            out.append(t.data_ptr())
+        else:
+            raise ValueError("tensors passed to liboxi_kv must be contiguous")
+    return out
+
+
 class KvPath:
     """One per device: owns the library workspace (oxi_create / oxi_destroy)."""
 
@@ -145,6 +158,10 @@ class KvPath:
             self.close()
         except Exception:
             pass
+
+    def _stream(self) -> int:
+        """torch's current stream on the handle's device."""
+        return torch._C._cuda_getCurrentRawStream(self.device)
 
     @property
     def workspace_bytes(self) -> int:
@@ -240,63 +257,61 @@ class KvPath:
         """RMSNorm + RoPE of q and k and the quantising append of k and v (oxi_append_q8): row r is token pos_ids[r]
         of table row row_seq[r] (None: of row r).  q_out may be q_in."""
         n = q_in.shape[0] if rows is None else rows
-        _check(self.lib.oxi_append_q8(self.h, _stream(), _p(q_out), _p(q_in), _p(k_in), _p(v_in), _p(q_norm_w),
-                                      _p(k_norm_w), _p(cos), _p(sin), _p(pos_ids), C.addressof(layout), _p(row_seq), n,
-                                      eps), "oxi_append_q8")
+        ptrs = _ptrs(q_out, q_in, k_in, v_in, q_norm_w, k_norm_w, cos, sin, pos_ids)
+        _check(self.lib.oxi_append_q8(self.h, self._stream(), *ptrs, C.addressof(layout), _p(row_seq), n, eps),
+               "oxi_append_q8")
 
     def decode_attn_q8(self, ctx_out, q, gate, layout: PagedQ8Layout, seq_lens, window: int = 0, sinks: int = 0,
                        batch: int | None = None):
         """Attention of one token per sequence over the 8-bit cache; window 0: every token is visible, otherwise the
         last `window` and the first `sinks` tokens are (oxi_decode_attn_q8)."""
         b = q.shape[0] if batch is None else batch
-        _check(self.lib.oxi_decode_attn_q8(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), C.addressof(layout),
+        _check(self.lib.oxi_decode_attn_q8(self.h, self._stream(), *_ptrs(ctx_out, q, gate), C.addressof(layout),
                                            _p(seq_lens), b, window, sinks), "oxi_decode_attn_q8")
 
     def prefill_attn_q8(self, ctx_out, q, gate, layout: PagedQ8Layout, row_seq, seq_lens, window: int = 0,
                         sinks: int = 0, rows: int | None = None):
         """Attention of the rows of a prefill wave over the 8-bit cache (oxi_prefill_attn_q8)."""
         n = q.shape[0] if rows is None else rows
-        _check(self.lib.oxi_prefill_attn_q8(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), C.addressof(layout),
-                                            _p(row_seq), _p(seq_lens), n, window, sinks), "oxi_prefill_attn_q8")
+        _check(self.lib.oxi_prefill_attn_q8(self.h, self._stream(), *_ptrs(ctx_out, q, gate), C.addressof(layout),
+                                            *_ptrs(row_seq, seq_lens), n, window, sinks), "oxi_prefill_attn_q8")
 
     # ---- sliding window with sinks (the first tokens stay visible) over the f16 caches
     def decode_attn_sinks(self, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, window: int, sinks: int,
                           batch: int | None = None):
         b = q.shape[0] if batch is None else batch
-        _check(self.lib.oxi_decode_attn_sinks(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), _p(k_ptrs), _p(v_ptrs),
-                                              _p(seq_lens), b, window, sinks), "oxi_decode_attn_sinks")
+        ptrs = _ptrs(ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens)
+        _check(self.lib.oxi_decode_attn_sinks(self.h, self._stream(), *ptrs, b, window, sinks), "oxi_decode_attn_sinks")
 
     def decode_attn_paged_sinks(self, ctx_out, q, gate, layout: PagedLayout, seq_lens, window: int, sinks: int,
                                 batch: int | None = None):
         b = q.shape[0] if batch is None else batch
-        _check(self.lib.oxi_decode_attn_paged_sinks(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), C.addressof(layout),
+        _check(self.lib.oxi_decode_attn_paged_sinks(self.h, self._stream(), *_ptrs(ctx_out, q, gate), C.addressof(layout),
                                                     _p(seq_lens), b, window, sinks), "oxi_decode_attn_paged_sinks")
 
     def append_decode_sinks(self, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos, sin, pos_ids, seq_lens,
                             k_ptrs, v_ptrs, window: int, sinks: int, eps: float = 1e-5):
-        _check(self.lib.oxi_append_decode_sinks(self.h, _stream(), _p(ctx_out), _p(q_io), _p(k_in), _p(v_in), _p(gate),
-                                                _p(q_norm_w), _p(k_norm_w), _p(cos), _p(sin), _p(pos_ids), _p(seq_lens),
-                                                _p(k_ptrs), _p(v_ptrs), q_io.shape[0], window, sinks, eps),
+        ptrs = _ptrs(ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos, sin, pos_ids, seq_lens, k_ptrs, v_ptrs)
+        _check(self.lib.oxi_append_decode_sinks(self.h, self._stream(), *ptrs, q_io.shape[0], window, sinks, eps),
                "oxi_append_decode_sinks")
 
     def append_decode_paged_sinks(self, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos, sin, seq_lens,
                                   layout: PagedLayout, window: int, sinks: int, eps: float = 1e-5):
-        _check(self.lib.oxi_append_decode_paged_sinks(self.h, _stream(), _p(ctx_out), _p(q_io), _p(k_in), _p(v_in),
-                                                      _p(gate), _p(q_norm_w), _p(k_norm_w), _p(cos), _p(sin),
-                                                      _p(seq_lens), C.addressof(layout), q_io.shape[0], window, sinks,
-                                                      eps), "oxi_append_decode_paged_sinks")
+        ptrs = _ptrs(ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos, sin, seq_lens)
+        _check(self.lib.oxi_append_decode_paged_sinks(self.h, self._stream(), *ptrs, C.addressof(layout), q_io.shape[0],
+                                                      window, sinks, eps), "oxi_append_decode_paged_sinks")
 
     def prefill_attn_sinks(self, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, window: int, sinks: int,
                            rows: int | None = None):
         n = q.shape[0] if rows is None else rows
-        _check(self.lib.oxi_prefill_attn_sinks(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), _p(k_ptrs), _p(v_ptrs),
-                                               _p(seq_lens), n, window, sinks), "oxi_prefill_attn_sinks")
+        ptrs = _ptrs(ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens)
+        _check(self.lib.oxi_prefill_attn_sinks(self.h, self._stream(), *ptrs, n, window, sinks), "oxi_prefill_attn_sinks")
 
     def prefill_attn_paged_sinks(self, ctx_out, q, gate, layout: PagedLayout, row_seq, seq_lens, window: int, sinks: int,
                                  rows: int | None = None):
         n = q.shape[0] if rows is None else rows
-        _check(self.lib.oxi_prefill_attn_paged_sinks(self.h, _stream(), _p(ctx_out), _p(q), _p(gate), C.addressof(layout),
-                                                     _p(row_seq), _p(seq_lens), n, window, sinks),
+        _check(self.lib.oxi_prefill_attn_paged_sinks(self.h, self._stream(), *_ptrs(ctx_out, q, gate), C.addressof(layout),
+                                                     *_ptrs(row_seq, seq_lens), n, window, sinks),
                "oxi_prefill_attn_paged_sinks")
 
     def prefill_attn(self, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, window: int = 0,
