@@ -24,6 +24,7 @@ constexpr int COMBOS = 2 * NKV;                    // K or V of a KV head
 constexpr int STEP_THREADS = (NQ + COMBOS) * 32;   // a warp for each head of the row
 constexpr int WAVE_WARPS = 16, WAVE_THREADS = WAVE_WARPS * 32;
 constexpr int KV_PAIRS = NKV;                      // pairs of K or V heads of a row: K 0-1, K 2-3, V 0-1, V 2-3
+constexpr int Q_PARTS = 2, Q_PAIRS = NQ / 2 / Q_PARTS;  // CTAs for a window's query heads, pairs of heads of a warp there
 }  // namespace aq
 
 struct AppendQ8Params {
@@ -233,20 +234,21 @@ __device__ __forceinline__ void store_dims(unsigned char* head, int j, const flo
     reinterpret_cast<uint32_t*>(head)[16 + j] = q8_codes2<kFmt>(x[4], x[5], inv) | (q8_codes2<kFmt>(x[6], x[7], inv) << 16);
 }
 
-// Row r is a token of table row row_seq[r].  A CTA takes a window of 16 rows and one of kSplit groups of heads: the
-// query heads of its rows, and for its K and V heads the segments that BEGIN in its window, to their end: rows behind
-// the window (its last segment may go on for up to 255 rows) are read twice, once for the scale and once for the
-// codes.  Rows at the window's start that go on with a segment of the window before are left to that CTA.  Warp w owns
-// row w of the window; all its K and V loads are in flight together.
+// Row r is a token of table row row_seq[r].  grid = (windows of 16 rows, kSplit + Q_PARTS), warp w has row w of the window.
+// CTAs with y >= kSplit do query heads, with nothing to agree on; CTA y < kSplit takes one of kSplit groups of K and V heads
+// for the segments that BEGIN in its window, to their end: rows behind the window (its last segment may go on for up to 255
+// rows) are read twice, once for the scale and once for the codes.  Rows at the window's start that go on with a segment
+// of the window before are left to that CTA.
 template <uint32_t kFmt, int kSplit>
 __global__ void __launch_bounds__(aq::WAVE_THREADS, 2)
 append_q8_wave_kernel(const AppendQ8Params p) {
     using namespace aq;
     constexpr int ROWS = WAVE_WARPS;             // a warp for each row of the window
-    constexpr int NP = KV_PAIRS / kSplit;        // K / V pairs of a warp; it does twice as many query pairs
+    constexpr int NP = KV_PAIRS / kSplit;        // K / V pairs of a warp
     // per row of the window; a segment is named by its first row
     __shared__ uint32_t s_pos[ROWS], s_seq[ROWS], s_id[ROWS], s_end[ROWS], s_bad[ROWS];
     __shared__ int s_lead[ROWS];  // the row's segment, -1: not of this CTA
+    __shared__ uint32_t s_list[ROWS], s_grown[COMBOS];  // the segments in order; those whose stored codes move to a larger scale
     __shared__ float s_amax[ROWS][COMBOS], s_old[ROWS][COMBOS], s_scale[ROWS][COMBOS], s_tailmax[ROWS][COMBOS];
     __shared__ uint32_t s_leaders, s_tail;
     const uint32_t row0 = blockIdx.x * ROWS;
@@ -255,7 +257,34 @@ append_q8_wave_kernel(const AppendQ8Params p) {
     const int pair0 = (int)blockIdx.y * NP;      // and its first K / V pair
     const uint32_t lbs = p.map.lbs, bs = 1u << lbs;
     pdl_launch_dependents();
+    // this warp's row, read by every warp itself: its rotary values are then on their way before the window is sorted out
+    const uint32_t my_pos = row0 + w < p.rows ? p.pos_ids[row0 + w] : 0xffffffffu;
+    const bool there = my_pos < p.max_seq_len && (my_pos >> lbs) < p.map.max_blocks;  // a row that is skipped is not read either
+    const uint32_t pos = there ? my_pos : 0u;
+    const Dims cv = dims_of(p.cos_t + (size_t)pos * HD, j), sv = dims_of(p.sin_t + (size_t)pos * HD, j);
+    const size_t row = there ? row0 + w : 0u;
+    if (blockIdx.y >= kSplit) {
+        const Dims qw = dims_of(p.q_norm_w, j);
+        pdl_wait();  // q comes from the preceding kernel
+        if (!there) return;
+        const size_t at = (row * NQ + 2 * Q_PAIRS * (blockIdx.y - kSplit) + half) * HD;
+        Dims y[Q_PAIRS];
+#pragma unroll
+        for (int k = 0; k < Q_PAIRS; k++) y[k] = dims_of(p.q_in + at + 2 * k * HD, j);
+#pragma unroll
+        for (int k = 0; k < Q_PAIRS; k++) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = y[k][i];
+            norm_rope_dims(v, qw, cv, sv, p.eps);
+            uint16_t* out = p.q_out + at + 2 * k * HD;
+            reinterpret_cast<uint2*>(out)[j] = make_uint2(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]));
+            reinterpret_cast<uint2*>(out)[16 + j] = make_uint2(pack_h2(v[4], v[5]), pack_h2(v[6], v[7]));
+        }
+        return;
+    }
     if (tid == 0) s_tail = 256u;
+    uint32_t block_id = 0;  // warp 0: the block of the segment that begins at row `lane`
     if (warp == 0) {
         const uint32_t r = row0 + (uint32_t)lane;
         uint32_t pos = 0, seq = 0, ppos = 0, pseq = 0;
@@ -281,8 +310,10 @@ append_q8_wave_kernel(const AppendQ8Params p) {
             // where the segment that begins here ends inside the window: the next leader or row that is not valid
             const uint32_t stop = (leaders | ~valids) & ~(0xffffffffu >> (31 - lane));
             s_end[lane] = min((uint32_t)ROWS, stop ? (uint32_t)__ffs((int)stop) - 1u : 32u);
-            s_id[lane] = leader ? p.map.block_tables[(size_t)seq * p.map.max_blocks + (pos >> lbs)] : 0u;
+            if (leader) block_id = p.map.block_tables[(size_t)seq * p.map.max_blocks + (pos >> lbs)];
             s_bad[lane] = 0u;
+            if (leader) s_list[__popc(leaders & ((1u << lane) - 1u))] = lane;
+            if (lane < COMBOS) s_grown[lane] = 0u;
         }
         if (lane == 0) s_leaders = leaders;
     }
@@ -290,12 +321,10 @@ append_q8_wave_kernel(const AppendQ8Params p) {
         s_amax[tid / COMBOS][tid % COMBOS] = 0.0f;
         s_tailmax[tid / COMBOS][tid % COMBOS] = 0.0f;
     }
+    const Dims kw = dims_of(p.k_norm_w, j);
     __syncthreads();
-    const uint32_t leaders = s_leaders, pos = s_pos[w];
-    const bool there = pos != 0xffffffffu;  // a row that is skipped is not read either
+    const uint32_t leaders = s_leaders;
     const int last = s_lead[ROWS - 1];
-    const Dims cv = dims_of(p.cos_t + (size_t)(there ? pos : 0u) * HD, j), sv = dims_of(p.sin_t + (size_t)(there ? pos : 0u) * HD, j);
-    const Dims kw = dims_of(p.k_norm_w, j), qw = dims_of(p.q_norm_w, j);
     if (tid < 256) {
         // rows behind the window that go on with its last row's segment: the first that does not ends the tail
         const uint32_t i = 1u + (uint32_t)tid, r = row0 + ROWS - 1u + i, lp = s_pos[ROWS - 1];
@@ -305,35 +334,40 @@ append_q8_wave_kernel(const AppendQ8Params p) {
     }
     __syncthreads();
     const uint32_t tail = s_tail;
-    // another run of this call in a segment's block would race with it: both are refused
-    for (uint32_t m = leaders; m; m &= m - 1u) {
-        const int li = __ffs((int)m) - 1;
-        const uint32_t seq = s_seq[li], blk = s_pos[li] >> lbs, first = row0 + li, end = row0 + s_end[li] + (li == last ? tail : 0u);
-        auto look = [&](uint32_t r) {
-            if (r < first || r >= end) {
-                const uint32_t q = p.pos_ids[r];
-                if ((q >> lbs) == blk && q < p.max_seq_len) s_bad[li] = 1u;
-            }
-        };
-        const uint32_t quads = (((uintptr_t)p.row_seq) & 15u) == 0u ? p.rows / 4u : 0u;
-        for (uint32_t i = tid; i < quads; i += WAVE_THREADS) {
-            const uint4 q = reinterpret_cast<const uint4*>(p.row_seq)[i];
-            if (q.x == seq) look(4u * i);
-            if (q.y == seq) look(4u * i + 1u);
-            if (q.z == seq) look(4u * i + 2u);
-            if (q.w == seq) look(4u * i + 3u);
+    // another run of this call in a segment's block would race with it: both are refused (a thread for each segment and
+    // four rows of the call)
+    const uint32_t quads = (p.rows + 3u) / 4u, nsegs = (uint32_t)__popc(leaders), looks = nsegs * quads;
+    const bool aligned = (((uintptr_t)p.row_seq) & 15u) == 0u;
+    for (uint32_t i = tid; i < looks; i += WAVE_THREADS) {
+        const uint32_t rank = nsegs == 1u ? 0u : i / quads, r0 = (i - rank * quads) * 4u, li = s_list[rank], seq = s_seq[li];
+        uint4 q = make_uint4(~seq, ~seq, ~seq, ~seq);
+        if (aligned && r0 + 4u <= p.rows) {
+            q = *reinterpret_cast<const uint4*>(p.row_seq + r0);
+        } else {
+            q.x = p.row_seq[r0];
+            if (r0 + 1u < p.rows) q.y = p.row_seq[r0 + 1u];
+            if (r0 + 2u < p.rows) q.z = p.row_seq[r0 + 2u];
+            if (r0 + 3u < p.rows) q.w = p.row_seq[r0 + 3u];
         }
-        for (uint32_t i = 4u * quads + tid; i < p.rows; i += WAVE_THREADS)
-            if (p.row_seq[i] == seq) look(i);
+        auto look = [&](uint32_t r, uint32_t s) {
+            if (s != seq || (r >= row0 + li && r < row0 + s_end[li] + ((int)li == last ? tail : 0u))) return;
+            const uint32_t at = p.pos_ids[r];
+            if ((at >> lbs) == (s_pos[li] >> lbs) && at < p.max_seq_len) s_bad[li] = 1u;
+        };
+        look(r0, q.x);
+        look(r0 + 1u, q.y);
+        look(r0 + 2u, q.z);
+        look(r0 + 3u, q.w);
     }
-    pdl_wait();  // q, k, v come from the preceding kernel; the cache may still be read by it
+    if (warp == 0 && lane < ROWS) s_id[lane] = block_id;
+    __syncthreads();
+    pdl_wait();  // k and v come from the preceding kernel; the cache may still be read by it
     // heads of pair i: K (i < 2) or V, heads 2 (i mod 2) and + 1; combination (K 0-3, V 0-3) of this lane's head
     auto combo_of = [&](int i) { return 2 * i + half; };
     auto kv_head = [&](int i, size_t row) {
         return (i < KV_PAIRS / 2 ? p.k_in : p.v_in) + (row * NKV + 2 * (i % (KV_PAIRS / 2)) + half) * HD;
     };
-    const size_t row = there ? row0 + w : 0u;
-    float x[NP][8], y[8];
+    float x[NP][8];
 #pragma unroll
     for (int k = 0; k < NP; k++) load_dims(kv_head(pair0 + k, row), j, x[k]);
     if (tid < ROWS * COMBOS) {  // a segment that begins behind slot 0 starts from the block's scale
@@ -386,17 +420,7 @@ append_q8_wave_kernel(const AppendQ8Params p) {
             if (c == 0 && blockIdx.y == 0) atomicOr(p.status, no_block ? DEV_BAD_BLOCK : DEV_BLOCK_CONFLICT);
         } else if (c / (COMBOS / kSplit) == (int)blockIdx.y) {
             ((c < NKV ? p.map.k_scales : p.map.v_scales) + (size_t)s_id[li] * p.map.scale_stride)[c & (NKV - 1)] = scale;
-        }
-    }
-    // the query heads, while the scales settle
-    if (there) {
-#pragma unroll 4
-        for (int k = 0; k < 2 * NP; k++) {
-            const size_t at = (row * NQ + 2 * (2 * pair0 + k) + half) * HD;
-            load_dims(p.q_in + at, j, y);
-            norm_rope_dims(y, qw, cv, sv, p.eps);
-            reinterpret_cast<uint2*>(p.q_out + at)[j] = make_uint2(pack_h2(y[0], y[1]), pack_h2(y[2], y[3]));
-            reinterpret_cast<uint2*>(p.q_out + at)[16 + j] = make_uint2(pack_h2(y[4], y[5]), pack_h2(y[6], y[7]));
+            if (scale > s_old[li][c] && (s_pos[li] & (bs - 1u)) != 0u) atomicOr(&s_grown[c], 1u << li);
         }
     }
     __syncthreads();
@@ -404,13 +428,11 @@ append_q8_wave_kernel(const AppendQ8Params p) {
     auto head_codes = [&](int li, int c) {  // this head's codes in the segment's block
         return (c < NKV ? p.map.k_pool : p.map.v_pool) + (size_t)s_id[li] * p.map.block_stride + (c & (NKV - 1)) * HD;
     };
-    for (uint32_t m = leaders; m; m &= m - 1u) {
-        const int li = __ffs((int)m) - 1;
-        const uint32_t slots = s_pos[li] & (bs - 1u);
-        if (slots == 0u || !usable(li)) continue;
-        for (int k = 0; k < 2 * NP; k++) {
-            const int c = 2 * pair0 + k;
-            if (s_scale[li][c] > s_old[li][c]) requantise<kFmt>(head_codes(li, c), w, ROWS, slots, lane, s_old[li][c], s_scale[li][c]);
+    for (int k = 0; k < 2 * NP; k++) {
+        const int c = 2 * pair0 + k;
+        for (uint32_t m = s_grown[c]; m; m &= m - 1u) {
+            const int li = __ffs((int)m) - 1;
+            requantise<kFmt>(head_codes(li, c), w, ROWS, s_pos[li] & (bs - 1u), lane, s_old[li][c], s_scale[li][c]);
         }
     }
     const int li = there ? s_lead[w] : -1;
@@ -438,17 +460,19 @@ append_q8_wave_kernel(const AppendQ8Params p) {
 
 template <uint32_t kFmt, int kSplit>
 static cudaError_t launch_wave(cudaStream_t stream, const AppendQ8Params& p) {
-    return launch_pdl(append_q8_wave_kernel<kFmt, kSplit>, dim3((p.rows + aq::WAVE_WARPS - 1) / aq::WAVE_WARPS, kSplit), dim3(aq::WAVE_THREADS), 0,
+    return launch_pdl(append_q8_wave_kernel<kFmt, kSplit>, dim3((p.rows + aq::WAVE_WARPS - 1) / aq::WAVE_WARPS, kSplit + aq::Q_PARTS), dim3(aq::WAVE_THREADS), 0,
                       stream, p);
 }
 
 template <uint32_t kFmt>
 static cudaError_t launch_fmt(cudaStream_t stream, const AppendQ8Params& p) {
     if (!p.row_seq) return launch_pdl(append_q8_step_kernel<kFmt>, dim3(p.rows), dim3(aq::STEP_THREADS), 0, stream, p);
-    // two CTAs fit an SM: four groups of heads while all CTAs are resident at once, else two (fewer CTAs repeat a window's
-    // set-up).  Measured, us: 128 rows in one run, blocks of 16 / 256: 3.5 / 12.2 with four groups, 4.9 / 22.0 with two;
-    // 2,048 rows 10.3 / 16.5 against 7.3 / 27.2; 4,096 rows 23.2 / 28.2 against 17.8 / 32.4.
-    return p.rows <= 1184u ? launch_wave<kFmt, 4>(stream, p) : launch_wave<kFmt, 2>(stream, p);
+    // How many CTAs share a window's K and V heads.  More of them give a long segment's rows more warps (rows behind the
+    // window are serial work), fewer repeat a window's set-up less often; two CTAs fit an SM.  Measured, us, for 1 / 2 / 4
+    // groups: 128 rows in one run, blocks of 16: 4.6 / 3.4 / 2.7, of 256: 27.9 / 19.1 / 10.9; 4,096 rows in runs of 128,
+    // blocks of 16: 13.3 / 16.0 / 22.7, of 64: 23.2 / 18.2 / 22.0, of 256: 40.2 / 28.5 / 23.8.
+    if (p.rows <= 1184u || p.map.lbs > 6u) return launch_wave<kFmt, 4>(stream, p);
+    return p.map.lbs == 6u ? launch_wave<kFmt, 2>(stream, p) : launch_wave<kFmt, 1>(stream, p);
 }
 
 cudaError_t launch_append_q8(cudaStream_t stream, void* q_out, const void* q_in, const void* k_in, const void* v_in,
