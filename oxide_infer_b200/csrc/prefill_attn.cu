@@ -428,13 +428,20 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
 
     // Claims the next item and prepares its tables in buffer `buf`; run by all lanes of the K loader warp
     // while the other roles finish the current item (before the loop for the first item).
+    // kSinks with order == nullptr (no plan kernel ran): at most one item per CTA, its index is the CTA's.
+    bool first_item = true;
     auto prepare_item = [&](uint32_t buf) {
         uint32_t item = 0xffffffffu;  // kFault: a CTA one of whose waits gave up claims nothing more, the others take its share
-        if (lane == 0 && (!kFault || *const_cast<volatile uint32_t*>(&s_abort) == 0u)) item = atomicAdd(counter, 1u);
-        item = __shfl_sync(0xffffffffu, item, 0);
+        if (kSinks && !order) {
+            if (first_item) item = blockIdx.x;
+            first_item = false;
+        } else {
+            if (lane == 0 && (!kFault || *const_cast<volatile uint32_t*>(&s_abort) == 0u)) item = atomicAdd(counter, 1u);
+            item = __shfl_sync(0xffffffffu, item, 0);
+        }
         if (lane == 0) s_item[buf] = item;
         if (item >= nitems) return;
-        const uint32_t ud = kSplit ? sp.units[item >> 2] : order[item >> 2];
+        const uint32_t ud = kSplit ? sp.units[item >> 2] : kSinks && !order ? item >> 2 : order[item >> 2];
         if (lane == 0) s_unit[buf] = ud;
         const uint32_t row0 = (kSplit ? (ud & 0xffffu) : ud) * BLK;
         const int kvh = item & 3u;
@@ -1307,7 +1314,16 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
     // the split is for waves that leave SMs idle; larger waves balance by claiming longest first
     // an armed test fault runs the plain instantiation: pointer tables, unsplit, per-thread copies
     const bool armed = flt.skip_plus1 != 0u && !pm && !sinks;
-    const bool split = !armed && ws && ws->max_slots != 0u && part_keys != 0u && nblocks * NKV < (uint32_t)num_sms;
+    bool split = !armed && ws && ws->max_slots != 0u && part_keys != 0u && nblocks * NKV < (uint32_t)num_sms;
+    // with sinks or the 8-bit cache: a window so short that a block's run has no more tiles than the smallest part is not
+    // split (the merge costs 2.5 us: 64 rows, window 64: 16.1 against 18.6 us; window 512 24.9 / 24.7, 1,024 34.3 / 26.7), ...
+    const bool view_variant = sinks || q8;
+    if (view_variant && window && window <= (1u << 22) &&
+        (window + pf::BLK - 1u + 15u + pf::TK - 1u) / pf::TK + (sinks < window ? (sinks + pf::TK - 1u) / pf::TK : (window + pf::TK - 1u) / pf::TK) <=
+            (part_keys + pf::TK - 1u) / pf::TK)
+        split = false;
+    // ... and a wave of at most one item per SM needs no order: no plan kernel
+    const bool direct = view_variant && !split && nblocks * NKV <= (uint32_t)num_sms;
     PfSplit sp{};
     if (split) {
         sp.units = ws->units;
@@ -1319,7 +1335,9 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
         sp.max_slots = ws->max_slots;
         sp.target_items = (uint32_t)num_sms;
     }
-    if (nblocks <= 1024u)
+    if (direct)
+        order = nullptr;
+    else if (nblocks <= 1024u)
         (void)launch_pdl(prefill_plan_small_kernel, dim3(1), dim3(1024), 0, stream, seq_lens, rows, window, sinks, order, counter, sp);
     else
         prefill_plan_kernel<<<1, 1024, 0, stream>>>(seq_lens, rows, window, sinks, order, counter);
