@@ -121,7 +121,7 @@ struct PfView {
     uint64_t scale_stride;
 };
 // The 64-key tiles of a run whose rows' windows start at `wlo` or later and whose tokens end at hi: nst tiles of
-// sinks from token 0, then tiles from token lo on.  Tiles of the 8-bit cache start at a multiple of 16 tokens, so
+// sinks from token 0, then tiles from token lo on.  Tiles of paged caches start at a multiple of 16 tokens, so
 // that 16 keys of a tile share a block.
 struct PfTiles {
     uint32_t nst, lo, n;
@@ -330,6 +330,53 @@ __device__ __forceinline__ bool pf_next_run(uint32_t& next, uint32_t nruns, cons
     return false;
 }
 
+// Block ids of a run's tiles for one loader warp of the f16 cache (kAlign): a lane holds one page of a stretch of CHUNK tiles, whose
+// pages fit a warp, and one of the stretch after it, requested when the first began.  With one tile of lookahead
+// every tile at an item's start waited for a table entry: 64 rows with a window of 1,024 took 35 us instead of 32, the wave
+// of 4,096 rows 86 instead of 79.  (The loaders of the 8-bit cache gained nothing from it.)
+struct PfPages {
+    static constexpr uint32_t CHUNK = 7;       // 7 * 64 tokens from a multiple of 16 on: at most 29 pages of >= 16 tokens
+    static constexpr uint32_t WINDOW = 1u << 20;  // stretches of the window part are numbered from here on
+    const uint32_t* trow;                      // the sequence's row of the block table
+    uint32_t last_page;
+    uint32_t chunk, page0, id, nchunk, npage0, nid;
+    __device__ __forceinline__ void open(const PagedMap& pm, uint32_t seq, uint32_t hi) {
+        trow = pm.block_tables + (size_t)seq * pm.max_blocks;
+        last_page = (hi - 1u) >> pm.lbs;
+        chunk = nchunk = 0xffffffffu;
+    }
+    __device__ __forceinline__ static uint32_t first_tile(const PfTiles& tl, uint32_t c) {
+        return c < WINDOW ? c * CHUNK : tl.nst + (c - WINDOW) * CHUNK;
+    }
+    __device__ __forceinline__ uint32_t request(const PagedMap& pm, const PfTiles& tl, uint32_t c, uint32_t& p0) const {
+        p0 = tl.first_key(first_tile(tl, c)) >> pm.lbs;
+        const uint32_t pg = p0 + (threadIdx.x & 31u);
+        return pg <= last_page ? __ldg(trow + pg) : 0u;
+    }
+    // makes `tile` (of a run whose tiles end at tile1) the current one
+    __device__ __forceinline__ void seek(const PagedMap& pm, const PfTiles& tl, uint32_t tile, uint32_t tile1, uint32_t* status) {
+        const uint32_t c = tile < tl.nst ? tile / CHUNK : WINDOW + (tile - tl.nst) / CHUNK;
+        if (c == chunk) return;
+        if (c == nchunk) {
+            id = nid;
+            page0 = npage0;
+        } else {
+            id = request(pm, tl, c, page0);
+        }
+        if (id >= pm.num_blocks) {
+            atomicOr(status, DEV_BAD_BLOCK);
+            id = 0u;
+        }
+        chunk = c;
+        nchunk = c < WINDOW && (c + 1u) * CHUNK >= tl.nst ? WINDOW : c + 1u;
+        if (first_tile(tl, nchunk) < tile1) nid = request(pm, tl, nchunk, npage0);
+        else nchunk = 0xffffffffu;
+    }
+    __device__ __forceinline__ uint32_t block(const PagedMap& pm, uint32_t token) const {
+        return __shfl_sync(0xffffffffu, id, ((token >> pm.lbs) - page0) & 31u);
+    }
+};
+
 // kFault (test support only) compiles in the hooks of oxi_debug_arm_wait_fault: a wait limit taken from the
 // launch, a K tile of CTA 0 that is never published, and the propagation of a give-up to the roles whose own
 // waits passed (the MMA warps withhold "O is final", the CTA claims nothing more).  The production
@@ -361,7 +408,8 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
     constexpr uint32_t kCodes = kFmt == PF_INT8 ? Q8_INT8 : Q8_E4M3;
     constexpr int ROWB = kQ8 ? Q8_ROW_BYTES : KV_ROW_BYTES;
     static_assert(!kQ8 || (kPaged && kSinks && !kTma && !kFault), "variants of the 8-bit cache");
-    auto tiles_of = [&](const PfRun& r) { return pf_tiles<kSinks, kQ8>(r.lo, r.hi, view.sinks); };
+    constexpr bool kAlign = kSinks && kPaged;  // tiles start at a multiple of 16 tokens: 16 keys of a tile lie in one block
+    auto tiles_of = [&](const PfRun& r) { return pf_tiles<kSinks, kAlign>(r.lo, r.hi, view.sinks); };
     const uint32_t wait_us = kFault ? fault.limit_us : WAIT_LIMIT_US;
     // paged K/V: k_ptrs / v_ptrs are unused, wave row r reads row row_seq[r] of pm.block_tables
     constexpr bool paged = kPaged;
@@ -1050,7 +1098,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             auto fetch_pages = [&](uint32_t kb) -> uint32_t {
                 const uint32_t pg = (kb >> pm.lbs) + (uint32_t)lane;
                 uint32_t id = 0;
-                if (lane < 8 && pg <= last_page) {
+                if (!kAlign && lane < 8 && pg <= last_page) {
                     id = __ldg(trow + pg);
                     if (id >= pm.num_blocks) {
                         atomicOr(status, DEV_BAD_BLOCK);
@@ -1066,6 +1114,8 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                 tflat += ntiles;
             }
             uint32_t pg_next = (paged && tile0 < tile1) ? fetch_pages(tl.first_key(tile0)) : 0u;
+            PfPages pages;
+            if (kAlign) pages.open(pm, (uint32_t)((c_kp[run.r0] >> 4) - 1ull), run.hi);
             // Rows of a registered slab (at a whole number of 1024-byte rows from its base) come through the
             // TMA unit: two boxes per full tile, written in the same swizzled layout, completion counted on
             // the stage's barrier.  The run's ragged last tile keeps the zero-filling copies below.
@@ -1100,7 +1150,25 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                 }
                 const uint32_t dst = ring + st * KV_TILE + (c >> 3) * KV_SUB;
                 const char* src = base + (size_t)(kbeg + r0) * KV_ROW_BYTES + c * 16;
-                if (paged) {
+                if (kAlign) {
+                    // one table entry for 16 rows (a lookup for every row, as below, made this loader the bottleneck:
+                    // 1.55 us a tile against 1.05 from pointer tables)
+                    pages.seek(pm, tl, tile, tile1, status);
+                    const uint32_t mask = (1u << pm.lbs) - 1u;
+                    const bool all = kbeg + TK <= run.hi && (kbeg >= run.lo || kbeg + TK <= view.sinks);
+#pragma unroll
+                    for (int b = 0; b < 4; b++) {
+                        const uint32_t t = kbeg + 16 * b;
+                        const uint32_t pid = pages.block(pm, t);
+                        const char* g = base + (size_t)pid * pm.block_stride + (size_t)((t & mask) + r0) * KV_ROW_BYTES + c * 16;
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            const uint32_t row = 16 * b + r0 + 2 * k;
+                            const bool valid = all || seen(kbeg + row);
+                            cp_async_16(dst + row * ROW_B + (((c & 7u) ^ (row & 7u)) << 4), valid ? g + k * 2 * KV_ROW_BYTES : base, valid);
+                        }
+                    }
+                } else if (paged) {
                     const uint32_t pg_cur = pg_next;
                     if (tile + 1 < tile1) pg_next = fetch_pages(tl.first_key(tile + 1));
                     const uint32_t p0 = kbeg >> pm.lbs, mask = (1u << pm.lbs) - 1u;
