@@ -260,6 +260,13 @@ struct RowView {
     uint32_t sinks, start, slen;
     template <uint32_t G>
     __device__ __forceinline__ uint32_t token(uint32_t v) const { return (v < gs ? v : v - gs + gw) * G; }
+    // Key ranges of `per` groups each; up to one and a half ranges stay one, so that a window of one range plus a few sinks
+    // does not need the merge (8 rows, window 256, 5 sinks: 13.2 -> 12.5 us; joining rests behind more ranges made a batch of
+    // 48 rows with a window of 1,024 slower, 16.7 -> 18.5 us).
+    __device__ __forceinline__ uint32_t ranges(uint32_t per) const { return ng <= per + per / 2u ? 1u : (ng + per - 1u) / per; }
+    __device__ __forceinline__ uint32_t range_end(uint32_t c, uint32_t per) const {
+        return ng <= per + per / 2u ? ng : min(ng, (c + 1u) * per);
+    }
     // bit i: token t0 + i is visible (i < G <= 16)
     template <uint32_t G>
     __device__ __forceinline__ uint32_t visible_bits(uint32_t t0) const {

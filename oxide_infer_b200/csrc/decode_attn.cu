@@ -142,10 +142,8 @@ __device__ __forceinline__ uint32_t row_chunks(uint32_t slen, uint32_t window) {
     const uint32_t eff = slen - window_start(slen, window);
     return (eff + dec::CHUNK - 1) / dec::CHUNK;
 }
-// with sinks a row's keys are the groups of its view, in order: CHUNK / GK groups make a work item
-__device__ __forceinline__ uint32_t view_chunks(const RowView& rv) {
-    return (rv.ng + dec::CHUNK / dec::GK - 1) / (dec::CHUNK / dec::GK);
-}
+// with sinks a row's keys are the groups of its view, in order: CHUNK / GK groups make a work item (RowView::ranges)
+__device__ __forceinline__ uint32_t view_chunks(const RowView& rv) { return rv.ranges(dec::CHUNK / dec::GK); }
 
 // largest b with prefix[b] <= item  (prefix[0] = 0, prefix[batch] = total)
 __device__ __forceinline__ uint32_t find_row(const uint32_t* prefix, uint32_t batch, uint32_t item) {
@@ -242,13 +240,13 @@ decode_attn_kernel(const DecodeParams p) {
         // pages), fetched one item ahead like the row pointers
         uint32_t cpg = 0, cfp = 0;
         // kSinks: lanes 0 .. npa-1 hold the pages of the item's sink groups from page `first_page` on, the lanes
-        // behind them those of its window groups from page `first_page_w` on (CHUNK / 16 + 2 pages at most)
+        // behind them those of its window groups from page `first_page_w` on (3 / 2 CHUNK / 16 + 2 pages at most)
         uint32_t cfw = 0, cna = 0;
         auto fetch_pages = [&](uint32_t b, uint32_t c, uint32_t slen, uint32_t& first_page, uint32_t& first_page_w,
                                uint32_t& npa) -> uint32_t {
             if (kSinks) {
                 const RowView rv = row_view<GK>(slen, p.window, p.sinks);
-                const uint32_t v0 = c * (CHUNK / GK), v1 = min(v0 + (uint32_t)(CHUNK / GK), rv.ng);
+                const uint32_t v0 = c * (CHUNK / GK), v1 = rv.range_end(c, CHUNK / GK);
                 first_page = (v0 * GK) >> p.paged.lbs;
                 npa = v0 < rv.gs ? (((min(v1, rv.gs) - 1u) * GK) >> p.paged.lbs) - first_page + 1u : 0u;
                 const uint32_t vw = max(v0, rv.gs);
@@ -321,7 +319,7 @@ decode_attn_kernel(const DecodeParams p) {
             // kSinks: virtual positions; the last group of the view ends with the row's last key
             const uint32_t vend = rv.ng * GK - ((0u - cslen) & (uint32_t)(GK - 1));
             const uint32_t t0 = kSinks ? cc * CHUNK : window_start(cslen, p.window) + cc * CHUNK;
-            const uint32_t t1 = min(t0 + (uint32_t)CHUNK, kSinks ? vend : cslen);
+            const uint32_t t1 = kSinks ? (last_range ? vend : t0 + CHUNK) : min(t0 + (uint32_t)CHUNK, cslen);
             // the lane that holds the page of token `tok` of virtual group v
             auto page_lane = [&](uint32_t v, uint32_t tok) -> uint32_t {
                 return v < rv.gs ? (tok >> p.paged.lbs) - cfp : cna + (tok >> p.paged.lbs) - cfw;
@@ -696,7 +694,7 @@ decode_merge_kernel(const DecodeParams p) {
     if (slen == 0u || slen > p.max_seq_len || (kvp & 15ull) != 0ull) return;
     if (p.paged.block_tables && ((slen - 1u) >> p.paged.lbs) >= p.paged.max_blocks) return;
     const uint32_t nchunks = kRule == MERGE_SINKS ? view_chunks(row_view<dec::GK>(slen, p.window, p.sinks))
-                             : kRule == MERGE_Q8  ? (row_view<16>(slen, p.window, p.sinks).ng + dec::CHUNK / 16 - 1) / (dec::CHUNK / 16)
+                             : kRule == MERGE_Q8  ? row_view<16>(slen, p.window, p.sinks).ranges(dec::CHUNK / 16)
                                                   : row_chunks(slen, p.window);
     if (nchunks <= 1) return;
     const uint32_t nslices = kSliced ? (nchunks + MERGE_BLK - 1) / MERGE_BLK : 1u;

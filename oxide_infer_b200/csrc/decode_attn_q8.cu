@@ -51,7 +51,7 @@ constexpr int DESC_OFF = Q_OFF + Q_BYTES;         // 48 bytes: row / range / fla
 constexpr int STAGE_BYTES = DESC_OFF + 64;
 constexpr int CHUNK = 256;                        // keys per work item (the merge's key ranges)
 constexpr uint32_t CHUNK_G = CHUNK / GK;
-constexpr int PAGES = 20;                         // pages of an item: at most CHUNK / 16 + 2
+constexpr int PAGES = 28;                         // pages of an item: at most 3 / 2 CHUNK / 16 + 2
 constexpr int NTABLE = 4;                         // items whose scales are in shared memory
 constexpr int TABLE_BYTES = PAGES * 32;           // per page: 4 K scales, 4 V scales
 constexpr int N_CONSUMER_WARPS = NKV;
@@ -127,7 +127,7 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
         if (slen == 0u || slen > p.ws.max_seq_len || ((slen - 1u) >> p.map.lbs) >= p.map.max_blocks) {
             if (blockIdx.x == 0) atomicOr(status, DEV_BAD_SEQ_LEN);
         } else {
-            n = (row_view<GK>(slen, p.window, p.sinks).ng + CHUNK_G - 1u) / CHUNK_G;
+            n = row_view<GK>(slen, p.window, p.sinks).ranges(CHUNK_G);
         }
         prefix[b + 1] = n;
         s_len[b] = slen;
@@ -175,7 +175,7 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
             it.range = item - prefix[lo];
             it.slen = s_len[lo];
             const RowView rv = row_view<GK>(it.slen, p.window, p.sinks);
-            const uint32_t v0 = it.range * CHUNK_G, v1 = min(v0 + CHUNK_G, rv.ng), vw = max(v0, rv.gs);
+            const uint32_t v0 = it.range * CHUNK_G, v1 = rv.range_end(it.range, CHUNK_G), vw = max(v0, rv.gs);
             it.pa = (v0 * GK) >> lbs;
             it.npa = v0 < rv.gs ? (((min(v1, rv.gs) - 1u) * GK) >> lbs) - it.pa + 1u : 0u;
             it.pw = rv.token<GK>(vw) >> lbs;
@@ -212,7 +212,7 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
             // preceding kernel drains (what it may still write there is read after the wait, and L2 has it then)
             c = open_item(cur);
             const RowView rv = row_view<GK>(c.slen, p.window, p.sinks);
-            const uint32_t v = c.range * CHUNK_G + (lane & 15u), v1 = min((c.range + 1u) * CHUNK_G, rv.ng);
+            const uint32_t v = c.range * CHUNK_G + (lane & 15u), v1 = rv.range_end(c.range, CHUNK_G);
             const uint32_t tok = v < v1 ? rv.token<GK>(v) : 0u;
             const uint32_t ps = v >= v1 ? 0u : v < rv.gs ? (tok >> lbs) - c.pa : c.npa + (tok >> lbs) - c.pw;
             const uint32_t id = __shfl_sync(0xffffffffu, c.id, ps & 31u);
@@ -242,7 +242,7 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
             }
             const uint32_t nchunks = prefix[c.row + 1] - prefix[c.row];
             const RowView rv = row_view<GK>(c.slen, p.window, p.sinks);
-            const uint32_t v0 = c.range * CHUNK_G, v1 = min(v0 + CHUNK_G, rv.ng);
+            const uint32_t v0 = c.range * CHUNK_G, v1 = rv.range_end(c.range, CHUNK_G);
             unsigned char* table = tables + (nitem % NTABLE) * TABLE_BYTES;
             for (uint32_t v = v0; v < v1; v += NGROUP, ++fill) {
                 // Whatever does not need the slot comes before the wait for it: a slot's refill starts when its last

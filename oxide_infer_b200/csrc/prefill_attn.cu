@@ -1383,11 +1383,12 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
     // an armed test fault runs the plain instantiation: pointer tables, unsplit, per-thread copies
     const bool armed = flt.skip_plus1 != 0u && !pm && !sinks;
     bool split = !armed && ws && ws->max_slots != 0u && part_keys != 0u && nblocks * NKV < (uint32_t)num_sms;
-    // with sinks or the 8-bit cache: a window so short that a block's run has no more tiles than the smallest part is not
-    // split (the merge costs 2.5 us: 64 rows, window 64: 16.1 against 18.6 us; window 512 24.9 / 24.7, 1,024 34.3 / 26.7), ...
+    // with sinks or the 8-bit cache: a window so short that two runs in a block have no more tiles than the smallest part is
+    // not split (the merge costs 2.5 us: 64 rows, window 64: 16.1 against 18.6 us; window 512 24.9 / 24.7, 1,024 34.3 / 26.7;
+    // blocks of up to three runs with a window of 100 and 70 sinks: 36.8 against 30.3), ...
     const bool view_variant = sinks || q8;
     if (view_variant && window && window <= (1u << 22) &&
-        (window + pf::BLK - 1u + 15u + pf::TK - 1u) / pf::TK + (sinks < window ? (sinks + pf::TK - 1u) / pf::TK : (window + pf::TK - 1u) / pf::TK) <=
+        2u * ((window + pf::BLK - 1u + 15u + pf::TK - 1u) / pf::TK + ((sinks < (1u << 22) ? sinks : 1u << 22) + pf::TK - 1u) / pf::TK) <=
             (part_keys + pf::TK - 1u) / pf::TK)
         split = false;
     // ... and a wave of at most one item per SM needs no order: no plan kernel

@@ -1,0 +1,116 @@
+"""Support paths of the 8-bit cache and sink kernels: a wait that runs out on purpose, and the tests of both against the
+bounds-checking build."""
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+from tests import q8case as Q
+
+pytestmark = pytest.mark.gpu
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+WAIT_TIMEOUT = 4
+
+
+@pytest.mark.parametrize("stage", [0, 1, 3])
+def test_q8_decode_wait_runs_out_and_the_handle_recovers(stage):
+    """CTA 0 withholds one stage of its first item: the call returns in milliseconds and says so, rows that CTA 0 did not
+    own are right, the next call is right altogether."""
+    from oxide_infer_b200 import KvPath
+    kv = KvPath(0, max_batch=8, max_seq_len=8192, max_prefill_rows=0)
+    lens = [2000, 300, 4095, 64, 700]
+    c = Q.Q8Cache(lens, "int8", 16, seed=60)
+    q, g = Q.activations(len(lens), 61)
+    call = lambda ctx: kv.decode_attn_q8(ctx, q, g, c.layout(), Q.i32(lens))  # noqa: E731
+    good, hit, again = (torch.zeros(len(lens), 16, 128, dtype=torch.float16, device="cuda") for _ in range(3))
+    call(good)
+    assert kv.device_status() == 0
+    kv.arm_wait_fault(0, stage, 1000)
+    t0, t1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    t0.record()
+    call(hit)
+    t1.record()
+    torch.cuda.synchronize()
+    assert t0.elapsed_time(t1) < 500.0
+    assert kv.device_status() == WAIT_TIMEOUT
+    for i in range(1, len(lens)):
+        assert torch.equal(hit[i].view(torch.int16), good[i].view(torch.int16)), i
+    call(again)
+    assert kv.device_status() == 0
+    assert torch.equal(again.view(torch.int16), good.view(torch.int16))
+
+
+def test_q8_and_sink_tests_are_clean_under_the_bounds_build():
+    if os.environ.get("OXI_KV_LIB"):
+        pytest.skip("already running against a substituted library")
+    from oxide_infer_b200 import build
+    env = dict(os.environ, OXI_KV_LIB=build.build(bounds=True))
+    subset = "append or fused or together or generated or skips or bad or ragged or prefix or 16-300 or 0-300 or batch"
+    r = subprocess.run([sys.executable, "-m", "pytest", "-q", "-x", "-m", "gpu", "-k", subset, "tests/test_gpu_q8.py",
+                        "tests/test_gpu_sinks.py"], cwd=ROOT, env=env, capture_output=True, text=True, timeout=900)
+    tail = (r.stdout + r.stderr)[-3000:]
+    assert r.returncode == 0 and " passed" in r.stdout and "failed" not in r.stdout, tail
+
+
+@pytest.mark.parametrize("window,sinks", [(256, 4), (512, 16), (1024, 1), (375, 5), (376, 16), (640, 100)])
+def test_windows_around_whole_key_ranges(window, sinks):
+    """Up to one and a half key ranges stay one: 1 to 5 ranges, f16 and 8-bit, lengths around every border."""
+    from oxide_infer_b200 import KvPath
+    from tests.test_gpu_sinks import F16Cache
+    lens = [window + sinks + d for d in (-130, -17, -1, 0, 1, 15, 16, 127, 128, 129, 300)]
+    kv = KvPath(0, max_batch=len(lens), max_seq_len=4096, max_prefill_rows=0)
+    q, g = Q.activations(len(lens), 62)
+    rows = [(i, i, Q.visible(n, window, sinks)) for i, n in enumerate(lens)]
+    for fmt, bs in (("int8", 16), ("e4m3", 128)):
+        c = Q.Q8Cache(lens, fmt, bs, seed=63)
+        ctx = torch.zeros(len(lens), 16, 128, dtype=torch.float16, device="cuda")
+        kv.decode_attn_q8(ctx, q, g, c.layout(), Q.i32(lens), window=window, sinks=sinks)
+        Q.check_rows(ctx, q, g, rows, c.values)
+    for bs in (0, 16):
+        c = F16Cache(lens, bs, seed=64)
+        ctx = torch.zeros(len(lens), 16, 128, dtype=torch.float16, device="cuda")
+        c.decode(kv, ctx, q, g, lens, window, sinks)
+        Q.check_rows(ctx, q, g, rows, c.values)
+    assert kv.device_status() == 0
+
+
+def test_two_graphs_of_one_handle_and_shared_tail_blocks():
+    """Two captured graphs of different layers share a handle's workspace on one stream; replayed in turn each keeps its result."""
+    from oxide_infer_b200 import KvPath
+    kv = KvPath(0, max_batch=16, max_seq_len=8192, max_prefill_rows=256)
+    stream = torch.cuda.Stream()
+    lens = [3000, 700, 41]
+    caches = [Q.Q8Cache(lens, fmt, 16, seed=65 + i) for i, fmt in enumerate(("int8", "e4m3"))]
+    q, g = Q.activations(3, 67)
+    row_seq, pos = Q.wave([(0, 2900, 100), (1, 650, 50)])
+    qp, gp = Q.activations(len(pos), 68)
+    layouts, lens_d, rs, pl = [c.layout() for c in caches], Q.i32(lens), Q.i32(row_seq), Q.i32(pos + 1)
+    outs = [(torch.zeros_like(q), torch.zeros_like(qp)) for _ in caches]
+    torch.cuda.synchronize()
+    graphs = []
+    with torch.cuda.stream(stream):
+        for lay, (o, op) in zip(layouts, outs):
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr, stream=stream):
+                kv.decode_attn_q8(o, q, g, lay, lens_d, window=900, sinks=4)
+                kv.prefill_attn_q8(op, qp, gp, lay, rs, pl)
+            graphs.append(gr)
+        first = None
+        for _ in range(3):
+            for o, op in outs:
+                o.fill_(7.0)
+                op.fill_(7.0)
+            for gr in graphs:
+                gr.replay()
+            stream.synchronize()
+            now = [t.clone() for pair in outs for t in pair]
+            assert first is None or all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(first, now))
+            first = now
+    for c, (o, op) in zip(caches, outs):
+        Q.check_rows(o, q, g, [(i, i, Q.visible(n, 900, 4)) for i, n in enumerate(lens)], c.values)
+        Q.check_rows(op, qp, gp, [(r, row_seq[r], np.arange(pos[r] + 1)) for r in range(0, len(pos), 9)], c.values)
+    assert kv.device_status() == 0
