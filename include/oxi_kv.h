@@ -315,6 +315,7 @@ typedef struct oxi_paged_q8_layout {
     uint32_t block_size;           /* tokens per block: 16, 32, 64, 128 or 256 */
     uint32_t num_blocks;
     uint32_t format;               /* OXI_Q8_INT8 or OXI_Q8_E4M3 */
+    uint32_t table_rows;           /* rows of block_tables */
 } oxi_paged_q8_layout;
 
 /* Per-head Q/K RMSNorm + RoPE and the quantising append of k and v, for decode rows and prefill waves.
@@ -328,9 +329,12 @@ typedef struct oxi_paged_q8_layout {
  * change rounds them once more).  A token at slot 0 starts its block afresh.  Slots behind the run keep
  * their codes.  Two separate runs of one call must not fall into one block (OXI_DEV_BLOCK_CONFLICT, k / v of
  * both skipped; with row_seq NULL every row is its own sequence), and table rows of one call must not share
- * a block that is written.  A position >= max_seq_len or beyond max_blocks sets OXI_DEV_BAD_SEQ_LEN and the
- * row is skipped, a block id >= num_blocks sets OXI_DEV_BAD_BLOCK and k / v are not written.  A row that is
- * skipped ends a run.  16-byte alignment of all tensors.  rows <= max(max_batch, max_prefill_rows). */
+ * a block that is written.  A position >= max_seq_len or beyond max_blocks, or a row_seq >= table_rows, sets
+ * OXI_DEV_BAD_SEQ_LEN and the row is skipped, a block id >= num_blocks sets OXI_DEV_BAD_BLOCK and k / v are not
+ * written.  A row that is skipped ends a run.  cos / sin cover the positions of all other rows.  16-byte
+ * alignment of all tensors.  rows <= max(max_batch, max_prefill_rows); with row_seq NULL rows <= table_rows.
+ * pos_ids, row_seq, seq_lens and block_tables are inputs of the step for this and the next two entry points: they
+ * are complete before the kernel that precedes the call in its stream begins (as k_ptrs elsewhere). */
 int32_t oxi_append_q8(oxi_handle* h, void* stream, void* q_out, const void* q_in, const void* k_in, const void* v_in,
                       const void* q_norm_w, const void* k_norm_w, const void* cos_table, const void* sin_table,
                       const uint32_t* pos_ids, const oxi_paged_q8_layout* layout, const uint32_t* row_seq, uint32_t rows,
@@ -342,13 +346,14 @@ int32_t oxi_append_q8(oxi_handle* h, void* stream, void* q_out, const void* q_in
  * the products exactly, the gated result is rounded once.  Codes and scales of visible tokens must be finite;
  * what invisible slots hold does not matter.  Rows with a length of 0, above max_seq_len or beyond max_blocks
  * set OXI_DEV_BAD_SEQ_LEN and keep their ctx_out; a block id >= num_blocks sets OXI_DEV_BAD_BLOCK and block 0
- * is read instead.  A row's result does not depend on the rest of the batch. */
+ * is read instead.  A row's result does not depend on the rest of the batch.  batch <= table_rows. */
 int32_t oxi_decode_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
                            const oxi_paged_q8_layout* layout, const uint32_t* seq_lens, uint32_t batch, uint32_t window,
                            uint32_t sinks);
 
 /* The same for the rows of a prefill wave: row r attends the tokens of table row row_seq[r] that are visible
- * from position seq_lens[r] - 1.  All rows' k / v were appended before (oxi_append_q8). */
+ * from position seq_lens[r] - 1 (row_seq >= table_rows: as a bad length).  All rows' k / v were appended before
+ * (oxi_append_q8).  Codes and scales are finite for every token that some row of a 64-row block sees. */
 int32_t oxi_prefill_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
                             const oxi_paged_q8_layout* layout, const uint32_t* row_seq, const uint32_t* seq_lens,
                             uint32_t rows, uint32_t window, uint32_t sinks);
@@ -357,7 +362,8 @@ int32_t oxi_prefill_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const vo
 /* The attention entry points above with the first `sinks` tokens of a sequence staying visible behind its
  * window: row b attends t < seq_lens[b] with t >= seq_lens[b] - window or t < sinks.  Keys keep the rotation of
  * their own positions.  Arguments otherwise as the entry point without `_sinks`, whose bytes they return when
- * window or sinks is 0; else the gated result is rounded once instead of before and after the gate. */
+ * window or sinks is 0; else the gated result is rounded once instead of before and after the gate, and rows
+ * of prefill waves longer than max_seq_len are skipped (OXI_DEV_BAD_SEQ_LEN).  What no row sees may hold anything. */
 int32_t oxi_decode_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
                               const uint64_t* k_ptrs, const uint64_t* v_ptrs, const uint32_t* seq_lens, uint32_t batch,
                               uint32_t window, uint32_t sinks);

@@ -259,7 +259,8 @@ append_q8_wave_kernel(const AppendQ8Params p) {
     pdl_launch_dependents();
     // this warp's row, read by every warp itself: its rotary values are then on their way before the window is sorted out
     const uint32_t my_pos = row0 + w < p.rows ? p.pos_ids[row0 + w] : 0xffffffffu;
-    const bool there = my_pos < p.max_seq_len && (my_pos >> lbs) < p.map.max_blocks;  // a row that is skipped is not read either
+    const uint32_t my_seq = row0 + w < p.rows ? p.row_seq[row0 + w] : 0xffffffffu;
+    const bool there = my_pos < p.max_seq_len && (my_pos >> lbs) < p.map.max_blocks && my_seq < p.map.table_rows;  // a row that is skipped is not read either
     const uint32_t pos = there ? my_pos : 0u;
     const Dims cv = dims_of(p.cos_t + (size_t)pos * HD, j), sv = dims_of(p.sin_t + (size_t)pos * HD, j);
     const size_t row = there ? row0 + w : 0u;
@@ -297,7 +298,7 @@ append_q8_wave_kernel(const AppendQ8Params p) {
                 pseq = p.row_seq[r - 1u];
             }
         }
-        const bool valid = there && pos < p.max_seq_len && (pos >> lbs) < p.map.max_blocks;
+        const bool valid = there && pos < p.max_seq_len && (pos >> lbs) < p.map.max_blocks && seq < p.map.table_rows;
         if (there && !valid && blockIdx.y == 0) atomicOr(p.status, DEV_BAD_SEQ_LEN);
         const bool leader = valid && ((pos & (bs - 1u)) == 0u || r == 0u || pseq != seq || ppos + 1u != pos);
         const uint32_t leaders = __ballot_sync(0xffffffffu, leader), valids = __ballot_sync(0xffffffffu, valid);

@@ -69,6 +69,7 @@ struct Q8Map {
     uint32_t max_blocks;
     uint32_t lbs;                  // log2(block size in tokens), 4 ... 8
     uint32_t num_blocks;
+    uint32_t table_rows;           // rows of block_tables
 };
 constexpr uint32_t Q8_INT8 = 0, Q8_E4M3 = 1;
 

@@ -502,7 +502,8 @@ static int32_t paged_q8_map(const oxi_paged_q8_layout* l, const char* who, Q8Map
     while ((1u << lbs) < l->block_size && lbs < 31) lbs++;
     if (l->block_size < 16 || l->block_size > 256 || (1u << lbs) != l->block_size)
         return fail(OXI_ERR_ARG, "paged q8 layout: block_size must be 16, 32, 64, 128 or 256 tokens");
-    if (l->max_blocks == 0 || l->num_blocks == 0) return fail(OXI_ERR_ARG, "paged q8 layout: max_blocks and num_blocks must be positive");
+    if (l->max_blocks == 0 || l->num_blocks == 0 || l->table_rows == 0)
+        return fail(OXI_ERR_ARG, "paged q8 layout: max_blocks, num_blocks and table_rows must be positive");
     if ((l->block_stride_bytes & 15ull) != 0ull || l->block_stride_bytes < (uint64_t)l->block_size * Q8_ROW_BYTES)
         return fail(OXI_ERR_ARG, "paged q8 layout: block_stride_bytes must be a multiple of 16 and hold block_size rows of 512 bytes");
     if ((l->scale_stride & 3ull) != 0ull || l->scale_stride < (uint64_t)NKV)
@@ -520,6 +521,7 @@ static int32_t paged_q8_map(const oxi_paged_q8_layout* l, const char* who, Q8Map
     m->max_blocks = l->max_blocks;
     m->lbs = lbs;
     m->num_blocks = l->num_blocks;
+    m->table_rows = l->table_rows;
     return OXI_OK;
 }
 // Launches go to the calling thread's current device: another one than the handle's is refused (its stream would be
@@ -546,6 +548,7 @@ int32_t oxi_append_q8(oxi_handle* h, void* stream, void* q_out, const void* q_in
                     (uintptr_t)cos_table | (uintptr_t)sin_table, "oxi_append_q8");
     Q8Map m;
     if (int32_t rc = paged_q8_map(layout, "oxi_append_q8: the layout or one of its pointers is null", &m)) return rc;
+    if (!row_seq) REQ_BATCH(rows, m.table_rows, "oxi_append_q8");
     OXI_CUDA(launch_append_q8((cudaStream_t)stream, q_out, q_in, k_in, v_in, q_norm_w, k_norm_w, cos_table, sin_table, pos_ids,
                               row_seq, m, layout->format, rows, h->max_seq_len, eps, h->dws.status),
              "append_q8 launch");
@@ -562,6 +565,7 @@ int32_t oxi_decode_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const voi
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_decode_attn_q8");
     Q8Map m;
     if (int32_t rc = paged_q8_map(layout, "oxi_decode_attn_q8: the layout or one of its pointers is null", &m)) return rc;
+    REQ_BATCH(batch, m.table_rows, "oxi_decode_attn_q8");
     OXI_CUDA(launch_decode_attn_q8((cudaStream_t)stream, take_dws(h), ctx_out, q, gate, m, layout->format, seq_lens, batch, window,
                                    sinks),
              "decode_attn_q8 launch");

@@ -119,6 +119,7 @@ struct PfView {
     const float* k_scales; // 8-bit cache: block i's scales at + i * scale_stride
     const float* v_scales;
     uint64_t scale_stride;
+    uint32_t table_rows;   // 8-bit cache: rows of the block tables
 };
 // The 64-key tiles of a run whose rows' windows start at `wlo` or later and whose tokens end at hi: nst tiles of
 // sinks from token 0, then tiles from token lo on.  Tiles of paged caches start at a multiple of 16 tokens, so
@@ -512,7 +513,8 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                     // the run logic below only compares these two words: (table row + 1) * 16 keeps rows of one
                     // sequence equal, non-zero and "aligned"
                     kp[hf] = vp[hf] = ((uint64_t)row_seq[r] + 1ull) << 4;
-                    too_long = sl[hf] != 0u && ((sl[hf] - 1u) >> pm.lbs) >= pm.max_blocks;  // more blocks than the table has columns
+                    if (kQ8 && row_seq[r] >= view.table_rows) too_long = true;
+                    too_long |= sl[hf] != 0u && ((sl[hf] - 1u) >> pm.lbs) >= pm.max_blocks;  // more blocks than the table has columns
                 } else {
                     kp[hf] = k_ptrs[r];
                     vp[hf] = v_ptrs[r];
@@ -1371,7 +1373,7 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
                                 const PagedMap* pm, const uint32_t* row_seq, const PrefillSplitWs* ws,
                                 uint32_t part_keys, const PrefillSlab* slab, const WaitFault* fault, uint32_t sinks,
                                 uint32_t max_seq_len, const Q8Map* q8, uint32_t format) {
-    const PfView view{sinks, max_seq_len, q8 ? q8->k_scales : nullptr, q8 ? q8->v_scales : nullptr, q8 ? q8->scale_stride : 0};
+    const PfView view{sinks, max_seq_len, q8 ? q8->k_scales : nullptr, q8 ? q8->v_scales : nullptr, q8 ? q8->scale_stride : 0, q8 ? q8->table_rows : 0};
     PagedMap q8pm{};
     if (q8) {
         q8pm = PagedMap{q8->k_pool, q8->v_pool, q8->block_tables, q8->block_stride, q8->max_blocks, q8->lbs, q8->num_blocks};

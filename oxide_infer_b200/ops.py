@@ -42,7 +42,8 @@ class PagedQ8Layout(C.Structure):
     INT8, E4M3 = 0, 1
     _fields_ = [("k_pool", C.c_void_p), ("v_pool", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
                 ("block_tables", C.c_void_p), ("block_stride_bytes", C.c_uint64), ("scale_stride", C.c_uint64),
-                ("max_blocks", C.c_uint32), ("block_size", C.c_uint32), ("num_blocks", C.c_uint32), ("format", C.c_uint32)]
+                ("max_blocks", C.c_uint32), ("block_size", C.c_uint32), ("num_blocks", C.c_uint32), ("format", C.c_uint32),
+                ("table_rows", C.c_uint32)]
 
     @classmethod
     def of(cls, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
@@ -64,7 +65,7 @@ class PagedQ8Layout(C.Structure):
             raise ValueError("block_tables must be contiguous int32 [batch][max_blocks]")
         tensors = (k_pool, v_pool, k_scales, v_scales, block_tables)
         out = cls(*[t.data_ptr() for t in tensors], k_pool.stride(0), k_scales.stride(0), block_tables.shape[1],
-                  k_pool.shape[1], k_pool.shape[0], formats[k_pool.dtype])
+                  k_pool.shape[1], k_pool.shape[0], formats[k_pool.dtype], block_tables.shape[0])
         out._keep = tensors
         return out
 

@@ -158,6 +158,22 @@ def test_append_refuses_rows_that_it_cannot_place(kv):
     assert bool((a.q_out[2] == 7.0).all())
 
 
+def test_rows_of_a_sequence_that_the_table_does_not_have(kv):
+    """row_seq beyond the table's rows: nothing of such a row is read or written, its neighbours are right."""
+    c = Q.Q8Cache([30, 30], "int8", 16, seed=16)
+    a = Append(c, [0, 0, 1, 1, 1], [28, 29, 28, 29, 30], seed=17)
+    for bad in (2, 2 ** 31, 2 ** 32 - 1):
+        a.row_seq = np.array([0, bad, bad, 1, 1])
+        a.run(kv, status=BAD_SEQ_LEN, skip_q=(1, 2), skip_kv=(1, 2))
+        assert bool((a.q_out[1:3] == 7.0).all())
+        q, g = Q.activations(5, 18)
+        ctx = guarded(np.full((5, Q.NQ, Q.HD), 7.0, np.float16), "ctx")
+        kv.prefill_attn_q8(ctx, q, g, c.layout(), Q.i32(a.row_seq), Q.i32([29, 30, 29, 30, 31]))
+        assert kv.device_status() == BAD_SEQ_LEN
+        assert bool((ctx[1:3] == 7.0).all())
+        Q.check_rows(ctx, q, g, [(0, 0, np.arange(29)), (3, 1, np.arange(30)), (4, 1, np.arange(31))], c.values)
+
+
 def test_append_refuses_two_runs_in_one_block(kv):
     """Rows 0-1 and 4-5 are two runs of sequence 0 in its first block; row 2-3 (sequence 1) and 6 (the next block) are fine."""
     c = Q.Q8Cache([30, 30], "e4m3", 16, seed=11)
@@ -245,7 +261,22 @@ def test_decode_attention_with_gaps_and_offsets_behind_32_bits(kv):
     kv.decode_attn_q8(ctx, q, g, PagedQ8Layout.of(*pools, *scales, tables), Q.i32([n]))
     t = torch.arange(n, device="cuda")
     b = tables[0].long()[t // bs]
-    Q.check_rows(ctx, q, g, [(0, 0, np.arange(n))], lambda s, tk: tuple(p[b, t % bs].double() * sc.double()[b][..., None] for p, sc in zip(pools, scales)))
+    def values(seq, tokens):
+        t = torch.as_tensor(tokens, device="cuda")
+        b = tables[0].long()[t // bs]
+        return tuple(p[b, t % bs].double() * sc.double()[b][..., None] for p, sc in zip(pools, scales))
+    Q.check_rows(ctx, q, g, [(0, 0, np.arange(n))], values)
+    # a chunk of 20 rows appended behind them, and its attention
+    lay, m = PagedQ8Layout.of(*pools, *scales, tables), 20
+    half = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float16)).cuda()  # noqa: E731
+    q, k, v, gate, w = half(m, 16, 128), half(m, 4, 128), half(m, 4, 128), half(m, 16), torch.ones(128, dtype=torch.float16, device="cuda")
+    cos, sin = torch.ones(128, 128, dtype=torch.float16, device="cuda"), torch.zeros(128, 128, dtype=torch.float16, device="cuda")
+    pos, rs, ctx = Q.i32(np.arange(n, n + m)), Q.i32(np.zeros(m)), torch.zeros(m, 16, 128, dtype=torch.float16, device="cuda")
+    kv.append_q8(q, q, k, v, w, w, cos, sin, pos, lay, row_seq=rs)
+    got = values(0, np.arange(n, n + m))[1]
+    assert float((got - v.double()).abs().max()) <= float(v.double().abs().max()) / 250
+    kv.prefill_attn_q8(ctx, q, gate, lay, rs, pos + 1)
+    Q.check_rows(ctx, q, gate, [(r, 0, np.arange(n + r + 1)) for r in range(m)], values)
     assert kv.device_status() == 0
 
 
@@ -284,7 +315,7 @@ def test_decode_attention_of_a_row_does_not_depend_on_the_batch(kv, window, sink
     for i, n in enumerate(lens):
         ctx = torch.zeros(1, 16, 128, dtype=torch.float16, device="cuda")
         lay = c.layout()
-        lay.block_tables = c.dtables[i:i + 1].data_ptr()
+        lay.block_tables, lay.table_rows = c.dtables[i:i + 1].data_ptr(), 1
         other.decode_attn_q8(ctx, q[i:i + 1].contiguous(), g[i:i + 1].contiguous(), lay, Q.i32([n]), window=window, sinks=sinks)
         assert torch.equal(ctx[0].view(torch.int16), full[i].view(torch.int16)), n
     assert kv.device_status() == 0 and other.device_status() == 0
@@ -489,12 +520,13 @@ def test_refusals(kv):
     dec = lambda lay, **kw: kv.decode_attn_q8(ctx, q, g, lay, sl, **kw)  # noqa: E731
     for kw in (dict(k_pool=None), dict(v_scales=None), dict(block_tables=None)):
         assert code(lambda: dec(broken(**kw))) == -1
-    for kw in (dict(block_size=8), dict(block_size=24), dict(block_size=512), dict(max_blocks=0), dict(num_blocks=0),
+    for kw in (dict(table_rows=0), dict(block_size=8), dict(block_size=24), dict(block_size=512), dict(max_blocks=0), dict(num_blocks=0),
                dict(block_stride_bytes=16 * 512 - 16), dict(block_stride_bytes=16 * 512 + 8), dict(scale_stride=2),
                dict(scale_stride=6), dict(format=2), dict(k_pool=c.kp.data_ptr() + 8), dict(k_scales=c.ks.data_ptr() + 4)):
         assert code(lambda: dec(broken(**kw))) == -3, kw
     assert code(lambda: dec(c.layout(), batch=0)) == -2
     assert code(lambda: dec(c.layout(), batch=65)) == -2
+    assert code(lambda: dec(c.layout(), batch=2)) == -2  # the table has one row
     assert code(lambda: kv.prefill_attn_q8(ctx, q, g, c.layout(), None, sl)) == -1
     assert code(lambda: kv.prefill_attn_q8(ctx, q, g, c.layout(), sl, sl, rows=1025)) == -2
     k = torch.zeros(1, 4, 128, dtype=torch.float16, device="cuda")
@@ -503,6 +535,7 @@ def test_refusals(kv):
     assert code(lambda: app(eps=-1.0)) == -3
     assert code(lambda: app(eps=float("nan"))) == -3
     assert code(lambda: app(rows=1025)) == -2
+    assert code(lambda: app(rows=2)) == -2
     odd = torch.zeros(2 * 16 * 128, dtype=torch.float16, device="cuda")[1:1 + 16 * 128].view(1, 16, 128)
     assert code(lambda: kv.decode_attn_q8(ctx, odd, g, c.layout(), sl)) == -3
     assert kv.device_status() == 0

@@ -33,12 +33,12 @@ def _parts(dtype=torch.int8):
 
 def test_layout_fields():
     from oxide_infer_b200 import PagedQ8Layout
-    assert C.sizeof(PagedQ8Layout) == 5 * 8 + 2 * 8 + 4 * 4
+    assert C.sizeof(PagedQ8Layout) == 5 * 8 + 2 * 8 + 5 * 4 + 4  # 4 bytes of padding
     p = _parts()
     lay = PagedQ8Layout.of(*p)
     assert (lay.k_pool, lay.v_scales, lay.block_tables) == (p[0].data_ptr(), p[3].data_ptr(), p[4].data_ptr())
     assert (lay.block_stride_bytes, lay.scale_stride) == (16 * 512, 4)
-    assert (lay.max_blocks, lay.block_size, lay.num_blocks, lay.format) == (3, 16, 5, 0)
+    assert (lay.max_blocks, lay.block_size, lay.num_blocks, lay.format, lay.table_rows) == (3, 16, 5, 0, 2)
     assert PagedQ8Layout.of(*_parts(torch.float8_e4m3fn)).format == 1
     wide = [torch.zeros(5, 2, 16, 4, 128, dtype=torch.int8) for _ in range(2)]
     lay = PagedQ8Layout.of(wide[0][:, 0], wide[1][:, 1], *_parts()[2:])
