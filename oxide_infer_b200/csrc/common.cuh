@@ -278,6 +278,11 @@ struct RowView {
         return (in_sinks | in_window) & in_row;
     }
 };
+// Whether every row's view fits one key range of `per` groups of G tokens (RowView::ranges), whatever its length.
+inline bool view_is_one_range(uint32_t window, uint32_t sinks, uint32_t per, uint32_t G) {
+    if (window == 0u || window > 4096u || sinks > 4096u) return false;
+    return (sinks + G - 1u) / G + (window + G - 1u) / G + 1u <= per + per / 2u;
+}
 template <uint32_t G>
 __device__ __forceinline__ RowView row_view(uint32_t slen, uint32_t window, uint32_t sinks) {
     RowView r;

@@ -122,6 +122,7 @@ struct DecodeParams {
     uint32_t batch;
     uint32_t window;
     uint32_t sinks;        // kSinks variants only
+    uint32_t direct;       // kSinks variants only: every row is one item, no merge follows: items in fixed order, no claims
     uint32_t max_chunks;
     uint32_t max_seq_len;
     // paged variant only: K/V rows live in fixed-size blocks of a pool, block_tables[b][i] is the
@@ -289,16 +290,17 @@ decode_attn_kernel(const DecodeParams p) {
             }
         }
         uint32_t claim = 0;
-        if (lane == 0 && cur < total_items) claim = atomicAdd(p.work_counter, 1u);
+        if (lane == 0 && cur < total_items && !(kSinks && p.direct)) claim = atomicAdd(p.work_counter, 1u);
 
         while (cur < total_items && ok) {
             uint32_t nxt = __shfl_sync(0xffffffffu, claim, 0);
+            if (kSinks && p.direct) nxt = cur;
             nxt = (nxt >= total_items) ? total_items : min(nxt + gridDim.x, total_items);
             uint32_t nb = 0, nc = 0, nslen = 0, npg = 0, nfp = 0, nfw = 0, nna = 0;
             uint64_t nkp = 0, nvp = 0;
             claim = 0xffffffffu;  // "no more items" unless a new claim is made
             if (nxt < total_items) {
-                if (lane == 0) claim = atomicAdd(p.work_counter, 1u);
+                if (lane == 0 && !(kSinks && p.direct)) claim = atomicAdd(p.work_counter, 1u);
                 nb = find_row(prefix, p.batch, nxt);
                 nc = nxt - prefix[nb];
                 nslen = s_len[nb];
@@ -885,9 +887,12 @@ static DecodeParams make_params(const DecodeWorkspace& ws, void* ctx_out, const 
 template <bool kFused, bool kPaged>
 static cudaError_t launch_decode(cudaStream_t stream, const DecodeWorkspace& ws, uint32_t sinks, DecodeParams p) {
     p.sinks = sinks;
+    // a window of at most one key range (a window of 256 and a few sinks): nothing to merge, one launch (8 rows, window
+    // 256, 5 sinks: 12.5 -> 11.5 us)
+    p.direct = sinks && view_is_one_range(p.window, sinks, dec::CHUNK / dec::GK, dec::GK);
     cudaError_t e = launch_pdl(sinks ? decode_attn_kernel<kFused, kPaged, true> : decode_attn_kernel<kFused, kPaged, false>,
                                dim3(ws.num_sms), dim3(dec::THREADS), dec::SMEM_BYTES, stream, p);
-    if (e != cudaSuccess) return e;
+    if (e != cudaSuccess || p.direct) return e;
     return sinks ? launch_merge<MERGE_SINKS>(stream, ws, p.batch, p) : launch_merge<MERGE_WINDOW>(stream, ws, p.batch, p);
 }
 

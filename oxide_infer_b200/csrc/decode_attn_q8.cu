@@ -73,6 +73,7 @@ struct DecodeQ8Params {
     const uint32_t* seq_lens;
     DecodeWorkspace ws;
     uint32_t batch, window, sinks;
+    uint32_t direct;  // every row is one item, no merge follows: items in fixed order, no claims
 };
 
 // mma.m16n8k16, free to be scheduled among independent ones
@@ -192,7 +193,7 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
         // leave stages empty: `c` is streamed now, the pages of `n` and `m` after it have been requested, and a claim
         // behind them is in flight.
         const uint32_t rounds = total_items / gridDim.x;
-        const uint32_t fixed = rounds <= 8u ? min(rounds, 4u) : rounds - 4u;  // rounds in fixed order
+        const uint32_t fixed = p.direct ? 0xffffffffu : rounds <= 8u ? min(rounds, 4u) : rounds - 4u;  // rounds in fixed order
         uint32_t asked = 0, claim = 0;  // items of this CTA so far, the claim in flight
         auto ask = [&]() {
             // in PTX: the compiler's warp-aggregated form of atomicAdd waits for the result at once
@@ -567,9 +568,10 @@ cudaError_t launch_decode_attn_q8(cudaStream_t stream, const DecodeWorkspace& ws
     p.batch = batch;
     p.window = window;
     p.sinks = sinks;
+    p.direct = view_is_one_range(window, sinks, dq::CHUNK_G, dq::GK) || ws.max_seq_len <= (uint32_t)dq::CHUNK;  // nothing to merge
     const cudaError_t e = launch_pdl(format == Q8_INT8 ? decode_attn_q8_kernel<Q8_INT8> : decode_attn_q8_kernel<Q8_E4M3>,
                                      dim3(ws.num_sms), dim3(dq::THREADS), dq::SMEM_BYTES, stream, p);
-    if (e != cudaSuccess) return e;
+    if (e != cudaSuccess || p.direct) return e;
     return launch_decode_merge_q8(stream, ws, ctx_out, gate, map, seq_lens, batch, window, sinks);
 }
 

@@ -114,3 +114,29 @@ def test_two_graphs_of_one_handle_and_shared_tail_blocks():
         Q.check_rows(o, q, g, [(i, i, Q.visible(n, 900, 4)) for i, n in enumerate(lens)], c.values)
         Q.check_rows(op, qp, gp, [(r, row_seq[r], np.arange(pos[r] + 1)) for r in range(0, len(pos), 9)], c.values)
     assert kv.device_status() == 0
+
+
+def test_short_windows_take_one_launch_and_leave_the_handle_as_it_was():
+    """Windows of one key range run without the merge; calls that claim work and merge, in between, are not disturbed."""
+    from oxide_infer_b200 import KvPath
+    from tests.test_gpu_sinks import F16Cache
+    rng = np.random.default_rng(69)
+    lens = [int(n) for n in rng.integers(1, 2500, 400)]
+    kv = KvPath(0, max_batch=400, max_seq_len=4096, max_prefill_rows=0)
+    q, g = Q.activations(400, 70)
+    c8, c16 = Q.Q8Cache(lens, "e4m3", 32, seed=71), F16Cache(lens, 0, seed=72)
+    for window, sinks in ((256, 4), (0, 0), (100, 3), (1500, 20), (256, 4)):
+        a, b = (torch.zeros(400, 16, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+        kv.decode_attn_q8(a, q, g, c8.layout(), Q.i32(lens), window=window, sinks=sinks)
+        c16.decode(kv, b, q, g, lens, window, sinks)
+        rows = [(i, i, Q.visible(lens[i], window, sinks)) for i in range(0, 400, 17)]
+        Q.check_rows(a, q, g, rows, c8.values)
+        if window:
+            Q.check_rows(b, q, g, rows, c16.values)
+    assert kv.device_status() == 0
+    small = KvPath(0, max_batch=400, max_seq_len=256, max_prefill_rows=0)  # every row of the handle is one key range
+    short = [min(n, 256) for n in lens]
+    a = torch.zeros(400, 16, 128, dtype=torch.float16, device="cuda")
+    small.decode_attn_q8(a, q, g, c8.layout(), Q.i32(short))
+    Q.check_rows(a, q, g, [(i, i, np.arange(short[i])) for i in range(0, 400, 17)], c8.values)
+    assert small.device_status() == 0
