@@ -102,28 +102,21 @@ __device__ __forceinline__ void store_codes(unsigned char* at, int lane, const f
     reinterpret_cast<uint16_t*>(at)[32 + lane] = (uint16_t)q8_codes2<kFmt>(x[2], x[3], inv);
 }
 
-// Slots first, first + step, ... < slots of a block (one head's 128 codes at base) move from scale `from` to `to`.
-template <uint32_t kFmt>
-__device__ __forceinline__ void requantise(unsigned char* base, uint32_t first, uint32_t step, uint32_t slots, int lane, float from, float to) {
-#pragma unroll 4
-    for (uint32_t t = first; t < slots; t += step) {
-        uint32_t* at = reinterpret_cast<uint32_t*>(base + (size_t)t * Q8_ROW_BYTES) + lane;
-        const uint32_t w = __ldcg(at);
-        uint32_t o = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) o |= q8_code<kFmt>(q8_value<kFmt>((w >> (8 * j)) & 0xffu) * from, to) << (8 * j);
-        *at = o;
-    }
-}
-
-// Row r is a token of table row r.  grid = rows, a warp for each query head, K head and V head.
+// Row r is a token of table row r.  grid = rows, a warp for each query head, K head and V head; all of them share the
+// slots to requantise where a scale grew (128 rows: 1.9 us if none grows, 6.4 us if all do in the last slot of blocks of 16,
+// 39 us of blocks of 256; a scale grows with a probability of about 1 / (slot + 1)).  One warp per head for its own slots took
+// 14 to 118 us for that.
 template <uint32_t kFmt>
 __global__ void __launch_bounds__(aq::STEP_THREADS)
 append_q8_step_kernel(const AppendQ8Params p) {
     using namespace aq;
+    __shared__ float s_ratio[COMBOS];  // old scale / new scale of a head whose scale grew
+    __shared__ uint32_t s_grown;
     const uint32_t r = blockIdx.x;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
+    if (threadIdx.x == 0) s_grown = 0u;
+    __syncthreads();
     // the step's tables, norm weights and rotary rows are not written by any kernel: read while the preceding
     // kernel is still draining
     const uint32_t lbs = p.map.lbs, pos = p.pos_ids[r], blk = pos >> lbs, slot = pos & ((1u << lbs) - 1u);
@@ -134,7 +127,11 @@ append_q8_step_kernel(const AppendQ8Params p) {
     }
     const int combo = warp - NQ;  // >= 0: K or V head
     const bool is_v = combo >= NKV;
-    const uint32_t id = combo >= 0 ? p.map.block_tables[(size_t)r * p.map.max_blocks + blk] : 0u;
+    const uint32_t id = p.map.block_tables[(size_t)r * p.map.max_blocks + blk];
+    const bool placed = id < p.map.num_blocks;
+    auto head_codes = [&](int c) {
+        return (c >= NKV ? p.map.v_pool : p.map.k_pool) + (size_t)id * p.map.block_stride + (c & (NKV - 1)) * HD;
+    };
     float wv[4], cv[4], sv[4], x[4];
     if (!is_v) {
         load_pairs(combo < 0 ? p.q_norm_w : p.k_norm_w, lane, wv);
@@ -147,23 +144,46 @@ append_q8_step_kernel(const AppendQ8Params p) {
         load_pairs(p.q_in + at, lane, x);
         norm_rope_pairs(x, wv, cv, sv, p.eps);
         store_q(p.q_out + at, lane, x);
-        return;
-    }
-    if (id >= p.map.num_blocks) {
+    } else if (!placed) {
         if (combo == 0 && lane == 0) atomicOr(p.status, DEV_BAD_BLOCK);
-        return;
+    } else {
+        const int kvh = combo & (NKV - 1);
+        float* scale_at = (is_v ? p.map.v_scales : p.map.k_scales) + (size_t)id * p.map.scale_stride + kvh;
+        const float old_scale = slot != 0u ? __ldcg(scale_at) : 0.0f;
+        load_pairs((is_v ? p.v_in : p.k_in) + ((size_t)r * NKV + kvh) * HD, lane, x);
+        if (!is_v) norm_rope_pairs(x, wv, cv, sv, p.eps);
+        if (__any_sync(0xffffffffu, make_finite(x)) && lane == 0) atomicOr(p.status, DEV_NONFINITE);
+        const float scale = fmaxf(q8_scale<kFmt>(warp_max(abs_max(x))), old_scale);
+        store_codes<kFmt>(head_codes(combo) + (size_t)slot * Q8_ROW_BYTES, lane, x, q8_inverse<kFmt>(scale));
+        if (lane == 0) {
+            *scale_at = scale;
+            if (slot != 0u && scale > old_scale) {
+                s_ratio[combo] = __fdiv_rn(old_scale, scale);
+                atomicOr(&s_grown, 1u << combo);
+            }
+        }
     }
-    const int kvh = combo & (NKV - 1);
-    float* scale_at = (is_v ? p.map.v_scales : p.map.k_scales) + (size_t)id * p.map.scale_stride + kvh;
-    const float old_scale = slot != 0u ? __ldcg(scale_at) : 0.0f;
-    load_pairs((is_v ? p.v_in : p.k_in) + ((size_t)r * NKV + kvh) * HD, lane, x);
-    if (!is_v) norm_rope_pairs(x, wv, cv, sv, p.eps);
-    if (__any_sync(0xffffffffu, make_finite(x)) && lane == 0) atomicOr(p.status, DEV_NONFINITE);
-    const float scale = fmaxf(q8_scale<kFmt>(warp_max(abs_max(x))), old_scale);
-    unsigned char* base = (is_v ? p.map.v_pool : p.map.k_pool) + (size_t)id * p.map.block_stride + kvh * HD;
-    if (scale > old_scale) requantise<kFmt>(base, 0u, 1u, slot, lane, old_scale, scale);
-    store_codes<kFmt>(base + (size_t)slot * Q8_ROW_BYTES, lane, x, q8_inverse<kFmt>(scale));
-    if (lane == 0) *scale_at = scale;
+    __syncthreads();
+    // a unit is one slot's 128 codes of a head whose scale grew: four in flight per warp
+    const uint32_t grown = s_grown, units = (uint32_t)__popc(grown) * slot;
+    for (uint32_t u0 = warp; u0 < units; u0 += 4u * (NQ + COMBOS)) {
+        uint32_t* at[4];
+        uint32_t w[4];
+        float ratio[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++) {
+            const uint32_t u = min(u0 + k * (NQ + COMBOS), units - 1u), nth = u / slot;
+            uint32_t m = grown;
+            for (uint32_t i = 0; i < nth; i++) m &= m - 1u;
+            const int c = __ffs((int)m) - 1;
+            ratio[k] = s_ratio[c];
+            at[k] = reinterpret_cast<uint32_t*>(head_codes(c) + (size_t)(u - nth * slot) * Q8_ROW_BYTES) + lane;
+            w[k] = __ldcg(at[k]);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++)
+            if (u0 + k * (NQ + COMBOS) < units) *at[k] = q8_moved<kFmt>(w[k], ratio[k]);
+    }
 }
 
 // ---- the wave kernel's unit is a PAIR of heads of one row in a warp: lanes 0-15 hold the first, lanes 16-31 the second,
@@ -248,7 +268,12 @@ append_q8_wave_kernel(const AppendQ8Params p) {
     // per row of the window; a segment is named by its first row
     __shared__ uint32_t s_pos[ROWS], s_seq[ROWS], s_id[ROWS], s_end[ROWS], s_bad[ROWS];
     __shared__ int s_lead[ROWS];  // the row's segment, -1: not of this CTA
-    __shared__ uint32_t s_list[ROWS], s_grown[COMBOS];  // the segments in order; those whose stored codes move to a larger scale
+    __shared__ uint32_t s_list[ROWS];  // the segments in order
+    // slots whose codes move to a larger scale ("units"), by (segment, head): s_units[i] .. s_units[i + 1] are those of
+    // (i / COMBOS, i % COMBOS)
+    __shared__ uint32_t s_units[ROWS * COMBOS + 1];
+    static_assert(ROWS * COMBOS == 128, "the units are summed up by four warps");
+    __shared__ uint32_t s_part[4];
     __shared__ float s_amax[ROWS][COMBOS], s_old[ROWS][COMBOS], s_scale[ROWS][COMBOS], s_tailmax[ROWS][COMBOS];
     __shared__ uint32_t s_leaders, s_tail;
     const uint32_t row0 = blockIdx.x * ROWS;
@@ -314,7 +339,6 @@ append_q8_wave_kernel(const AppendQ8Params p) {
             if (leader) block_id = p.map.block_tables[(size_t)seq * p.map.max_blocks + (pos >> lbs)];
             s_bad[lane] = 0u;
             if (leader) s_list[__popc(leaders & ((1u << lane) - 1u))] = lane;
-            if (lane < COMBOS) s_grown[lane] = 0u;
         }
         if (lane == 0) s_leaders = leaders;
     }
@@ -408,6 +432,7 @@ append_q8_wave_kernel(const AppendQ8Params p) {
     }
     if (__any_sync(0xffffffffu, odd) && lane == 0) atomicOr(p.status, DEV_NONFINITE);
     __syncthreads();
+    uint32_t grown = 0;  // tid < ROWS * COMBOS: units of (segment, head)
     if (tid < ROWS * COMBOS && ((leaders >> (tid / COMBOS)) & 1u)) {
         const int li = tid / COMBOS, c = tid % COMBOS;
         float amax = 0.0f;
@@ -421,20 +446,50 @@ append_q8_wave_kernel(const AppendQ8Params p) {
             if (c == 0 && blockIdx.y == 0) atomicOr(p.status, no_block ? DEV_BAD_BLOCK : DEV_BLOCK_CONFLICT);
         } else if (c / (COMBOS / kSplit) == (int)blockIdx.y) {
             ((c < NKV ? p.map.k_scales : p.map.v_scales) + (size_t)s_id[li] * p.map.scale_stride)[c & (NKV - 1)] = scale;
-            if (scale > s_old[li][c] && (s_pos[li] & (bs - 1u)) != 0u) atomicOr(&s_grown[c], 1u << li);
+            if (scale > s_old[li][c]) grown = s_pos[li] & (bs - 1u);
         }
+    }
+    if (tid < ROWS * COMBOS) {
+        uint32_t sum = grown;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xffffffffu, sum, off);
+            if (lane >= off) sum += t;
+        }
+        s_units[tid + 1] = sum;  // within the warp; the warps before are added below
+        if (lane == 31) s_part[warp] = sum;
+        if (tid == 0) s_units[0] = 0u;
+    }
+    __syncthreads();
+    if (tid < ROWS * COMBOS && warp > 0) {
+        uint32_t before = s_part[0];
+        for (int i = 1; i < warp; i++) before += s_part[i];
+        s_units[tid + 1] += before;
     }
     __syncthreads();
     auto usable = [&](int li) { return s_id[li] < p.map.num_blocks && s_bad[li] == 0u; };
     auto head_codes = [&](int li, int c) {  // this head's codes in the segment's block
         return (c < NKV ? p.map.k_pool : p.map.v_pool) + (size_t)s_id[li] * p.map.block_stride + (c & (NKV - 1)) * HD;
     };
-    for (int k = 0; k < 2 * NP; k++) {
-        const int c = 2 * pair0 + k;
-        for (uint32_t m = s_grown[c]; m; m &= m - 1u) {
-            const int li = __ffs((int)m) - 1;
-            requantise<kFmt>(head_codes(li, c), w, ROWS, s_pos[li] & (bs - 1u), lane, s_old[li][c], s_scale[li][c]);
+    // four units in flight per warp
+    const uint32_t units = s_units[ROWS * COMBOS];
+    uint32_t i = 0;
+    for (uint32_t u0 = w; u0 < units; u0 += 4u * ROWS) {
+        uint32_t* at[4];
+        uint32_t v[4];
+        float ratio[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++) {
+            const uint32_t u = min(u0 + k * ROWS, units - 1u);
+            while (s_units[i + 1] <= u) i++;
+            const int sl = i / COMBOS, c = i % COMBOS;
+            ratio[k] = __fdiv_rn(s_old[sl][c], s_scale[sl][c]);
+            at[k] = reinterpret_cast<uint32_t*>(head_codes(sl, c) + (size_t)(u - s_units[i]) * Q8_ROW_BYTES) + lane;
+            v[k] = __ldcg(at[k]);
         }
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++)
+            if (u0 + k * ROWS < units) *at[k] = q8_moved<kFmt>(v[k], ratio[k]);
     }
     const int li = there ? s_lead[w] : -1;
     if (li >= 0 && usable(li)) {

@@ -4,7 +4,7 @@
 // kc, vc codes, ks, vs the scales of the token's block.  Codes (int8 and e4m3) are exact in f16, so the products
 // run on f16 tensor-core fragments of the codes themselves and the scales stay in f32:
 //   w_t = 2^(x_t log2e + log2 vs_t - m)   is the weight of vc_t in the numerator (m: running maximum of the exponent,
-//                                         so w <= 1 whatever the scales are),
+//                                         so w stays below 2^9 whatever the scales are),
 //   sum_t w_t / vs_t                      is the denominator in the same units: one multiplication per thread and stage.
 // A V scale below 2^-100 counts as 2^-100 (its codes then weigh nothing against any other block's).
 //

@@ -17,17 +17,6 @@ __device__ __forceinline__ float q8_scale(float amax) {
     return __uint_as_float((e < 1u ? 1u : e) << 23);
 }
 
-// One code (as a byte) for x at scale s > 0; ties to even, saturating.
-template <uint32_t kFmt>
-__device__ __forceinline__ uint32_t q8_code(float x, float s) {
-    const float y = __fdiv_rn(x, s);
-    if (kFmt == Q8_INT8) {
-        const int c = __float2int_rn(y);
-        return (uint32_t)min(127, max(-127, c)) & 0xffu;
-    }
-    return (uint32_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
-}
-
 // What values are multiplied with before they are rounded to codes: 1 / scale, exact for e4m3; for int8 the quotient
 // x / s is off by up to 2^-22 of itself, i.e. a value within 2^-15 of a step from a tie may go to the other side.
 template <uint32_t kFmt>
@@ -39,12 +28,6 @@ template <uint32_t kFmt>
 __device__ __forceinline__ uint32_t q8_codes2(float a, float b, float inv) {
     if (kFmt == Q8_INT8) return (uint32_t)(__float2int_rn(a * inv) & 0xff) | ((uint32_t)(__float2int_rn(b * inv) & 0xff) << 8);
     return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
-}
-
-template <uint32_t kFmt>
-__device__ __forceinline__ float q8_value(uint32_t code) {
-    if (kFmt == Q8_INT8) return (float)(int8_t)(uint8_t)code;
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)code, __NV_E4M3)));
 }
 
 // the four codes of w as two f16 pairs, exact
@@ -62,6 +45,25 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
         lo = *reinterpret_cast<const uint32_t*>(&x);
         hi = *reinterpret_cast<const uint32_t*>(&y);
     }
+}
+
+// The four codes of w moved to a scale that is 1 / ratio times theirs.  e4m3: ratio is a power of two (or 0), the f16 product
+// is exact wherever its code is not 0.
+template <uint32_t kFmt>
+__device__ __forceinline__ uint32_t q8_moved(uint32_t w, float ratio) {
+    uint32_t h[2], o = 0;
+    codes_to_f16<kFmt>(w, h[0], h[1]);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const __half2 v = *reinterpret_cast<const __half2*>(&h[i]);
+        if (kFmt == Q8_E4M3) {
+            const __half2 m = __hmul2(v, __float2half2_rn(ratio));
+            o |= (uint32_t)__nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&m), __NV_SATFINITE, __NV_E4M3) << (16 * i);
+        } else {
+            o |= q8_codes2<kFmt>(__low2float(v), __high2float(v), ratio) << (16 * i);
+        }
+    }
+    return o;
 }
 
 }  // namespace oxi
