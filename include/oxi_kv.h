@@ -363,7 +363,9 @@ int32_t oxi_prefill_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const vo
  * window: row b attends t < seq_lens[b] with t >= seq_lens[b] - window or t < sinks.  Keys keep the rotation of
  * their own positions.  Arguments otherwise as the entry point without `_sinks`, whose bytes they return when
  * window or sinks is 0; else the gated result is rounded once instead of before and after the gate, and rows
- * of prefill waves longer than max_seq_len are skipped (OXI_DEV_BAD_SEQ_LEN).  What no row sees may hold anything. */
+ * of prefill waves longer than max_seq_len are skipped (OXI_DEV_BAD_SEQ_LEN).  What no row sees may hold anything, and so
+ * may the table entries of blocks without a visible token (here and in the 8-bit forms): a block between sinks
+ * and window can be given back. */
 int32_t oxi_decode_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
                               const uint64_t* k_ptrs, const uint64_t* v_ptrs, const uint32_t* seq_lens, uint32_t batch,
                               uint32_t window, uint32_t sinks);

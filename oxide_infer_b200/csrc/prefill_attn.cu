@@ -331,6 +331,12 @@ __device__ __forceinline__ bool pf_next_run(uint32_t& next, uint32_t nruns, cons
     return false;
 }
 
+// Whether a row of a run whose windows start at `lo` or later sees a token of page pg: the table entries of the other pages
+// may be those of blocks that were given back.
+__device__ __forceinline__ bool pf_page_seen(const PagedMap& pm, uint32_t pg, uint32_t lo, uint32_t last_page, uint32_t sinks) {
+    return pg <= last_page && (((pg + 1u) << pm.lbs) > lo || (pg << pm.lbs) < sinks);
+}
+
 // Block ids of a run's tiles for one loader warp of the f16 cache (kAlign): a lane holds one page of a stretch of CHUNK tiles, whose
 // pages fit a warp, and one of the stretch after it, requested when the first began.  With one tile of lookahead
 // every tile at an item's start waited for a table entry: 64 rows with a window of 1,024 took 35 us instead of 32, the wave
@@ -339,11 +345,13 @@ struct PfPages {
     static constexpr uint32_t CHUNK = 7;       // 7 * 64 tokens from a multiple of 16 on: at most 29 pages of >= 16 tokens
     static constexpr uint32_t WINDOW = 1u << 20;  // stretches of the window part are numbered from here on
     const uint32_t* trow;                      // the sequence's row of the block table
-    uint32_t last_page;
+    uint32_t lo, last_page, sinks;
     uint32_t chunk, page0, id, nchunk, npage0, nid;
-    __device__ __forceinline__ void open(const PagedMap& pm, uint32_t seq, uint32_t hi) {
+    __device__ __forceinline__ void open(const PagedMap& pm, const PfRun& run, uint32_t seq, uint32_t nsinks) {
         trow = pm.block_tables + (size_t)seq * pm.max_blocks;
-        last_page = (hi - 1u) >> pm.lbs;
+        lo = run.lo;
+        last_page = (run.hi - 1u) >> pm.lbs;
+        sinks = nsinks;
         chunk = nchunk = 0xffffffffu;
     }
     __device__ __forceinline__ static uint32_t first_tile(const PfTiles& tl, uint32_t c) {
@@ -352,7 +360,7 @@ struct PfPages {
     __device__ __forceinline__ uint32_t request(const PagedMap& pm, const PfTiles& tl, uint32_t c, uint32_t& p0) const {
         p0 = tl.first_key(first_tile(tl, c)) >> pm.lbs;
         const uint32_t pg = p0 + (threadIdx.x & 31u);
-        return pg <= last_page ? __ldg(trow + pg) : 0u;
+        return pf_page_seen(pm, pg, lo, last_page, sinks) ? __ldg(trow + pg) : 0u;
     }
     // makes `tile` (of a run whose tiles end at tile1) the current one
     __device__ __forceinline__ void seek(const PagedMap& pm, const PfTiles& tl, uint32_t tile, uint32_t tile1, uint32_t* status) {
@@ -989,7 +997,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
         auto fetch_pages = [&]() -> uint32_t {
             const uint32_t pg = (tl.first_key(tile) >> pm.lbs) + (uint32_t)lane;
             uint32_t id = 0;
-            if (lane < 4 && pg <= last_page) {
+            if (lane < 4 && pf_page_seen(pm, pg, run.lo, last_page, view.sinks)) {
                 id = __ldg(trow + pg);
                 if (id >= pm.num_blocks) {
                     atomicOr(status, DEV_BAD_BLOCK);
@@ -1117,7 +1125,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             }
             uint32_t pg_next = (paged && tile0 < tile1) ? fetch_pages(tl.first_key(tile0)) : 0u;
             PfPages pages;
-            if (kAlign) pages.open(pm, (uint32_t)((c_kp[run.r0] >> 4) - 1ull), run.hi);
+            if (kAlign) pages.open(pm, run, (uint32_t)((c_kp[run.r0] >> 4) - 1ull), view.sinks);
             // Rows of a registered slab (at a whole number of 1024-byte rows from its base) come through the
             // TMA unit: two boxes per full tile, written in the same swizzled layout, completion counted on
             // the stage's barrier.  The run's ragged last tile keeps the zero-filling copies below.

@@ -412,6 +412,27 @@ def test_prefill_attention_ignores_keys_between_sinks_and_windows(kv, fmt, bad):
     assert torch.equal(base.view(torch.int16), again.view(torch.int16)) and kv.device_status() == 0
 
 
+@pytest.mark.parametrize("fmt,bs", [("int8", 16), ("e4m3", 32), ("int8", 64)])
+@pytest.mark.parametrize("window,sinks", [(70, 4), (40, 40), (300, 90), (100, 0)])
+def test_blocks_between_sinks_and_window_may_be_given_back(kv, fmt, bs, window, sinks):
+    """Table entries of blocks without a visible token hold an id that the pool does not have: same bytes, no status."""
+    c = Q.Q8Cache([700, 2000], fmt, bs, seed=47)
+    chunks = [(0, 620, 60), (1, 1900, 100)]
+    q, g = Q.activations(2, 48)
+
+    def both():
+        b = guarded(np.full((2, Q.NQ, Q.HD), 7.0, np.float16), "ctx")
+        kv.decode_attn_q8(b, q, g, c.layout(), Q.i32([680, 2000]), window, sinks)
+        return _prefill(kv, c, chunks, window, sinks)[0], b
+
+    want = both()
+    for s, p, _ in chunks:
+        c.dtables[s, -(-sinks // bs):(p + 1 - window) // bs] = -1
+    got = both()
+    assert kv.device_status() == 0
+    assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(want, got))
+
+
 def test_prefill_attention_skips_rows_and_reports_blocks(kv):
     c = Q.Q8Cache([100, 40], "int8", 16, seed=44)
     row_seq, lens = [0, 0, 1, 1, 0], [5, 0, 40, 16 * c.max_blocks + 1, 100]

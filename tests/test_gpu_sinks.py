@@ -247,6 +247,30 @@ def test_prefill_ignores_what_no_row_sees(kv, bs, window, sinks):
     assert torch.equal(a.view(torch.int16), b.view(torch.int16)) and kv.device_status() == 0
 
 
+@pytest.mark.parametrize("bs", [16, 32])
+@pytest.mark.parametrize("window,sinks", [(70, 4), (40, 40), (300, 90)])
+def test_blocks_between_sinks_and_window_may_be_given_back(kv, bs, window, sinks):
+    """Table entries of blocks without a visible token hold an id that the pool does not have: same bytes, no status."""
+    c = F16Cache([700, 2000], bs, seed=90)
+    chunks = [(0, 620, 60), (1, 1900, 100)]
+    row_seq, pos = Q.wave(chunks)
+    q, g = Q.activations(len(pos), 91)
+    last = np.array([680, 2000])
+
+    def both():
+        a, b = _ctx(len(pos)), _ctx(2)
+        c.prefill(kv, a, q, g, row_seq, pos + 1, window, sinks)
+        c.decode(kv, b, q[:2], g[:2], last, window, sinks)
+        return a, b
+
+    want = both()
+    for s, p, _ in chunks:
+        c.dtables[s, -(-sinks // bs):(p + 1 - window) // bs] = -1
+    got = both()
+    assert kv.device_status() == 0
+    assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(want, got))
+
+
 def test_prefill_skips_rows(kv):
     c = F16Cache([100, 40], 16, seed=74)
     row_seq, lens = [0, 0, 1, 1, 0], [5, 0, 40, 16 * c.max_blocks + 1, 100]
