@@ -594,9 +594,9 @@ int32_t oxi_prefill_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const vo
 int32_t oxi_decode_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
                               const uint64_t* k_ptrs, const uint64_t* v_ptrs, const uint32_t* seq_lens, uint32_t batch,
                               uint32_t window, uint32_t sinks) {
-    if (window == 0u || sinks == 0u) return oxi_decode_attn(h, stream, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, batch, window);
     REQ_HANDLE("oxi_decode_attn_sinks");
     REQ_DEVICE("oxi_decode_attn_sinks");
+    if (window == 0u || sinks == 0u) return oxi_decode_attn(h, stream, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, batch, window);
     REQ_PTR(ctx_out && q && k_ptrs && v_ptrs && seq_lens, "oxi_decode_attn_sinks");
     REQ_BATCH(batch, h->max_batch, "oxi_decode_attn_sinks");
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_decode_attn_sinks");
@@ -608,9 +608,9 @@ int32_t oxi_decode_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const 
 int32_t oxi_decode_attn_paged_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
                                     const oxi_paged_layout* layout, const uint32_t* seq_lens, uint32_t batch,
                                     uint32_t window, uint32_t sinks) {
-    if (window == 0u || sinks == 0u) return oxi_decode_attn_paged(h, stream, ctx_out, q, gate, layout, seq_lens, batch, window);
     REQ_HANDLE("oxi_decode_attn_paged_sinks");
     REQ_DEVICE("oxi_decode_attn_paged_sinks");
+    if (window == 0u || sinks == 0u) return oxi_decode_attn_paged(h, stream, ctx_out, q, gate, layout, seq_lens, batch, window);
     REQ_PTR(ctx_out && q && seq_lens, "oxi_decode_attn_paged_sinks");
     REQ_BATCH(batch, h->max_batch, "oxi_decode_attn_paged_sinks");
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_decode_attn_paged_sinks");
@@ -626,11 +626,11 @@ int32_t oxi_append_decode_sinks(oxi_handle* h, void* stream, void* ctx_out, void
                                 const void* cos_table, const void* sin_table, const uint32_t* pos_ids,
                                 const uint32_t* seq_lens, const uint64_t* k_ptrs, const uint64_t* v_ptrs,
                                 uint32_t batch, uint32_t window, uint32_t sinks, float eps) {
+    REQ_HANDLE("oxi_append_decode_sinks");
+    REQ_DEVICE("oxi_append_decode_sinks");
     if (window == 0u || sinks == 0u)
         return oxi_append_decode(h, stream, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos_table, sin_table, pos_ids,
                                  seq_lens, k_ptrs, v_ptrs, batch, window, eps);
-    REQ_HANDLE("oxi_append_decode_sinks");
-    REQ_DEVICE("oxi_append_decode_sinks");
     REQ_PTR(ctx_out && q_io && k_in && v_in && q_norm_w && k_norm_w && cos_table && sin_table && pos_ids &&
                 seq_lens && k_ptrs && v_ptrs, "oxi_append_decode_sinks");
     REQ_BATCH(batch, h->max_batch, "oxi_append_decode_sinks");
@@ -648,11 +648,11 @@ int32_t oxi_append_decode_paged_sinks(oxi_handle* h, void* stream, void* ctx_out
                                       const void* cos_table, const void* sin_table, const uint32_t* seq_lens,
                                       const oxi_paged_layout* layout, uint32_t batch, uint32_t window, uint32_t sinks,
                                       float eps) {
+    REQ_HANDLE("oxi_append_decode_paged_sinks");
+    REQ_DEVICE("oxi_append_decode_paged_sinks");
     if (window == 0u || sinks == 0u)
         return oxi_append_decode_paged(h, stream, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos_table, sin_table,
                                        seq_lens, layout, batch, window, eps);
-    REQ_HANDLE("oxi_append_decode_paged_sinks");
-    REQ_DEVICE("oxi_append_decode_paged_sinks");
     REQ_PTR(ctx_out && q_io && k_in && v_in && q_norm_w && k_norm_w && cos_table && sin_table && seq_lens,
             "oxi_append_decode_paged_sinks");
     REQ_BATCH(batch, h->max_batch, "oxi_append_decode_paged_sinks");
@@ -670,9 +670,9 @@ int32_t oxi_append_decode_paged_sinks(oxi_handle* h, void* stream, void* ctx_out
 int32_t oxi_prefill_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
                                const uint64_t* k_ptrs, const uint64_t* v_ptrs, const uint32_t* seq_lens, uint32_t rows,
                                uint32_t window, uint32_t sinks) {
-    if (window == 0u || sinks == 0u) return oxi_prefill_attn(h, stream, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, rows, window);
     REQ_HANDLE("oxi_prefill_attn_sinks");
     REQ_DEVICE("oxi_prefill_attn_sinks");
+    if (window == 0u || sinks == 0u) return oxi_prefill_attn(h, stream, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, rows, window);
     REQ_PTR(ctx_out && q && k_ptrs && v_ptrs && seq_lens, "oxi_prefill_attn_sinks");
     REQ_BATCH(rows, h->max_prefill_rows, "oxi_prefill_attn_sinks");
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_prefill_attn_sinks");
@@ -687,9 +687,9 @@ int32_t oxi_prefill_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const
 int32_t oxi_prefill_attn_paged_sinks(oxi_handle* h, void* stream, void* ctx_out, const void* q, const void* gate,
                                      const oxi_paged_layout* layout, const uint32_t* row_seq, const uint32_t* seq_lens,
                                      uint32_t rows, uint32_t window, uint32_t sinks) {
-    if (window == 0u || sinks == 0u) return oxi_prefill_attn_paged(h, stream, ctx_out, q, gate, layout, row_seq, seq_lens, rows, window);
     REQ_HANDLE("oxi_prefill_attn_paged_sinks");
     REQ_DEVICE("oxi_prefill_attn_paged_sinks");
+    if (window == 0u || sinks == 0u) return oxi_prefill_attn_paged(h, stream, ctx_out, q, gate, layout, row_seq, seq_lens, rows, window);
     REQ_PTR(ctx_out && q && row_seq && seq_lens, "oxi_prefill_attn_paged_sinks");
     REQ_BATCH(rows, h->max_prefill_rows, "oxi_prefill_attn_paged_sinks");
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_prefill_attn_paged_sinks");

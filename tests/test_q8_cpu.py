@@ -56,6 +56,7 @@ def test_layout_fields():
     lambda p: p.__setitem__(2, torch.zeros(5, 8)[:, :4]),
     lambda p: p.__setitem__(4, p[4].long()),
     lambda p: p.__setitem__(4, torch.zeros(3, 2, dtype=torch.int32).t()),
+    lambda p: p.__setitem__(4, p[4].to("meta")),
 ])
 def test_layout_refuses_tensors_of_another_form(change):
     from oxide_infer_b200 import PagedQ8Layout
@@ -63,3 +64,52 @@ def test_layout_refuses_tensors_of_another_form(change):
     change(p)
     with pytest.raises(ValueError):
         PagedQ8Layout.of(*p)
+
+
+def test_tensors_on_another_device_than_the_handle_are_refused():
+    """Before anything is called: a handle without a library behind it, host tensors, a layout of host tensors."""
+    from oxide_infer_b200 import KvPath, PagedQ8Layout
+
+    class Somewhere(torch.Tensor):
+        """Says that it is on the handle's device."""
+        def get_device(self):
+            return 0
+
+    kv = KvPath.__new__(KvPath)
+    kv.device, kv.lib, kv.h = 0, None, None
+    kv._stream = lambda: 0
+    there = lambda: torch.zeros(1, 16, 128).as_subclass(Somewhere)  # noqa: E731
+    here = torch.zeros(1, 16, 128)
+    lay = PagedQ8Layout.of(*_parts())
+    near = PagedQ8Layout.of(*_parts())
+    near.device = 0
+    assert lay.device == -1
+
+    class _Refuses:
+        def __getattr__(self, name):
+            def call(*a):
+                raise AssertionError("called")
+            return call
+
+    def refused(name, n, layout_at, rest):
+        fn = getattr(kv, name)
+        for bad in range(n):
+            args = [here if i == bad else near if i == layout_at else there() for i in range(n)]
+            if bad == layout_at:
+                if name.endswith("q8"):
+                    args[bad] = lay
+                else:
+                    continue
+            kv.lib = _Refuses()
+            with pytest.raises(ValueError):
+                fn(*args, *rest)
+
+    refused("append_q8", 11, 9, ())
+    refused("decode_attn_q8", 5, 3, ())
+    refused("prefill_attn_q8", 6, 3, ())
+    refused("decode_attn_sinks", 6, None, (4, 2))
+    refused("decode_attn_paged_sinks", 5, 3, (4, 2))
+    refused("append_decode_sinks", 13, None, (4, 2))
+    refused("append_decode_paged_sinks", 11, 10, (4, 2))
+    refused("prefill_attn_sinks", 6, None, (4, 2))
+    refused("prefill_attn_paged_sinks", 6, 3, (4, 2))
