@@ -165,7 +165,8 @@ int32_t oxi_prefill_attn(oxi_handle* h, void* stream, void* ctx_out, const void*
  * launch to launch.  min_part_keys = 0 or slots = 0 turns the split off and
  * frees the reservation; otherwise min_part_keys >= 256 and slots <= 4096.
  * Synchronises the device; call it with no work of this handle in flight.
- * Applies to oxi_prefill_attn and oxi_prefill_attn_paged. */
+ * Applies to oxi_prefill_attn and oxi_prefill_attn_paged, and with a quarter of min_part_keys to oxi_prefill_attn_q8
+ * and the _sinks forms. */
 #define OXI_PREFILL_SPLIT_DEFAULT_MIN_PART_KEYS 512u
 int32_t oxi_prefill_split_configure(oxi_handle* h, uint32_t min_part_keys, uint32_t slots);
 uint64_t oxi_prefill_split_slot_bytes(void);

@@ -110,6 +110,7 @@ struct PfSplit {
     uint32_t part_tiles;    // smallest part, in tiles; 0: no split
     uint32_t max_slots;     // slots of part_o / part_ml
     uint32_t target_items;  // items the wave should not exceed (the SM count)
+    uint32_t by_runs;       // a block's work: the sum of its runs' tiles, not the tiles of the union of its rows' intervals
 };
 
 // Sliding window with sinks and the 8-bit cache (kSinks, kFmt of the kernel).
@@ -227,7 +228,16 @@ prefill_plan_small_kernel(const uint32_t* __restrict__ seq_lens, uint32_t rows, 
     __syncthreads();
     for (uint32_t r = tid; r < rows; r += 1024) {
         const uint32_t sl = seq_lens[r];
-        if (sl != 0u) {
+        if (sp.by_runs) {
+            // rows whose lengths go up by one are taken for a run: s_hi sums up the runs' keys, s_lo counts the runs
+            const uint32_t b = r / BLK;
+            if (sl != 0u && (r % BLK == 0u || seq_lens[r - 1u] + 1u != sl)) {
+                const uint32_t w = window_start(sl, window);
+                atomicAdd(&s_hi[b], (min(sinks, w) + TK - 1u) / TK * TK - w);
+                atomicAdd(&s_lo[b], 1u);
+            }
+            if (sl != 0u && (r % BLK == BLK - 1u || r + 1u == rows || seq_lens[r + 1u] != sl + 1u)) atomicAdd(&s_hi[b], sl);
+        } else if (sl != 0u) {
             atomicMin(&s_lo[r / BLK], window_start(sl, window));
             atomicMax(&s_hi[r / BLK], sl);
         }
@@ -237,18 +247,17 @@ prefill_plan_small_kernel(const uint32_t* __restrict__ seq_lens, uint32_t rows, 
     uint32_t key = 0, ns = 1;
     if (tid < nblocks) {
         const uint32_t lo = s_lo[tid], hi = s_hi[tid];
-        key = hi > lo ? pf_tiles<true, false>(lo, hi, sinks).n : 0u;
+        key = sp.by_runs ? hi / TK + lo + 1u : hi > lo ? pf_tiles<true, false>(lo, hi, sinks).n : 0u;
+        s_key[tid] = key;
     }
+    __syncthreads();
     if (sp.part_tiles != 0u) {
         // Part size: the smallest P >= part_tiles with sum_b ceil(tiles_b / P) * 4 <= target_items and
         // at most 32 parts per block, by bisection in warp 0 (a split wave has at most 64 blocks).
         if (tid < 32) {
             const uint32_t t0 = key;  // tiles of block tid and of block tid + 32
             uint32_t tb = 0u;
-            if (tid + 32 < nblocks) {
-                const uint32_t lo2 = s_lo[tid + 32], hi2 = s_hi[tid + 32];
-                tb = hi2 > lo2 ? pf_tiles<true, false>(lo2, hi2, sinks).n : 0u;
-            }
+            if (tid + 32 < nblocks) tb = s_key[tid + 32];
             uint32_t tmax = max(t0, tb);
 #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) tmax = max(tmax, __shfl_xor_sync(0xffffffffu, tmax, off));
@@ -1240,6 +1249,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
         }
     };
+    if constexpr (kQ8) __syncwarp();  // setmaxnreg is executed by whole warps
     if constexpr (!kQ8) {
         run_items(std::integral_constant<int, 0>{});
         finish();
@@ -1404,6 +1414,7 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
     // ... and a wave of at most one item per SM needs no order: no plan kernel
     const bool direct = view_variant && !split && nblocks * NKV <= (uint32_t)num_sms;
     PfSplit sp{};
+    sp.by_runs = view_variant;  // (the plain entry points keep their parts, on which the bytes of a split wave depend)
     if (split) {
         sp.units = ws->units;
         sp.slots = ws->units + 1024 * PF_MAX_SPLIT;
@@ -1411,6 +1422,10 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
         sp.part_o = ws->part;
         sp.part_ml = ws->part + (size_t)ws->max_slots * NKV * 2 * pf::M * HD;
         sp.part_tiles = (part_keys + pf::TK - 1) / pf::TK;
+        // The variants' blocks are short (a window) or slow per tile (8 bits), and plan and merge are paid already: a quarter.
+        // Parts of 8 / 5 / 4 / 2 tiles: 585 rows, window 512, e4m3 32.7 / 29.2 / 27.9 / 27.7 us; 6 chunks, window 100, 70
+        // sinks, f16 34.4 / 30.7 / 28.6 / 26.3; 64 rows on 4,096 keys, int8 31.1 / 28.2 / 27.3 / 27.2.
+        if (view_variant) sp.part_tiles = (sp.part_tiles + 3u) / 4u;
         sp.max_slots = ws->max_slots;
         sp.target_items = (uint32_t)num_sms;
     }
