@@ -404,9 +404,9 @@ struct PfPages {
 // kSinks: the window leaves the first tokens visible (PfView); a run's tiles are then PfTiles, keys that no row of the
 // run sees are zero-filled, and the gate is applied before the one rounding of the result.
 // kFmt (with kPaged and kSinks): the 8-bit cache.  Loader warps (two for K, two for V: a conversion takes one warp about as long
-// as a tile's MMAs and softmax; three each measured 3 % slower: they take issue slots from the softmax) hold the next tile's codes in registers while they convert the current one to an f16 tile of the
-// ring, exactly: scales never enter the operands.  A tile's four
-// 16-key groups have one K scale and one V scale each; the softmax multiplies the scores of a group by its K scale in
+// as a tile's MMAs and softmax; three each measured 3 % slower: they take issue slots from the softmax) hold the next
+// tile's codes in registers while they convert the current one to an f16 tile of the ring, exactly: scales never enter
+// the operands.  A tile's four 16-key groups have one K scale and one V scale each; the softmax multiplies the scores of a group by its K scale in
 // the fma that it does anyway and adds log2 of the V scale to the exponent, so that P carries the V scales, and the
 // row sum takes each group's partial sum times 1 / (V scale): 8 instructions a tile more than the f16 cache.
 constexpr uint32_t PF_F16 = 0, PF_INT8 = 1, PF_E4M3 = 2;
@@ -1404,8 +1404,8 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
     const bool armed = flt.skip_plus1 != 0u && !pm && !sinks;
     bool split = !armed && ws && ws->max_slots != 0u && part_keys != 0u && nblocks * NKV < (uint32_t)num_sms;
     // with sinks or the 8-bit cache: a window so short that two runs in a block have no more tiles than the smallest part is
-    // not split (the merge costs 2.5 us: 64 rows, window 64: 16.1 against 18.6 us; window 512 24.9 / 24.7, 1,024 34.3 / 26.7;
-    // blocks of up to three runs with a window of 100 and 70 sinks: 36.8 against 30.3), ...
+    // not split (plan and merge cost 3.5 us: 64 rows of one sequence, int8, unsplit / split, window 64: 15 / 18.6 us, 256
+    // 19.2 / 21.2, 512 24.1 / 21.8, 1,024 33.8 / 23.1; blocks of up to three runs, window 100, 70 sinks: 36.8 / 26.3), ...
     const bool view_variant = sinks || q8;
     if (view_variant && window && window <= (1u << 22) &&
         2u * ((window + pf::BLK - 1u + 15u + pf::TK - 1u) / pf::TK + ((sinks < (1u << 22) ? sinks : 1u << 22) + pf::TK - 1u) / pf::TK) <=
