@@ -200,8 +200,9 @@ def run(state):
     op = c["op"]
     if op == "append":
         if own:
+            # a decode step (row r is the one token of sequence r) passes no row_seq
             s["kv"].append_q8(s["q_out"], s["q"], s["k"], s["v"], s["wq"], s["wk"], s["cos"], s["sin"], s["pos"], s["layout"],
-                              row_seq=s["row_seq"], eps=EPS)
+                              row_seq=None if s["total"] == s["n"] else s["row_seq"], eps=EPS)
         else:
             _plain_append(s)
         out = {"q": s["q_out"], "k_scales": s["ks"], "v_scales": s["vs"]}
