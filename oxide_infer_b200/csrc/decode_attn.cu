@@ -103,7 +103,7 @@ static_assert(STAGE_BYTES % 16 == 0, "stage alignment");
 
 // stage descriptor flags (word z)
 constexpr uint32_t F_FIRST = 0x100u, F_LAST = 0x200u, F_END = 0x400u;
-constexpr uint32_t F_LASTRANGE = 0x800u;  // the item is its row's last key range (fused: the row's owner)
+constexpr uint32_t F_LASTRANGE = 0x800u;  // the item is its row's last key range (fused: the row's owner, unless the appended token has no block)
 }  // namespace dec
 
 struct DecodeParams {
@@ -243,8 +243,14 @@ decode_attn_kernel(const DecodeParams p) {
         // kSinks: lanes 0 .. npa-1 hold the pages of the item's sink groups from page `first_page` on, the lanes
         // behind them those of its window groups from page `first_page_w` on (3 / 2 CHUNK / 16 + 2 pages at most)
         uint32_t cfw = 0, cna = 0;
+        // A page whose table entry is not a block reads block 0.  Fused: bit l of `bad` - the page of lane l is such a page;
+        // the token being appended is not written there, and its key is read like the page's other keys (as after
+        // oxi_append_paged, which leaves the row out).
+        uint32_t cbad = 0;
         auto fetch_pages = [&](uint32_t b, uint32_t c, uint32_t slen, uint32_t& first_page, uint32_t& first_page_w,
-                               uint32_t& npa) -> uint32_t {
+                               uint32_t& npa, uint32_t& bad) -> uint32_t {
+            uint32_t id = 0;
+            bool none = false;
             if (kSinks) {
                 const RowView rv = row_view<GK>(slen, p.window, p.sinks);
                 const uint32_t v0 = c * (CHUNK / GK), v1 = rv.range_end(c, CHUNK / GK);
@@ -253,29 +259,26 @@ decode_attn_kernel(const DecodeParams p) {
                 const uint32_t vw = max(v0, rv.gs);
                 first_page_w = rv.token<GK>(vw) >> p.paged.lbs;
                 const uint32_t npw = vw < v1 ? (rv.token<GK>(v1 - 1u) >> p.paged.lbs) - first_page_w + 1u : 0u;
-                uint32_t id = 0;
                 if ((uint32_t)lane < npa + npw) {
                     id = __ldg(p.paged.block_tables + (size_t)b * p.paged.max_blocks +
                                ((uint32_t)lane < npa ? first_page + lane : first_page_w + lane - npa));
-                    if (id >= p.paged.num_blocks) {
-                        atomicOr(p.status, DEV_BAD_BLOCK);
-                        id = 0;
-                    }
+                    none = id >= p.paged.num_blocks;
                 }
-                return id;
-            }
-            const uint32_t t0 = window_start(slen, p.window) + c * CHUNK;
-            const uint32_t t1 = min(t0 + (uint32_t)CHUNK, slen);
-            first_page = t0 >> p.paged.lbs;
-            const uint32_t pg = first_page + (uint32_t)lane;
-            uint32_t id = 0;
-            if (pg <= ((t1 - 1u) >> p.paged.lbs)) {
-                id = __ldg(p.paged.block_tables + (size_t)b * p.paged.max_blocks + pg);
-                if (id >= p.paged.num_blocks) {
-                    atomicOr(p.status, DEV_BAD_BLOCK);
-                    id = 0;
+            } else {
+                const uint32_t t0 = window_start(slen, p.window) + c * CHUNK;
+                const uint32_t t1 = min(t0 + (uint32_t)CHUNK, slen);
+                first_page = t0 >> p.paged.lbs;
+                const uint32_t pg = first_page + (uint32_t)lane;
+                if (pg <= ((t1 - 1u) >> p.paged.lbs)) {
+                    id = __ldg(p.paged.block_tables + (size_t)b * p.paged.max_blocks + pg);
+                    none = id >= p.paged.num_blocks;
                 }
             }
+            if (none) {
+                atomicOr(p.status, DEV_BAD_BLOCK);
+                id = 0;
+            }
+            if (kFused) bad = __ballot_sync(0xffffffffu, none);
             return id;
         };
         if (cur < total_items) {
@@ -283,7 +286,7 @@ decode_attn_kernel(const DecodeParams p) {
             cc = cur - prefix[cb];
             cslen = s_len[cb];
             if (kPaged) {
-                cpg = fetch_pages(cb, cc, cslen, cfp, cfw, cna);
+                cpg = fetch_pages(cb, cc, cslen, cfp, cfw, cna, cbad);
             } else {
                 ckp = p.k_ptrs[cb];
                 cvp = p.v_ptrs[cb];
@@ -296,7 +299,7 @@ decode_attn_kernel(const DecodeParams p) {
             uint32_t nxt = __shfl_sync(0xffffffffu, claim, 0);
             if (kSinks && p.direct) nxt = cur;
             nxt = (nxt >= total_items) ? total_items : min(nxt + gridDim.x, total_items);
-            uint32_t nb = 0, nc = 0, nslen = 0, npg = 0, nfp = 0, nfw = 0, nna = 0;
+            uint32_t nb = 0, nc = 0, nslen = 0, npg = 0, nfp = 0, nfw = 0, nna = 0, nbad = 0;
             uint64_t nkp = 0, nvp = 0;
             claim = 0xffffffffu;  // "no more items" unless a new claim is made
             if (nxt < total_items) {
@@ -305,7 +308,7 @@ decode_attn_kernel(const DecodeParams p) {
                 nc = nxt - prefix[nb];
                 nslen = s_len[nb];
                 if (kPaged) {
-                    npg = fetch_pages(nb, nc, nslen, nfp, nfw, nna);
+                    npg = fetch_pages(nb, nc, nslen, nfp, nfw, nna, nbad);
                 } else {
                     nkp = p.k_ptrs[nb];
                     nvp = p.v_ptrs[nb];
@@ -327,10 +330,13 @@ decode_attn_kernel(const DecodeParams p) {
                 return v < rv.gs ? (tok >> p.paged.lbs) - cfp : cna + (tok >> p.paged.lbs) - cfw;
             };
             const uint32_t bs_mask = kPaged ? (1u << p.paged.lbs) - 1u : 0u;
+            bool placed = true;  // fused: the appended token has a block
             if (kPaged && kFused) {
                 // the consumers write the appended row at base + pos * row bytes: give them the base that
                 // makes this the row's place in its block (only meaningful in the row's last range)
-                const uint32_t pid = __shfl_sync(0xffffffffu, cpg, (kSinks ? page_lane(rv.ng - 1u, pos) : (pos >> p.paged.lbs) - cfp) & 31u);
+                const uint32_t at = (kSinks ? page_lane(rv.ng - 1u, pos) : (pos >> p.paged.lbs) - cfp) & 31u;
+                const uint32_t pid = __shfl_sync(0xffffffffu, cpg, at);
+                placed = !((cbad >> at) & 1u);
                 const uint64_t off = (uint64_t)pid * p.paged.block_stride + (uint64_t)(pos & bs_mask) * KV_ROW_BYTES -
                                      (uint64_t)pos * KV_ROW_BYTES;
                 ckp = (uint64_t)(uintptr_t)p.paged.k_pool + off;
@@ -350,7 +356,7 @@ decode_attn_kernel(const DecodeParams p) {
                 const bool first = (t == t0), last = (t + KS >= t1);
                 // fused: the owner's last stage ends with the key being appended; it is not in the
                 // cache yet, so one key less is copied and the raw k/v rows are delivered instead
-                const bool owner = kFused && last && last_range;
+                const bool owner = kFused && last && last_range && placed;
                 const uint32_t ncopy = owner ? nvalid - 1u : nvalid;
                 unsigned char* sb = stages + (size_t)slot * STAGE_BYTES;
                 const uint32_t vgrp = t / GK + (lane & (NGROUP - 1));         // kSinks: this lane's group and its first token
@@ -365,7 +371,7 @@ decode_attn_kernel(const DecodeParams p) {
                     *reinterpret_cast<uint4*>(sb + DESC_OFF) =
                         make_uint4(cb, cc | (nchunks << 16),
                                    nvalid | (first ? F_FIRST : 0u) | (last ? F_LAST : 0u) |
-                                       (last_range ? F_LASTRANGE : 0u), pos);
+                                       (last_range && placed ? F_LASTRANGE : 0u), pos);
                     *reinterpret_cast<uint4*>(sb + DESC_OFF + 16) =
                         make_uint4((uint32_t)ckp, (uint32_t)(ckp >> 32), (uint32_t)cvp, (uint32_t)(cvp >> 32));
                     uint32_t bytes = ncopy * 2u * KV_ROW_BYTES + (first ? Q_BYTES : 0);
@@ -422,7 +428,7 @@ decode_attn_kernel(const DecodeParams p) {
                     bulk_g2s(sbase + X_OFF + (lane == 19 ? X_K : X_V), src, KV_ROW_BYTES, &full_bar[slot]);
                 }
             }
-            cur = nxt; cb = nb; cc = nc; cslen = nslen; ckp = nkp; cvp = nvp; cpg = npg; cfp = nfp; cfw = nfw; cna = nna;
+            cur = nxt; cb = nb; cc = nc; cslen = nslen; ckp = nkp; cvp = nvp; cpg = npg; cfp = nfp; cfw = nfw; cna = nna; cbad = nbad;
         }
         if (ok) {
             // end-of-work descriptor so the consumers leave their loop

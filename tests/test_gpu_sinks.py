@@ -190,6 +190,47 @@ def test_fused_step_is_append_then_decode(kv, bs, window, sinks):
     assert torch.equal(outs[0][0].view(torch.int16), outs[1][0].view(torch.int16)) and torch.equal(outs[0][1], outs[1][1])
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 0), (100, 4), (8, 4), (400, 20)])
+@pytest.mark.parametrize("tail", [0, 1, 2, 3])
+def test_fused_step_does_not_write_a_token_that_has_no_block(kv, window, sinks, tail):
+    """The appended token's table entry is not a block of the pool: its key and value are not stored (block 0 belongs to another
+    sequence here, whose result stays), and the context is that of append and decode attention one after the other."""
+    lens = [16 + tail, 600, 560 + tail, 43]
+    n = len(lens)
+    gen = torch.Generator(device="cuda").manual_seed(92)
+    half = lambda *s: torch.randn(*s, generator=gen, device="cuda").half()  # noqa: E731
+    q, k, v, g = half(n, 16, 128), half(n, 4, 128), half(n, 4, 128), half(n, 16)
+    w = (1 + 0.1 * torch.randn(128, generator=gen, device="cuda")).half()
+    ang = torch.rand(max(lens) + 1, 128, generator=gen, device="cuda") * 6.28
+    cos, sin = ang.cos().half(), ang.sin().half()
+    pos, sl = Q.i32(lens), Q.i32([x + 1 for x in lens])
+    outs = []
+    for fused in (False, True):
+        c = F16Cache(lens, 16, seed=93)
+        c.kp.nan_to_num_(0.5)  # what is read in place of the missing block is finite
+        c.vp.nan_to_num_(0.5)
+        c.dtables[1, 0], c.dtables[0, 0], c.dtables[2, 3] = 0, 1, 2  # block 0 holds tokens that row 1 sees
+        for i, entry in ((0, c.nblocks), (2, -1)):
+            c.dtables[i, lens[i] // 16] = entry
+        before = [p.clone() for p in (c.kp, c.vp)]
+        qq, ctx = q.clone(), _ctx(n)
+        if fused:
+            kv.append_decode_paged_sinks(ctx, qq, k, v, g, w, w, cos, sin, sl, c.layout(), window, sinks)
+        else:
+            kv.append_paged(qq, k, v, w, w, cos, sin, pos, c.layout())
+            c.decode(kv, ctx, qq, g, [x + 1 for x in lens], window, sinks)
+        assert kv.device_status() == BAD_BLOCK
+        for p, old, new in ((c.kp, before[0], None), (c.vp, before[1], v)):
+            for i in (1, 3):  # the rows whose token has a block; everything else stays
+                b = int(c.dtables[i, lens[i] // 16])
+                if new is not None:
+                    assert torch.equal(p[b, lens[i] % 16], new[i])
+                old[b, lens[i] % 16] = p[b, lens[i] % 16]
+            assert torch.equal(p, old)
+        outs.append((ctx, c.kp, c.vp))
+    assert all(torch.equal(a.contiguous().view(torch.int16), b.contiguous().view(torch.int16)) for a, b in zip(*outs))
+
+
 WAVES = {
     "one row": [(0, 0, 1)],
     "a row behind a prefix": [(0, 900, 1)],
