@@ -693,11 +693,12 @@ decode_merge_kernel(const DecodeParams p) {
     const uint32_t b = blockIdx.x >> 2;
     const int lane = threadIdx.x & 31;
     const uint32_t hd = (blockIdx.x & 3u) * 4 + (threadIdx.x >> 5);
-    // step inputs (not written by any kernel): fetched while the streaming kernel drains
+    // lengths and pointers are inputs of the step: fetched while the streaming kernel drains
     const uint32_t slen = p.seq_lens[b];
     const uint64_t kvp = p.paged.block_tables ? 0ull : (p.k_ptrs[b] | p.v_ptrs[b]);
-    const float gate_f = p.gate ? h2f(p.gate[(size_t)b * NQ + hd]) : 0.0f;
     pdl_wait();
+    // the gate is not: the projection before the streaming kernel may have written it, and only the wait orders that
+    const float gate_f = p.gate ? h2f(p.gate[(size_t)b * NQ + hd]) : 0.0f;
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.work_counter = 0u;
     if (slen == 0u || slen > p.max_seq_len || (kvp & 15ull) != 0ull) return;
     if (p.paged.block_tables && ((slen - 1u) >> p.paged.lbs) >= p.paged.max_blocks) return;

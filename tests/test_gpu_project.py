@@ -251,3 +251,31 @@ def test_wave_kernel_skips_rows_with_misaligned_cache_pointers(kv):
         want_v = torch.from_numpy(case.v_cache[i]).cuda() if i == 599 else good.v_cache[i]
         assert torch.equal(d.k_cache[i].view(torch.int16), want_k.view(torch.int16)), i
         assert torch.equal(d.v_cache[i].view(torch.int16), want_v.view(torch.int16)), i
+
+
+def test_attention_right_behind_the_projection_takes_its_gate(kv):
+    """Projection and decode attention of rows of several key ranges, call after call without a wait on the host, every call with
+    another x and hence another gate in the same buffer: the bytes of the same calls with a wait behind each kernel."""
+    from oxide_infer_b200 import Linear
+    lens = [900, 3000, 513, 40, 7000]
+    b = len(lens)
+    case = DecodeCase(lens, seed=17)
+    lin = Linear(*_weights(18))
+    g = torch.Generator(device="cuda").manual_seed(19)
+    xs = [torch.randn(b, HIDDEN, device="cuda", generator=g).half() for _ in range(12)]
+
+    def run(wait):
+        d, q, gate = case.device(), torch.zeros(b, NQ, HD, dtype=torch.float16, device="cuda"), torch.zeros(b, NQ, dtype=torch.float16, device="cuda")
+        out = [torch.zeros(b, NQ, HD, dtype=torch.float16, device="cuda") for _ in xs]
+        torch.cuda.synchronize()
+        for x, ctx in zip(xs, out):
+            kv.project_append(lin, x, q, gate, d.q_norm_w, d.k_norm_w, d.cos, d.sin, d.pos_ids, d.k_ptrs, d.v_ptrs)
+            if wait:
+                torch.cuda.synchronize()
+            kv.decode_attn(ctx, q, gate, d.k_ptrs, d.v_ptrs, d.seq_lens, 0)
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return out
+
+    assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(run(True), run(False)))
