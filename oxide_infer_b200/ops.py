@@ -18,6 +18,7 @@ from . import _lib
 
 class PagedLayout(C.Structure):
     """oxi_paged_layout of include/oxi_kv.h: one layer's K/V pools and the rows' block tables."""
+    device = None  # of the tensors it was made of
     _fields_ = [("k_pool", C.c_void_p), ("v_pool", C.c_void_p), ("block_tables", C.c_void_p),
                 ("block_stride_bytes", C.c_uint64), ("max_blocks", C.c_uint32), ("block_size", C.c_uint32),
                 ("num_blocks", C.c_uint32)]
@@ -29,11 +30,16 @@ class PagedLayout(C.Structure):
         block_tables [batch][max_blocks] int32."""
         if not block_tables.is_contiguous():
             raise ValueError("block_tables must be contiguous")
+        if block_tables.element_size() != 4:
+            raise ValueError("block_tables must be int32")
+        if len({t.device for t in (k_pool, v_pool, block_tables)}) != 1:
+            raise ValueError("pools and block_tables must be on one device")
         stride = block_stride_bytes if block_stride_bytes is not None else k_pool.stride(0) * k_pool.element_size()
         nb = num_blocks if num_blocks is not None else k_pool.shape[0]
         out = cls(k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(), stride, block_tables.shape[1],
                   block_size, nb)
         out._keep = (k_pool, v_pool, block_tables)
+        out.device = k_pool.get_device()
         return out
 
 
@@ -128,14 +134,19 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
-def _ptrs(device: int, *tensors):
-    """Addresses of contiguous tensors on the handle's device (None stays None)."""
+_F16, _U32, _ADDR = (torch.float16,), (torch.int32, torch.uint32), (torch.int64, torch.uint64)
+
+
+def _ptrs(device: int, dtypes, *tensors):
+    """Addresses of contiguous tensors of one of the dtypes on the handle's device (None stays None)."""
     out = []
     for t in tensors:
         if t is None:
             out.append(None)
         elif t.get_device() != device:
             raise ValueError(f"a tensor is on {t.device}, the handle on cuda:{device}")
+        elif t.dtype not in dtypes:
+            raise ValueError(f"a tensor is {t.dtype}, not {dtypes[0]}")
         elif t.is_contiguous():
             out.append(t.data_ptr())
         else:
@@ -259,7 +270,7 @@ class KvPath:
                                                _p(row_seq), _p(seq_lens), n, window), "oxi_prefill_attn_paged")
 
     # ---- paged K/V layout held in 8 bits
-    def _q8(self, layout: PagedQ8Layout) -> int:
+    def _layout(self, layout) -> int:
         if layout.device not in (None, self.device):
             raise ValueError("the layout's tensors are not on the handle's device")
         return C.addressof(layout)
@@ -269,61 +280,65 @@ class KvPath:
         """RMSNorm + RoPE of q and k and the quantising append of k and v (oxi_append_q8): row r is token pos_ids[r]
         of table row row_seq[r] (None: of row r).  q_out may be q_in."""
         n = q_in.shape[0] if rows is None else rows
-        ptrs = _ptrs(self.device, q_out, q_in, k_in, v_in, q_norm_w, k_norm_w, cos, sin, pos_ids)
-        _check(self.lib.oxi_append_q8(self.h, self._stream(), *ptrs, self._q8(layout), *_ptrs(self.device, row_seq), n, eps),
-               "oxi_append_q8")
+        ptrs = _ptrs(self.device, _F16, q_out, q_in, k_in, v_in, q_norm_w, k_norm_w, cos, sin)
+        _check(self.lib.oxi_append_q8(self.h, self._stream(), *ptrs, *_ptrs(self.device, _U32, pos_ids), self._layout(layout),
+                                      *_ptrs(self.device, _U32, row_seq), n, eps), "oxi_append_q8")
 
     def decode_attn_q8(self, ctx_out, q, gate, layout: PagedQ8Layout, seq_lens, window: int = 0, sinks: int = 0,
                        batch: int | None = None):
         """Attention of one token per sequence over the 8-bit cache; window 0: every token is visible, otherwise the
         last `window` and the first `sinks` tokens are (oxi_decode_attn_q8)."""
         b = q.shape[0] if batch is None else batch
-        _check(self.lib.oxi_decode_attn_q8(self.h, self._stream(), *_ptrs(self.device, ctx_out, q, gate), self._q8(layout),
-                                           *_ptrs(self.device, seq_lens), b, window, sinks), "oxi_decode_attn_q8")
+        _check(self.lib.oxi_decode_attn_q8(self.h, self._stream(), *_ptrs(self.device, _F16, ctx_out, q, gate), self._layout(layout),
+                                           *_ptrs(self.device, _U32, seq_lens), b, window, sinks), "oxi_decode_attn_q8")
 
     def prefill_attn_q8(self, ctx_out, q, gate, layout: PagedQ8Layout, row_seq, seq_lens, window: int = 0,
                         sinks: int = 0, rows: int | None = None):
         """Attention of the rows of a prefill wave over the 8-bit cache (oxi_prefill_attn_q8)."""
         n = q.shape[0] if rows is None else rows
-        _check(self.lib.oxi_prefill_attn_q8(self.h, self._stream(), *_ptrs(self.device, ctx_out, q, gate), self._q8(layout),
-                                            *_ptrs(self.device, row_seq, seq_lens), n, window, sinks), "oxi_prefill_attn_q8")
+        _check(self.lib.oxi_prefill_attn_q8(self.h, self._stream(), *_ptrs(self.device, _F16, ctx_out, q, gate), self._layout(layout),
+                                            *_ptrs(self.device, _U32, row_seq, seq_lens), n, window, sinks), "oxi_prefill_attn_q8")
 
     # ---- sliding window with sinks (the first tokens stay visible) over the f16 caches
     def decode_attn_sinks(self, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, window: int, sinks: int,
                           batch: int | None = None):
         b = q.shape[0] if batch is None else batch
-        ptrs = _ptrs(self.device, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens)
-        _check(self.lib.oxi_decode_attn_sinks(self.h, self._stream(), *ptrs, b, window, sinks), "oxi_decode_attn_sinks")
+        ptrs = _ptrs(self.device, _F16, ctx_out, q, gate)
+        _check(self.lib.oxi_decode_attn_sinks(self.h, self._stream(), *ptrs, *_ptrs(self.device, _ADDR, k_ptrs, v_ptrs),
+               *_ptrs(self.device, _U32, seq_lens), b, window, sinks), "oxi_decode_attn_sinks")
 
     def decode_attn_paged_sinks(self, ctx_out, q, gate, layout: PagedLayout, seq_lens, window: int, sinks: int,
                                 batch: int | None = None):
         b = q.shape[0] if batch is None else batch
-        _check(self.lib.oxi_decode_attn_paged_sinks(self.h, self._stream(), *_ptrs(self.device, ctx_out, q, gate), C.addressof(layout),
-                                                    *_ptrs(self.device, seq_lens), b, window, sinks), "oxi_decode_attn_paged_sinks")
+        _check(self.lib.oxi_decode_attn_paged_sinks(self.h, self._stream(), *_ptrs(self.device, _F16, ctx_out, q, gate), self._layout(layout),
+                                                    *_ptrs(self.device, _U32, seq_lens), b, window, sinks), "oxi_decode_attn_paged_sinks")
 
     def append_decode_sinks(self, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos, sin, pos_ids, seq_lens,
                             k_ptrs, v_ptrs, window: int, sinks: int, eps: float = 1e-5):
-        ptrs = _ptrs(self.device, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos, sin, pos_ids, seq_lens, k_ptrs, v_ptrs)
-        _check(self.lib.oxi_append_decode_sinks(self.h, self._stream(), *ptrs, q_io.shape[0], window, sinks, eps),
+        ptrs = _ptrs(self.device, _F16, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos, sin)
+        _check(self.lib.oxi_append_decode_sinks(self.h, self._stream(), *ptrs, *_ptrs(self.device, _U32, pos_ids, seq_lens),
+                                                *_ptrs(self.device, _ADDR, k_ptrs, v_ptrs), q_io.shape[0], window, sinks, eps),
                "oxi_append_decode_sinks")
 
     def append_decode_paged_sinks(self, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos, sin, seq_lens,
                                   layout: PagedLayout, window: int, sinks: int, eps: float = 1e-5):
-        ptrs = _ptrs(self.device, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos, sin, seq_lens)
-        _check(self.lib.oxi_append_decode_paged_sinks(self.h, self._stream(), *ptrs, C.addressof(layout), q_io.shape[0],
-                                                      window, sinks, eps), "oxi_append_decode_paged_sinks")
+        ptrs = _ptrs(self.device, _F16, ctx_out, q_io, k_in, v_in, gate, q_norm_w, k_norm_w, cos, sin)
+        _check(self.lib.oxi_append_decode_paged_sinks(self.h, self._stream(), *ptrs, *_ptrs(self.device, _U32, seq_lens),
+                                                      self._layout(layout), q_io.shape[0], window, sinks, eps),
+               "oxi_append_decode_paged_sinks")
 
     def prefill_attn_sinks(self, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, window: int, sinks: int,
                            rows: int | None = None):
         n = q.shape[0] if rows is None else rows
-        ptrs = _ptrs(self.device, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens)
-        _check(self.lib.oxi_prefill_attn_sinks(self.h, self._stream(), *ptrs, n, window, sinks), "oxi_prefill_attn_sinks")
+        ptrs = _ptrs(self.device, _F16, ctx_out, q, gate)
+        _check(self.lib.oxi_prefill_attn_sinks(self.h, self._stream(), *ptrs, *_ptrs(self.device, _ADDR, k_ptrs, v_ptrs),
+               *_ptrs(self.device, _U32, seq_lens), n, window, sinks), "oxi_prefill_attn_sinks")
 
     def prefill_attn_paged_sinks(self, ctx_out, q, gate, layout: PagedLayout, row_seq, seq_lens, window: int, sinks: int,
                                  rows: int | None = None):
         n = q.shape[0] if rows is None else rows
-        _check(self.lib.oxi_prefill_attn_paged_sinks(self.h, self._stream(), *_ptrs(self.device, ctx_out, q, gate), C.addressof(layout),
-                                                     *_ptrs(self.device, row_seq, seq_lens), n, window, sinks),
+        _check(self.lib.oxi_prefill_attn_paged_sinks(self.h, self._stream(), *_ptrs(self.device, _F16, ctx_out, q, gate), self._layout(layout),
+                                                     *_ptrs(self.device, _U32, row_seq, seq_lens), n, window, sinks),
                "oxi_prefill_attn_paged_sinks")
 
     def prefill_attn(self, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, window: int = 0,
