@@ -513,7 +513,7 @@ const uint32_t* oxi_tables_seq_lens(const oxi_step_tables* tables);
  * to exercise that path without faulting or hanging the GPU: it arms the NEXT
  * launch of this handle's decode-attention kernel (which = 0), prefill-attention
  * kernel (which = 1; oxi_prefill_attn only, the armed wave runs unsplit and without
- * a registered slab) or projection GEMM (which = 2: oxi_project_append or
+ * a registered slab; the paged, 8-bit and sink forms leave the arming for it) or projection GEMM (which = 2: oxi_project_append or
  * oxi_linear_forward, whichever kernel the row count selects) so that CTA 0
  * withholds its stage-th pipeline stage (decode and projection: no copy is issued
  * for it; prefill: the K tile is copied but never published) and all waits of that

@@ -473,10 +473,9 @@ int32_t oxi_prefill_attn_paged(oxi_handle* h, void* stream, void* ctx_out, const
     REQ_BATCH(rows, h->max_prefill_rows, "oxi_prefill_attn_paged");
     PagedMap pm;
     if (int32_t rc = paged_map(layout, "oxi_prefill_attn_paged", &pm)) return rc;
-    const WaitFault flt = take_prefill_fault(h);
     OXI_CUDA(launch_prefill_attn((cudaStream_t)stream, ctx_out, q, gate, nullptr, nullptr, seq_lens, rows, window,
                                  h->dws.status, h->num_sms, h->pf_order, h->dws.status + 48, &pm, row_seq,
-                                 &h->pf_split, h->pf_part_keys, nullptr, &flt),
+                                 &h->pf_split, h->pf_part_keys),
              "prefill_attn_paged launch");
     return OXI_OK;
 }
@@ -582,10 +581,9 @@ int32_t oxi_prefill_attn_q8(oxi_handle* h, void* stream, void* ctx_out, const vo
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_prefill_attn_q8");
     Q8Map m;
     if (int32_t rc = paged_q8_map(layout, "oxi_prefill_attn_q8: the layout or one of its pointers is null", &m)) return rc;
-    const WaitFault flt = take_prefill_fault(h);
     OXI_CUDA(launch_prefill_attn((cudaStream_t)stream, ctx_out, q, gate, nullptr, nullptr, seq_lens, rows, window, h->dws.status,
                                  h->num_sms, h->pf_order, h->dws.status + 48, nullptr, row_seq, &h->pf_split, h->pf_part_keys,
-                                 nullptr, &flt, window ? sinks : 0u, h->max_seq_len, &m, layout->format),
+                                 nullptr, nullptr, window ? sinks : 0u, h->max_seq_len, &m, layout->format),
              "prefill_attn_q8 launch");
     return OXI_OK;
 }
@@ -676,10 +674,9 @@ int32_t oxi_prefill_attn_sinks(oxi_handle* h, void* stream, void* ctx_out, const
     REQ_PTR(ctx_out && q && k_ptrs && v_ptrs && seq_lens, "oxi_prefill_attn_sinks");
     REQ_BATCH(rows, h->max_prefill_rows, "oxi_prefill_attn_sinks");
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_prefill_attn_sinks");
-    const WaitFault flt = take_prefill_fault(h);
     OXI_CUDA(launch_prefill_attn((cudaStream_t)stream, ctx_out, q, gate, k_ptrs, v_ptrs, seq_lens, rows, window, h->dws.status,
                                  h->num_sms, h->pf_order, h->dws.status + 48, nullptr, nullptr, &h->pf_split, h->pf_part_keys,
-                                 nullptr, &flt, sinks, h->max_seq_len),
+                                 nullptr, nullptr, sinks, h->max_seq_len),
              "prefill_attn_sinks launch");
     return OXI_OK;
 }
@@ -695,10 +692,9 @@ int32_t oxi_prefill_attn_paged_sinks(oxi_handle* h, void* stream, void* ctx_out,
     REQ_ALIGNED((uintptr_t)ctx_out | (uintptr_t)q, "oxi_prefill_attn_paged_sinks");
     PagedMap pm;
     if (int32_t rc = paged_map(layout, "oxi_prefill_attn_paged_sinks", &pm)) return rc;
-    const WaitFault flt = take_prefill_fault(h);
     OXI_CUDA(launch_prefill_attn((cudaStream_t)stream, ctx_out, q, gate, nullptr, nullptr, seq_lens, rows, window, h->dws.status,
                                  h->num_sms, h->pf_order, h->dws.status + 48, &pm, row_seq, &h->pf_split, h->pf_part_keys, nullptr,
-                                 &flt, sinks, h->max_seq_len),
+                                 nullptr, sinks, h->max_seq_len),
              "prefill_attn_paged_sinks launch");
     return OXI_OK;
 }

@@ -1401,7 +1401,7 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
     const uint32_t nblocks = (rows + pf::BLK - 1) / pf::BLK;
     // the split is for waves that leave SMs idle; larger waves balance by claiming longest first
     // an armed test fault runs the plain instantiation: pointer tables, unsplit, per-thread copies
-    const bool armed = flt.skip_plus1 != 0u && !pm && !sinks;
+    const bool armed = flt.skip_plus1 != 0u;  // only oxi_prefill_attn passes one: pointer tables, no sinks
     bool split = !armed && ws && ws->max_slots != 0u && part_keys != 0u && nblocks * NKV < (uint32_t)num_sms;
     // with sinks or the 8-bit cache: a window so short that two runs in a block have no more tiles than the smallest part is
     // not split (plan and merge cost 3.5 us: 64 rows of one sequence, int8, unsplit / split, window 64: 15 / 18.6 us, 256

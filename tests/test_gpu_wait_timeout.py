@@ -164,3 +164,44 @@ def test_projection_wait_runs_out_and_the_handle_recovers(rows, stage):
     for i in (0, rows // 2, rows - 1):
         assert torch.equal(again.k_cache[i].view(torch.int16), good.k_cache[i].view(torch.int16))
     kv.close()
+
+
+@pytest.mark.parametrize("form", ["paged", "q8", "sinks", "paged_sinks"])
+def test_an_armed_prefill_wait_is_left_for_the_entry_point_that_has_the_hook(form):
+    """The paged, 8-bit and sink forms neither lose a tile nor use the arming up: oxi_prefill_attn after them does."""
+    from oxide_infer_b200 import KvPath, PagedLayout, PagedQ8Layout
+    kv = KvPath(0, max_batch=4, max_seq_len=2048, max_prefill_rows=256)
+    kv.prefill_split_configure(0, 0)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    half = lambda *s: torch.randn(*s, device="cuda", generator=g).half()  # noqa: E731
+    n, length, bs = 128, 1024, 16
+    k, v, q, gate = half(length // bs, bs, NKV, HD), half(length // bs, bs, NKV, HD), half(n, NQ, HD), half(n, NQ)
+    table = torch.arange(length // bs, dtype=torch.int32, device="cuda")[None].contiguous()
+    lens = torch.arange(length - n + 1, length + 1, dtype=torch.int32, device="cuda")
+    seq = torch.zeros(n, dtype=torch.int32, device="cuda")
+    kp, vp = (torch.full((n,), t.data_ptr(), dtype=torch.int64, device="cuda") for t in (k, v))
+    paged = PagedLayout.of(k, v, table, bs)
+    codes = [(t * 16).round().clamp(-127, 127).to(torch.int8) for t in (k, v)]
+    q8 = PagedQ8Layout.of(*codes, *(torch.full((length // bs, NKV), 1 / 16, device="cuda") for _ in range(2)), table)
+
+    def run():
+        ctx = torch.zeros(n, NQ, HD, dtype=torch.float16, device="cuda")
+        if form == "paged":
+            kv.prefill_attn_paged(ctx, q, gate, paged, seq, lens)
+        elif form == "q8":
+            kv.prefill_attn_q8(ctx, q, gate, q8, seq, lens)
+        elif form == "sinks":
+            kv.prefill_attn_sinks(ctx, q, gate, kp, vp, lens, 300, 4)
+        else:
+            kv.prefill_attn_paged_sinks(ctx, q, gate, paged, seq, lens, 300, 4)
+        return ctx
+
+    good = run()
+    assert kv.device_status() == 0
+    kv.arm_wait_fault(1, 2, 1000)
+    assert torch.equal(run().view(torch.int16), good.view(torch.int16))
+    assert kv.device_status() == 0
+    kv.prefill_attn(torch.zeros_like(q), q, gate, kp, vp, lens, 0)
+    assert kv.device_status() == WAIT_TIMEOUT
+    kv.prefill_attn(torch.zeros_like(q), q, gate, kp, vp, lens, 0)
+    assert kv.device_status() == 0
