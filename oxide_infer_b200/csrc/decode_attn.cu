@@ -64,9 +64,6 @@
 #ifndef OXI_DEC_NSTAGE
 #define OXI_DEC_NSTAGE 3
 #endif
-#ifndef OXI_DEC_CHUNK
-#define OXI_DEC_CHUNK 256
-#endif
 #ifndef OXI_DEC_MAXROWS
 #define OXI_DEC_MAXROWS 1024
 #endif
@@ -88,7 +85,7 @@ constexpr int X_BYTES = 512 + 2 * KV_ROW_BYTES;
 constexpr int DESC_BYTES = 48;
 constexpr int Q_OFF = 2 * HALF_BYTES, X_OFF = Q_OFF + Q_BYTES, DESC_OFF = X_OFF + X_BYTES;
 constexpr int STAGE_BYTES = DESC_OFF + DESC_BYTES;
-constexpr int CHUNK = OXI_DEC_CHUNK;            // keys per work item
+constexpr int CHUNK = DECODE_CHUNK;             // keys per work item
 constexpr int N_CONSUMER_WARPS = NKV;           // one per KV head
 constexpr int THREADS = (N_CONSUMER_WARPS + 1) * 32;
 constexpr int MAX_ROWS = OXI_DEC_MAXROWS;       // rows per launch (prefix + length arrays in shared memory)
@@ -241,7 +238,7 @@ decode_attn_kernel(const DecodeParams p) {
         // pages), fetched one item ahead like the row pointers
         uint32_t cpg = 0, cfp = 0;
         // kSinks: lanes 0 .. npa-1 hold the pages of the item's sink groups from page `first_page` on, the lanes
-        // behind them those of its window groups from page `first_page_w` on (3 / 2 CHUNK / 16 + 2 pages at most)
+        // behind them those of its window groups from page `first_page_w` on (DECODE_PAGES at most)
         uint32_t cfw = 0, cna = 0;
         // A page whose table entry is not a block reads block 0.  Fused: bit l of `bad` - the page of lane l is such a page;
         // the token being appended is not written there, and its key is read like the page's other keys (as after

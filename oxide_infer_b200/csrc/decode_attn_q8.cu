@@ -49,9 +49,10 @@ constexpr int Q_OFF = V_OFF + NGROUP * VPITCH;
 constexpr int Q_BYTES = NQ * HD * 2;
 constexpr int DESC_OFF = Q_OFF + Q_BYTES;         // 48 bytes: row / range / flags, visible bits, page slots of the groups
 constexpr int STAGE_BYTES = DESC_OFF + 64;
-constexpr int CHUNK = 256;                        // keys per work item (the merge's key ranges)
+constexpr int CHUNK = DECODE_CHUNK;               // keys per work item (the merge's key ranges)
 constexpr uint32_t CHUNK_G = CHUNK / GK;
-constexpr int PAGES = 28;                         // pages of an item: at most 3 / 2 CHUNK / 16 + 2
+constexpr int PAGES = 28;                         // pages of an item
+static_assert(PAGES >= DECODE_PAGES, "the scales of an item's pages fit its table");
 constexpr int NTABLE = 4;                         // items whose scales are in shared memory
 constexpr int TABLE_BYTES = PAGES * 32;           // per page: 4 K scales, 4 V scales
 constexpr int N_CONSUMER_WARPS = NKV;

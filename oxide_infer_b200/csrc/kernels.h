@@ -8,6 +8,17 @@
 
 namespace oxi {
 
+// Keys per work item (key range) of the decode kernels, f16 and 8-bit: the workspace holds a partial result for each and the
+// merge counts them, so all of them go by this one.
+#ifndef OXI_DEC_CHUNK
+#define OXI_DEC_CHUNK 256
+#endif
+constexpr int DECODE_CHUNK = OXI_DEC_CHUNK;
+// An item of up to one and a half ranges (RowView::ranges) has at most this many pages of >= 16 tokens: two parts, each of which may
+// begin or end inside a page.  Lane l of a producer warp holds page l.
+constexpr int DECODE_PAGES = 3 * DECODE_CHUNK / 32 + 2;
+static_assert(DECODE_CHUNK % 64 == 0 && DECODE_PAGES <= 32, "a work item is a whole number of 64-key stages whose pages fit a warp");
+
 struct DecodeWorkspace {
     float* partial_acc;     // [max_batch][max_chunks][16][128]
     float* partial_stats;   // [max_batch][max_chunks][16][2]  (running max in log2 units, sum)
