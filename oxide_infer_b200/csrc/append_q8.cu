@@ -154,7 +154,8 @@ append_q8_step_kernel(const AppendQ8Params p) {
         if (!is_v) norm_rope_pairs(x, wv, cv, sv, p.eps);
         if (__any_sync(0xffffffffu, make_finite(x)) && lane == 0) atomicOr(p.status, DEV_NONFINITE);
         const float scale = fmaxf(q8_scale<kFmt>(warp_max(abs_max(x))), old_scale);
-        store_codes<kFmt>(head_codes(combo) + (size_t)slot * Q8_ROW_BYTES, lane, x, q8_inverse<kFmt>(scale));
+        // bounds build: the token's slot lies in a block of the pool
+        if (OXI_IN_BOUNDS(id < p.map.num_blocks && slot >> lbs == 0u, p.status)) store_codes<kFmt>(head_codes(combo) + (size_t)slot * Q8_ROW_BYTES, lane, x, q8_inverse<kFmt>(scale));
         if (lane == 0) {
             *scale_at = scale;
             if (slot != 0u && scale > old_scale) {
@@ -181,8 +182,12 @@ append_q8_step_kernel(const AppendQ8Params p) {
             w[k] = __ldcg(at[k]);
         }
 #pragma unroll
-        for (uint32_t k = 0; k < 4u; k++)
-            if (u0 + k * (NQ + COMBOS) < units) *at[k] = q8_moved<kFmt>(w[k], ratio[k]);
+        for (uint32_t k = 0; k < 4u; k++) {
+            const uint32_t u = u0 + k * (NQ + COMBOS);
+            // bounds build: the slot is one before the token's of a head whose scale grew, the block one of the pool
+            if (u < units && OXI_IN_BOUNDS(u / slot < (uint32_t)__popc(grown) && slot >> lbs == 0u && id < p.map.num_blocks, p.status))
+                *at[k] = q8_moved<kFmt>(w[k], ratio[k]);
+        }
     }
 }
 
@@ -478,6 +483,7 @@ append_q8_wave_kernel(const AppendQ8Params p) {
         uint32_t* at[4];
         uint32_t v[4];
         float ratio[4];
+        bool inside[4];  // bounds build: the slot lies before its segment, and the segment's block in the pool
 #pragma unroll
         for (uint32_t k = 0; k < 4u; k++) {
             const uint32_t u = min(u0 + k * ROWS, units - 1u);
@@ -485,18 +491,21 @@ append_q8_wave_kernel(const AppendQ8Params p) {
             const int sl = i / COMBOS, c = i % COMBOS;
             ratio[k] = __fdiv_rn(s_old[sl][c], s_scale[sl][c]);
             at[k] = reinterpret_cast<uint32_t*>(head_codes(sl, c) + (size_t)(u - s_units[i]) * Q8_ROW_BYTES) + lane;
-            v[k] = __ldcg(at[k]);
+            inside[k] = OXI_IN_BOUNDS(i < (uint32_t)(ROWS * COMBOS) && u - s_units[i] < (s_pos[sl] & (bs - 1u)) && s_id[sl] < p.map.num_blocks, p.status);
+            if (inside[k]) v[k] = __ldcg(at[k]);
         }
 #pragma unroll
         for (uint32_t k = 0; k < 4u; k++)
-            if (u0 + k * ROWS < units) *at[k] = q8_moved<kFmt>(v[k], ratio[k]);
+            if (u0 + k * ROWS < units && inside[k]) *at[k] = q8_moved<kFmt>(v[k], ratio[k]);
     }
     const int li = there ? s_lead[w] : -1;
     if (li >= 0 && usable(li)) {
 #pragma unroll
         for (int k = 0; k < NP; k++) {
             const int c = combo_of(pair0 + k);
-            store_dims<kFmt>(head_codes(li, c) + (size_t)(pos & (bs - 1u)) * Q8_ROW_BYTES, j, x[k], q8_inverse<kFmt>(s_scale[li][c]));
+            // bounds build: the row is the wave's, its block in the pool and its segment's
+            if (OXI_IN_BOUNDS(row < p.rows && s_id[li] < p.map.num_blocks && pos >> lbs == s_pos[li] >> lbs, p.status))
+                store_dims<kFmt>(head_codes(li, c) + (size_t)(pos & (bs - 1u)) * Q8_ROW_BYTES, j, x[k], q8_inverse<kFmt>(s_scale[li][c]));
         }
     }
     if (tail != 0u && usable(last)) {
@@ -508,7 +517,10 @@ append_q8_wave_kernel(const AppendQ8Params p) {
             for (uint32_t t = w; t < tail; t += ROWS) {
                 float v[8];
                 tail_row(t, pair0 + k, v);
-                store_dims<kFmt>(head_codes(last, c) + (size_t)((s_pos[ROWS - 1] + 1u + t) & (bs - 1u)) * Q8_ROW_BYTES, j, v, inv);
+                // bounds build: the row is the wave's and lies in the block of the window's last row
+                if (OXI_IN_BOUNDS(row0 + ROWS + t < p.rows && s_id[last] < p.map.num_blocks &&
+                                      (s_pos[ROWS - 1] + 1u + t) >> lbs == s_pos[last] >> lbs, p.status))
+                    store_dims<kFmt>(head_codes(last, c) + (size_t)((s_pos[ROWS - 1] + 1u + t) & (bs - 1u)) * Q8_ROW_BYTES, j, v, inv);
             }
         }
     }

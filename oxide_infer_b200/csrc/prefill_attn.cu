@@ -1020,6 +1020,12 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             const uint32_t kbeg = tl.first_key(tile), t = kbeg + 16 * b;
             const uint32_t pid = __shfl_sync(0xffffffffu, pages, ((t >> pm.lbs) - (kbeg >> pm.lbs)) & 31u);
             const char* src = base + (uint64_t)pid * pm.block_stride + (uint64_t)((t & ((1u << pm.lbs) - 1u)) + rr) * ROWB;
+            // bounds build: the group's block is one of the pool
+            if (!OXI_IN_BOUNDS(pid < pm.num_blocks && (t & ((1u << pm.lbs) - 1u)) + 16u <= 1u << pm.lbs, status)) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) d[b][k] = make_uint4(0u, 0u, 0u, 0u);
+                return;
+            }
             if (kbeg >= run.lo && kbeg + TK <= run.hi) {
 #pragma unroll
                 for (int k = 0; k < 4; k++) d[b][k] = __ldcg(reinterpret_cast<const uint4*>(src + k * 4 * ROWB));
@@ -1179,11 +1185,13 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                     for (int b = 0; b < 4; b++) {
                         const uint32_t t = kbeg + 16 * b;
                         const uint32_t pid = pages.block(pm, t);
+                        // bounds build: the 16 tokens lie in a block of the pool
+                        const bool placed = OXI_IN_BOUNDS(pid < pm.num_blocks && (t & mask) + 16u <= mask + 1u, status);
                         const char* g = base + (size_t)pid * pm.block_stride + (size_t)((t & mask) + r0) * KV_ROW_BYTES + c * 16;
 #pragma unroll
                         for (int k = 0; k < 8; k++) {
                             const uint32_t row = 16 * b + r0 + 2 * k;
-                            const bool valid = all || seen(kbeg + row);
+                            const bool valid = (all || seen(kbeg + row)) && placed;
                             cp_async_16(dst + row * ROW_B + (((c & 7u) ^ (row & 7u)) << 4), valid ? g + k * 2 * KV_ROW_BYTES : base, valid);
                         }
                     }
