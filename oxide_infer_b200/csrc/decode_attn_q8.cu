@@ -6,7 +6,7 @@
 //   w_t = 2^(x_t log2e + log2 vs_t - m)   is the weight of vc_t in the numerator (m: running maximum of the exponent,
 //                                         so w stays below 2^9 whatever the scales are),
 //   sum_t w_t / vs_t                      is the denominator in the same units: one multiplication per thread and stage.
-// A V scale below 2^-100 counts as 2^-100 (its codes then weigh nothing against any other block's).
+// A V scale below 2^-40 counts as 2^-40 (Q8_V_SCALE_MIN_LOG2).
 //
 // Work decomposition, claiming, merge and failure paths are those of decode_attn.cu: items are fixed ranges of
 // CHUNK keys of the row's own view (a row's arithmetic does not depend on the batch), 148 persistent CTAs claim
@@ -391,7 +391,7 @@ decode_attn_q8_kernel(const DecodeQ8Params p) {
             if (vis == 0u) ks = vs = 0.0f;  // no group: its scales are not in the table
         }
         const float xs = ks * X_SCALE;
-        const float lv = fmaxf(__log2f(vs), -100.0f), ivs = exp2f(-lv);
+        const float lv = fmaxf(__log2f(vs), Q8_V_SCALE_MIN_LOG2), ivs = exp2f(-lv);
 
         // ---- S^T: tile i holds tokens 4i and 4i + 1 of the 4 groups in rows 0-7 and tokens 4i + 2 and 4i + 3 in rows 8-15
         // (the four tiles side by side: their accumulations are independent)

@@ -1077,7 +1077,7 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
                 if (more) request(b, pages);
             }
             if (is_k) {
-                const float l2 = fminf(fmaxf(__log2f(scale), -100.0f), 100.0f);  // finite even for the scale of a block without visible keys
+                const float l2 = fminf(fmaxf(__log2f(scale), Q8_V_SCALE_MIN_LOG2), 100.0f);  // finite even for the scale of a block without visible keys
                 if (lane < 4) s_scl[g % SCL][0][lane] = fmaxf(scale * QK_SCALE_LOG2, 1.0e-30f);  // a masked score stays -inf under a zero scale
                 else if (lane < 8) {
                     s_scl[g % SCL][1][lane - 4] = l2;

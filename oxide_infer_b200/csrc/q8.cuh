@@ -6,6 +6,13 @@
 
 namespace oxi {
 
+// V scales enter the exponents of the softmax as their log2 and leave the row sum as 1 / scale; a smaller scale, that of a block of
+// zeros for one, counts as 2^-40.  Its values stay below 448 * 2^-40 < 2^-31, which an f16 result does not show (the smallest
+// f16 has a scale of 2^-32), and the weights of its tokens, which the row sum needs, do not fall out of f32: with 2^-100 in its
+// place a token of a zero block beside values of 3e4 got the weight 0 from e^-12 of the largest on, and 4,095 of them were
+// missing from a row's sum (1 % of it).
+constexpr float Q8_V_SCALE_MIN_LOG2 = -40.0f;
+
 // The scale of a block whose largest magnitude is amax.  int8: amax / 127.  e4m3: the power of two s with
 // amax / s in (224, 448], so that moving stored codes to a larger scale only changes their exponents.
 template <uint32_t kFmt>
