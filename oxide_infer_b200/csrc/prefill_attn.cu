@@ -121,6 +121,7 @@ struct PfView {
     const float* v_scales;
     uint64_t scale_stride;
     uint32_t table_rows;   // 8-bit cache: rows of the block tables
+    uint32_t shares;       // without a plan: CTAs that share an item by its runs
 };
 // The 64-key tiles of a run whose rows' windows start at `wlo` or later and whose tokens end at hi: nst tiles of
 // sinks from token 0, then tiles from token lo on.  Tiles of paged caches start at a multiple of 16 tokens, so
@@ -494,7 +495,9 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
 
     // Claims the next item and prepares its tables in buffer `buf`; run by all lanes of the K loader warp
     // while the other roles finish the current item (before the loop for the first item).
-    // kSinks with order == nullptr (no plan kernel ran): at most one item per CTA, its index is the CTA's.
+    // kSinks with order == nullptr (no plan kernel ran): at most one item per CTA, that of blockIdx.x.  Where the wave leaves SMs idle
+    // several CTAs share an item by its runs (run r is that of the CTA with blockIdx.y = r mod shares), whose rows nobody else
+    // writes: nothing to merge, and the rows of 64 sequences in one block are not 64 runs in series.
     bool first_item = true;
     auto prepare_item = [&](uint32_t buf) {
         uint32_t item = 0xffffffffu;  // kFault: a CTA one of whose waits gave up claims nothing more, the others take its share
@@ -574,6 +577,10 @@ prefill_attn_kernel(uint16_t* __restrict__ ctx_out, const uint16_t* __restrict__
             const uint32_t rr = (uint32_t)lane + 32u * hf;
             if (rr < nrows) {
                 const uint32_t id = (uint32_t)__popcll(starts & (~0ull >> (63u - rr))) - 1u;  // runs that start at or before rr
+                if (kSinks && !kSplit && view.shares > 1u && id % view.shares != blockIdx.y) {  // another CTA's row: skipped here
+                    sl[hf] = ws[hf] = 0u;
+                    s_len[buf][rr] = 0u;
+                }
                 if (sl[hf] != 0u) {
                     atomicMin(&s_runs[buf][id][2], ws[hf]);
                     atomicMax(&s_runs[buf][id][3], sl[hf]);
@@ -1386,7 +1393,7 @@ static cudaError_t launch_pf(cudaStream_t stream, uint32_t grid, void* ctx_out, 
                              const uint32_t* row_seq, const PfSplit& sp, const PrefillSlab& slab, const WaitFault& fault,
                              const PfView& view) {
     // programmatic dependent of the plan kernel: TMEM allocation and barrier set-up overlap it
-    return launch_pdl(prefill_attn_kernel<kPaged, kSplit, kTma, kFault, kSinks, kFmt>, dim3(grid), dim3(pf_threads(kFmt)),
+    return launch_pdl(prefill_attn_kernel<kPaged, kSplit, kTma, kFault, kSinks, kFmt>, dim3(grid, view.shares), dim3(pf_threads(kFmt)),
                       pf::SMEM_BYTES, stream,
                       (uint16_t*)ctx_out, (const uint16_t*)q, (const uint16_t*)gate, k_ptrs, v_ptrs, seq_lens, rows,
                       window, status, (const uint32_t*)order, counter, pm, row_seq, sp, slab.map, slab.base, slab.rows, fault, view);
@@ -1399,7 +1406,7 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
                                 const PagedMap* pm, const uint32_t* row_seq, const PrefillSplitWs* ws,
                                 uint32_t part_keys, const PrefillSlab* slab, const WaitFault* fault, uint32_t sinks,
                                 uint32_t max_seq_len, const Q8Map* q8, uint32_t format) {
-    const PfView view{sinks, max_seq_len, q8 ? q8->k_scales : nullptr, q8 ? q8->v_scales : nullptr, q8 ? q8->scale_stride : 0, q8 ? q8->table_rows : 0};
+    PfView view{sinks, max_seq_len, q8 ? q8->k_scales : nullptr, q8 ? q8->v_scales : nullptr, q8 ? q8->scale_stride : 0, q8 ? q8->table_rows : 0, 1u};
     PagedMap q8pm{};
     if (q8) {
         q8pm = PagedMap{q8->k_pool, q8->v_pool, q8->block_tables, q8->block_stride, q8->max_blocks, q8->lbs, q8->num_blocks};
@@ -1411,16 +1418,22 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
     // an armed test fault runs the plain instantiation: pointer tables, unsplit, per-thread copies
     const bool armed = flt.skip_plus1 != 0u;  // only oxi_prefill_attn passes one: pointer tables, no sinks
     bool split = !armed && ws && ws->max_slots != 0u && part_keys != 0u && nblocks * NKV < (uint32_t)num_sms;
-    // with sinks or the 8-bit cache: a window so short that two runs in a block have no more tiles than the smallest part is
-    // not split (plan and merge cost 3.5 us: 64 rows of one sequence, int8, unsplit / split, window 64: 15 / 18.6 us, 256
-    // 19.2 / 21.2, 512 24.1 / 21.8, 1,024 33.8 / 23.1; blocks of up to three runs, window 100, 70 sinks: 36.8 / 26.3), ...
+    // With sinks or the 8-bit cache a wave of at most one item per SM needs no order (no plan kernel), and the SMs that it leaves
+    // idle share its items by their runs (64 rows of 64 sequences, window 64, f16 / int8: 228 / 392 us with one CTA for all runs of a
+    // block, 21 / 25 shared).  What is left for the key-range split is a run that is long by itself, under a window so wide that it
+    // pays for plan and merge (which grow with the blocks: three quarters of a tile for each), on SMs that are idle.  Unsplit against
+    // split, us, f16 and int8, one run a block: 64 rows, window 256: 17 : 20 and 21 : 22, 512: 21 : 22 and 26 : 23, 1,024: 28 : 23 and
+    // 36 : 26; 576 rows, 512: 21 : 25 and 27 : 27, 768: 25 : 27 and 32 : 28, 1,024: 28 : 28 and 37 : 30; 2,048 rows, 1,024: 30 : 41 and
+    // 37 : 48.  The host does not know the number of runs: with more of them the shares win longer (576 rows, four runs a block,
+    // 512: 27 : 39 and 29 : 42, 1,024: 41 : 55 and 43 : 59).
     const bool view_variant = sinks || q8;
-    if (view_variant && window && window <= (1u << 22) &&
-        2u * ((window + pf::BLK - 1u + 15u + pf::TK - 1u) / pf::TK + ((sinks < (1u << 22) ? sinks : 1u << 22) + pf::TK - 1u) / pf::TK) <=
-            (part_keys + pf::TK - 1u) / pf::TK)
-        split = false;
-    // ... and a wave of at most one item per SM needs no order: no plan kernel
-    const bool direct = view_variant && !split && nblocks * NKV <= (uint32_t)num_sms;
+    const uint32_t shares = nblocks * NKV <= (uint32_t)num_sms ? (uint32_t)num_sms / (nblocks * NKV) : 0u;
+    if (view_variant && window && window <= (1u << 22)) {
+        const uint32_t run_tiles = (window + pf::BLK - 1u + 15u + pf::TK - 1u) / pf::TK + ((sinks < (1u << 22) ? sinks : 1u << 22) + pf::TK - 1u) / pf::TK;
+        if (run_tiles <= (part_keys + pf::TK - 1u) / pf::TK + 3u * nblocks / 4u) split = false;
+    }
+    const bool direct = view_variant && !split && shares != 0u;
+    if (direct) view.shares = shares < (uint32_t)pf::BLK ? shares : (uint32_t)pf::BLK;
     PfSplit sp{};
     sp.by_runs = view_variant;  // (the plain entry points keep their parts, on which the bytes of a split wave depend)
     if (split) {
