@@ -832,9 +832,18 @@ static dim3 merge_grid(const DecodeWorkspace& ws, uint32_t batch) {
     return dim3(batch * NKV, y);
 }
 
+// Most key ranges that a row has under p's window (the handle's longest row without one).
+template <int kRule>
+static uint32_t merge_ranges(const DecodeWorkspace& ws, const DecodeParams& p) {
+    if (p.window == 0u || p.window > (1u << 22) || p.sinks > (1u << 22)) return ws.max_chunks;
+    constexpr uint32_t G = kRule == MERGE_SINKS ? (uint32_t)dec::GK : kRule == MERGE_Q8 ? 16u : 1u, per = (uint32_t)dec::CHUNK / G;
+    const uint32_t groups = (p.sinks + G - 1u) / G + (p.window + G - 1u) / G + (G > 1u ? 1u : 0u);
+    return min(ws.max_chunks, (groups + per - 1u) / per);
+}
+
 template <int kRule>
 static cudaError_t launch_merge(cudaStream_t stream, const DecodeWorkspace& ws, uint32_t batch, const DecodeParams& p) {
-    if (ws.merge_acc) return launch_pdl(decode_merge_kernel<true, kRule>, merge_grid(ws, batch), dim3(128), 0, stream, p);
+    if (ws.merge_acc && merge_ranges<kRule>(ws, p) > (uint32_t)MERGE_BLK) return launch_pdl(decode_merge_kernel<true, kRule>, merge_grid(ws, batch), dim3(128), 0, stream, p);
     return launch_pdl(decode_merge_kernel<false, kRule>, dim3(batch * NKV), dim3(128), 0, stream, p);
 }
 
