@@ -130,6 +130,16 @@ def _scale_of(amax, fmt):
     return torch.where(amax > 0, torch.ldexp(torch.ones_like(amax), torch.where(m > 0.5, e, e - 1)), torch.zeros_like(amax))
 
 
+_kept = []
+
+
+def _handle(oxi):
+    """The process's one handle (a KvPath is one per device), with the limits of all cases."""
+    if not _kept:
+        _kept.append(oxi.KvPath(0, max_batch=128, max_seq_len=32768, max_prefill_rows=4096))
+    return _kept[0]
+
+
 def prepare(case, seed):
     dev = "cuda"
     g = torch.Generator(device=dev).manual_seed(int(seed) * 7919 + 13)
@@ -186,7 +196,7 @@ def prepare(case, seed):
         s["v_ptrs"] = s["vp"].data_ptr() + off[s["row_seq"].long()] * (NKV * HD * 2)
     if own:
         import oxide_infer_b200 as oxi
-        s["kv"] = oxi.KvPath(0, max_batch=n, max_seq_len=s["lmax"] + 1, max_prefill_rows=total if op != "decode" else 0)
+        s["kv"] = _handle(oxi)
         if op in ("append", "decode", "prefill"):
             s["layout"] = oxi.PagedQ8Layout.of(s["kp"], s["vp"], s["ks"], s["vs"], s["tables"])
         elif paged:
