@@ -166,7 +166,8 @@ int32_t oxi_prefill_attn(oxi_handle* h, void* stream, void* ctx_out, const void*
  * frees the reservation; otherwise min_part_keys >= 256 and slots <= 4096.
  * Synchronises the device; call it with no work of this handle in flight.
  * Applies to oxi_prefill_attn and oxi_prefill_attn_paged, and with a quarter of min_part_keys to oxi_prefill_attn_q8
- * and the _sinks forms. */
+ * and the _sinks forms, unless their window is so short that a wave is done sooner in one piece (about min_part_keys,
+ * more for waves of many rows). */
 #define OXI_PREFILL_SPLIT_DEFAULT_MIN_PART_KEYS 512u
 int32_t oxi_prefill_split_configure(oxi_handle* h, uint32_t min_part_keys, uint32_t slots);
 uint64_t oxi_prefill_split_slot_bytes(void);
@@ -334,8 +335,9 @@ typedef struct oxi_paged_q8_layout {
  * OXI_DEV_BAD_SEQ_LEN and the row is skipped, a block id >= num_blocks sets OXI_DEV_BAD_BLOCK and k / v are not
  * written.  A row that is skipped ends a run.  cos / sin cover the positions of all other rows.  16-byte
  * alignment of all tensors.  rows <= max(max_batch, max_prefill_rows); with row_seq NULL rows <= table_rows.
- * pos_ids, row_seq, seq_lens and block_tables are inputs of the step for this and the next two entry points: they
- * are complete before the kernel that precedes the call in its stream begins (as k_ptrs elsewhere). */
+ * pos_ids, row_seq, seq_lens and block_tables are inputs of the step for this and the next two entry points, and so are
+ * the norm weights, cos and sin here: they are complete before the kernel that precedes the call in its stream begins
+ * (as k_ptrs elsewhere). */
 int32_t oxi_append_q8(oxi_handle* h, void* stream, void* q_out, const void* q_in, const void* k_in, const void* v_in,
                       const void* q_norm_w, const void* k_norm_w, const void* cos_table, const void* sin_table,
                       const uint32_t* pos_ids, const oxi_paged_q8_layout* layout, const uint32_t* row_seq, uint32_t rows,

@@ -103,9 +103,10 @@ __device__ __forceinline__ void store_codes(unsigned char* at, int lane, const f
 }
 
 // Row r is a token of table row r.  grid = rows, a warp for each query head, K head and V head; all of them share the
-// slots to requantise where a scale grew (128 rows: 1.9 us if none grows, 6.4 us if all do in the last slot of blocks of 16,
-// 39 us of blocks of 256; a scale grows with a probability of about 1 / (slot + 1)).  One warp per head for its own slots took
-// 14 to 118 us for that.
+// slots to requantise where a scale grew.  128 rows: 1.8 us if none grows; if all do in the last slot of a block, int8 6.2 us in
+// blocks of 16 and 39 in blocks of 256 (e4m3 5.8 and 34; 67 MB, 10 us of memory time).  In use a head's scale grows with a
+// probability of about 1 / (slot + 1) (int8) or less (e4m3, whose scales are powers of two): on average over the tokens of a block
+// with normally distributed values 3.0 us a step in blocks of 16 and 64 and 4.4 to 4.9 in blocks of 256, e4m3 2.4 to 2.8.
 template <uint32_t kFmt>
 __global__ void __launch_bounds__(aq::STEP_THREADS)
 append_q8_step_kernel(const AppendQ8Params p) {
@@ -538,7 +539,7 @@ static cudaError_t launch_fmt(cudaStream_t stream, const AppendQ8Params& p) {
     // How many CTAs share a window's K and V heads.  More of them give a long segment's rows more warps (rows behind the
     // window are serial work), fewer repeat a window's set-up less often; two CTAs fit an SM.  Measured, us, for 1 / 2 / 4
     // groups: 128 rows in one run, blocks of 16: 4.6 / 3.4 / 2.7, of 256: 27.9 / 19.1 / 10.9; 4,096 rows in runs of 128,
-    // blocks of 16: 13.3 / 16.0 / 22.7, of 64: 23.2 / 18.2 / 22.0, of 256: 40.2 / 28.5 / 23.8.
+    // blocks of 16: 13.3 / 16.0 / 22.7, of 64: 23.2 / 18.2 / 22.0, of 256: 40.2 / 28.5 / 23.8 (between these points nothing was measured).
     if (p.rows <= 1184u || p.map.lbs > 6u) return launch_wave<kFmt, 4>(stream, p);
     return p.map.lbs == 6u ? launch_wave<kFmt, 2>(stream, p) : launch_wave<kFmt, 1>(stream, p);
 }

@@ -1444,8 +1444,7 @@ cudaError_t launch_prefill_attn(cudaStream_t stream, void* ctx_out, const void* 
         sp.part_ml = ws->part + (size_t)ws->max_slots * NKV * 2 * pf::M * HD;
         sp.part_tiles = (part_keys + pf::TK - 1) / pf::TK;
         // The variants' blocks are short (a window) or slow per tile (8 bits), and plan and merge are paid already: a quarter.
-        // Parts of 8 / 5 / 4 / 2 tiles: 585 rows, window 512, e4m3 32.7 / 29.2 / 27.9 / 27.7 us; 6 chunks, window 100, 70
-        // sinks, f16 34.4 / 30.7 / 28.6 / 26.3; 64 rows on 4,096 keys, int8 31.1 / 28.2 / 27.3 / 27.2.
+        // Parts of 8 / 5 / 4 / 2 tiles, 64 rows on 4,096 keys, int8: 31.1 / 28.2 / 27.3 / 27.2 us.
         if (view_variant) sp.part_tiles = (sp.part_tiles + 3u) / 4u;
         sp.max_slots = ws->max_slots;
         sp.target_items = (uint32_t)num_sms;
